@@ -1,0 +1,95 @@
+// Attention of several drafted tokens a request (a tree or a chain; one token: the plain decode step) over a paged cache, bf16 or e4m3.
+//
+//   o_i = sum_j softmax_j(scale q_i k_j) v_j   over the lens[b] cached tokens and those drafted ones whose bit is set in mask[b][i]
+//
+// Node i of a request stands in slot lens[b] + i.  All nodes and all query heads of a kv head are rows of one matrix, row = node * G + head, so that
+// a page is fetched once for all of them.
+//
+// Work is dealt on the device: an item is a (request, tile of rows, kv head), a unit one of its pages; the units of all items, in order, are cut into equal
+// runs, one for each CTA.  Lengths differ as they like, the host knows none of them, and a captured graph serves all.  A CTA writes the rows of an
+// item that lies in its run as a whole; of one that is cut it leaves (accumulators, maximum, sum) for paged_tree_merge_kernel.
+#pragma once
+#include "common.cuh"
+#include <cuda.h>
+
+int ptb_make_tmap_bf16(CUtensorMap* map, const void* base, long long inner, long long outer, long long ld, int box_inner, int box_outer);
+
+namespace ptb {
+namespace tree {
+
+constexpr int PAGE = 64;
+constexpr int MAX_NODES = 64;
+constexpr int MAX_B = 4096;
+
+struct Params {
+    const __nv_bfloat16* q;              // [B, T, q_row] pitches in elements; head h at column h * D
+    long long q_batch, q_row;
+    __nv_bfloat16* out;                  // [B, T, H D]
+    const int* lens;                     // [B] cached tokens before the drafted ones
+    const int* nodes;                    // [B] or null: T
+    const unsigned long long* mask;      // [B, T] or null: a chain (node i sees 0 .. i)
+    const int* page_table;
+    int pt_stride, n_pages;
+    const uint8_t* k_exp;                // [n_pages, Hk, 64] biased exponents, null: bf16 pages
+    const uint8_t* v_exp;
+    float* work;                         // partials of cut items
+    int B, T, H, Hk, G;
+    int tile_rows, tiles;                // rows of a tile, tiles of T nodes
+    int ctas;
+    float scale_log2;
+    int* status;
+};
+
+__host__ __device__ constexpr size_t partial_floats(int rows, int D) { return (size_t)rows * (D + 2); }
+
+__device__ __forceinline__ int nodes_of(const Params& P, int b) { return P.nodes ? max(0, min(P.nodes[b], P.T)) : P.T; }
+__device__ __forceinline__ int cached_of(const Params& P, int b, int n) { return max(0, min(P.lens[b], P.pt_stride * PAGE - n)); }
+
+// What a request asks for: tiles with rows, pages of an item.
+struct Req { int nodes, len, tiles, pages; };
+__device__ __forceinline__ Req req_of(const Params& P, int b) {
+    Req r;
+    r.nodes = nodes_of(P, b);
+    r.len = cached_of(P, b, r.nodes);
+    r.tiles = (r.nodes * P.G + P.tile_rows - 1) / P.tile_rows;
+    r.pages = (r.len + r.nodes + PAGE - 1) / PAGE;
+    return r;
+}
+__device__ __forceinline__ int units_of(const Params& P, const Req& r) { return r.tiles * P.Hk * r.pages; }
+
+// starts[b]: units before request b (starts[B]: all).  The block's N threads, with `part` of N / 32 ints.
+template <int N>
+__device__ __forceinline__ void plan(const Params& P, int* starts, int* part) {
+    int carry = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int b0 = 0; b0 < P.B; b0 += N) {
+        const int b = b0 + (int)threadIdx.x;
+        int u = b < P.B ? units_of(P, req_of(P, b)) : 0, upto = u;
+        if (b < P.B && P.status && (P.lens[b] < 0 || P.lens[b] > P.pt_stride * PAGE - nodes_of(P, b))) atomicExch(P.status, PTB_ERR_BOUNDS);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) part[warp] = upto;
+        __syncthreads();
+        int before = carry, all = carry;
+        for (int w = 0; w < N / 32; ++w) {
+            if (w == warp) before = all;
+            all += part[w];
+        }
+        if (b < P.B) starts[b + 1] = before + upto;
+        if (b == 0) starts[0] = 0;
+        carry = all;
+        __syncthreads();
+    }
+}
+
+// The run of units of a CTA: `per` each.
+__device__ __forceinline__ int units_per_cta(int all, int ctas) { return max(1, (all + ctas - 1) / ctas); }
+
+// Partials: a CTA leaves at most two, of the item its run begins in (slot 0) and of the one it ends in (slot 1; where both are the same item, slot 0).
+__device__ __forceinline__ size_t partial_at(const Params& P, int cta, int slot, int D) { return ((size_t)cta * 2 + slot) * partial_floats(P.tile_rows, D); }
+
+}  // namespace tree
+}  // namespace ptb

@@ -298,6 +298,26 @@ long long ptb_paged_attn_work_floats(int B, int H, int D, int nsplit);
 // One new token per request attends to its pages.  q: [B, q_stride] bf16; out: [B, H D] bf16; lens: [B].
 int ptb_paged_attn_decode(const void* q, long long q_stride, void* out, int B, int H, int Hk, int D, const int* lens, const int* page_table, int pt_stride, int n_pages, const void* k_pages, const void* v_pages, float scale, float* work, int nsplit, int* status, cudaStream_t st);
 
+// ---------------------------------------------------------------------------- paged_tree.cu
+// Floats of workspace that ptb_paged_attn_tree needs.
+long long ptb_paged_tree_work_floats(int T, int H, int Hk, int D);
+
+// T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with
+// pitches in elements, head h at column h * D; out [B, T, H D]; lens [B]: cached tokens before the drafted ones, node i stands in slot lens[b] + i; nodes [B]
+// (null: T), rows behind them come out as zeros, as do rows that see nothing; mask [B, T]: bit j, whether the node sees node j (null: a chain).  Pages
+// [n_pages, Hk, 64, D]: bf16, or e4m3 with exponents [n_pages, Hk, 64].  D is 64 or 128, T at most 64, B at most 4096.
+int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_row, void* out, int B, int T, int H, int Hk, int D, const int* lens, const int* nodes, const void* mask, const int* page_table, int pt_stride, int n_pages, const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, float scale, float* work, int* status, cudaStream_t st);
+
+// ---------------------------------------------------------------------------- paged_write.cu
+// Rotate q and k of `n` tokens (pairs (j, j + D/2)); q goes to q_out [n, H D], k and v to the page slots of (req, slot), slot null: the position, negative: not
+// stored.  qkv: [n, ld] bf16; cos / sin: [max_pos, D/2] fp32; k_out optional [n, Hk, D]: the rotated keys.  k_exp and v_exp null: bf16 pages
+// [n_pages, Hk, 64, D]; else e4m3 pages with one biased exponent byte for a token's keys (values) of a head.  D is 64 or 128.  Slots are distinct.
+int ptb_paged_write(const void* qkv, long long ld, int n, int H, int Hk, int D, const int* pos, const int* slot, const int* req, const int* page_table, int pt_stride, int pt_rows, int n_pages, const float* cos, const float* sin, int max_pos, void* q_out, void* k_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, int* status, cudaStream_t st);
+
+// The cache entries of each request's accepted drafted tokens, moved from slot lens[b] + path[b][j] to lens[b] + j for j in 1 .. count[b], in every
+// layer.  pools: [layers][4] device pointers (keys, values, their exponents or null), row: bytes of a token's keys of a head; path [B, T] ascends.
+int ptb_paged_keep(void* const* pools, int layers, int B, int T, int Hk, int row, int n_pages, const int* lens, const int* path, const int* count, const int* page_table, int pt_stride, int* status, cudaStream_t st);
+
 // ---------------------------------------------------------------------------- prompt_layers.cu
 // Floats of workspace that ptb_prompt_layers needs (T, H, heads, kv_heads, D, I and n_sm of the run are read).
 long long ptb_prompt_work_floats(const PtbPromptRun* r);

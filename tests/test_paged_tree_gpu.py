@@ -1,0 +1,403 @@
+"""Drafted tokens over the paged cache on the GPU: writing (plain and quantised), attention of trees, moving the accepted entries, against plain forms."""
+import math
+
+import pytest
+import torch
+
+from prometorch_b200.ops import paged as P
+from prometorch_b200.ops import paged_tree as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+PAGE = P.PAGE
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def pools(g, n, Hk, D, kind, v_scale=None):
+    """A pool of random keys and values: (k, v, k exponents, v exponents)."""
+    k, v = (torch.randn(n, Hk, PAGE, D, device=DEV, generator=g) for _ in range(2))
+    if v_scale is not None:
+        v = v * v_scale
+    if kind == "bf16":
+        return k.bfloat16(), v.bfloat16(), None, None
+    (k, ke), (v, ve) = R.quantise_rows(k), R.quantise_rows(v)
+    return k, v, ke, ve
+
+
+def table_for(lens, seed):
+    need = [-(-n // PAGE) for n in lens]
+    n = sum(need) + 2
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(seed)).int()
+    table, at = torch.zeros(len(lens), max(need) + 1, dtype=torch.int32), 0
+    for b, k in enumerate(need):
+        table[b, :k] = order[at:at + k]
+        at += k
+    return table.to(DEV), n
+
+
+def spoil(pool, exps, table, lens, value):
+    """What lies behind a request's last token is anything at all."""
+    for b, n in enumerate(lens):
+        if n % PAGE:
+            page = int(table[b, n // PAGE])
+            if exps is None:
+                pool[page, :, n % PAGE:] = value
+            else:
+                pool.view(torch.uint8)[page, :, n % PAGE:] = 0x7f
+                exps[page, :, n % PAGE:] = 255
+
+
+def oracle(q, H, Hk, D, lens, nodes, mask, table, k, v, ke, ve, scale):
+    """In fp64: the attention, and the same weights on the values' magnitudes."""
+    B, T = q.shape[:2]
+    out, mag = (torch.zeros(B, T, H * D, dtype=torch.float64, device=DEV) for _ in range(2))
+    for b in range(B):
+        n, t = lens[b], nodes[b]
+        if t == 0:
+            continue
+        ids = table[b, :-(-(n + t) // PAGE)].long()
+
+        def flat(pool, exps):
+            x = pool.view(torch.uint8)[ids].view(R.E4M3).double() if exps is not None else pool[ids].double()
+            if exps is not None:
+                x = x * torch.exp2(exps[ids].double() - 127)[..., None]
+            return x.permute(1, 0, 2, 3).reshape(Hk, -1, D)[:, :n + t]
+        kk, vv = flat(k, ke), flat(v, ve)
+        sees = torch.zeros(t, n + t, dtype=torch.bool, device=DEV)
+        sees[:, :n] = True
+        for i in range(t):
+            for j in range(t):
+                sees[i, n + j] = bool(int(mask[b, i]) >> j & 1) if mask is not None else j <= i
+        qq = q[b, :t, :H * D].double().view(t, Hk, H // Hk, D).permute(1, 0, 2, 3)                       # [Hk, t, G, D]
+        x = torch.einsum("ktgd,knd->ktgn", qq, kk) * scale
+        x = x.masked_fill(~sees[None, :, None], -math.inf)
+        w = torch.nan_to_num(torch.softmax(x, -1), nan=0.0) * sees[None, :, None]
+        vz = torch.where(sees.any(0)[None, :, None], vv, torch.zeros_like(vv))
+        out[b, :t] = torch.einsum("ktgn,knd->tkgd", w, vz).reshape(t, H * D)
+        mag[b, :t] = torch.einsum("ktgn,knd->tkgd", w, vz.abs()).reshape(t, H * D)
+    return out, mag
+
+
+def close(got, want, mag, kind):
+    """One rounding of the result to bf16 (2^-8 of it); each weight rounded to the operands' type (2^-8 of it in bf16, 2^-11 in fp16), which moves the result by at most that
+    share of the weighted magnitudes; fp32 scores (128 products of up to about 9 in all: 128 * 9 * 2^-24 < 2^-13) and exponentials (2^-21), once each in numerator and sum."""
+    bound = 2 ** -8 * want.abs() + (2 ** -8 if kind == "bf16" else 2 ** -11) * mag + 2 ** -11 * mag + 1e-30
+    worst = ((got.double() - want).abs() / bound).max()
+    assert torch.isfinite(got).all()
+    assert float(worst) <= 1.0, float(worst)
+
+
+def random_masks(g, B, T):
+    """Any bits at all, and rows without any."""
+    m = torch.randint(-2 ** 63, 2 ** 63 - 1, (B, T), generator=torch.Generator().manual_seed(g), dtype=torch.int64)
+    m[0, 0] = 0
+    if T > 3:
+        m[B - 1, 3] = 0
+    return m
+
+
+LENS = [0, 1, 59, 63, 64, 65, 300, 1000]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hk,T", [(2, 2, 1), (8, 2, 1), (8, 1, 2), (6, 2, 5), (2, 1, 9), (8, 2, 8), (14, 2, 7), (3, 3, 17), (8, 2, 16), (4, 2, 64), (16, 2, 33)])
+def test_trees(kind, D, H, Hk, T):
+    """Every tile height and more rows than one tile holds; any masks, rows that see nothing, requests without nodes, without cached tokens, around page borders."""
+    g = gen(H * 1000 + T)
+    nodes = [T, max(T // 2, 1), T, T, 0, T, 1, T]
+    totals = [n + T for n in LENS]
+    table, n_pages = table_for(totals, T)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    behind = [n + t for n, t in zip(LENS, nodes)]
+    spoil(k, ke, table, behind, math.nan)
+    spoil(v, ve, table, behind, math.inf)
+    mask = random_masks(T, len(LENS), T)
+    q = torch.randn(len(LENS), T, H * D, device=DEV, generator=g).bfloat16()
+    lens = torch.tensor(LENS, dtype=torch.int32, device=DEV)
+    nd = torch.tensor(nodes, dtype=torch.int32, device=DEV)
+    for m in (mask.to(DEV), None):
+        got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, mask=m, nodes=nd, k_exp=ke, v_exp=ve)
+        want, mag = oracle(q, H, Hk, D, LENS, nodes, m, table, k, v, ke, ve, D ** -0.5)
+        P.check_status(DEV)
+        close(got, want, mag, kind)
+        for b, t in enumerate(nodes):
+            assert not got[b, t:].any()
+    assert not R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, mask=mask.to(DEV), nodes=nd, k_exp=ke, v_exp=ve)[0, 0].any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_node_is_the_decode_step(kind, D):
+    """A whole batch of single tokens, lengths one after another: every place of the last token in a page."""
+    H, Hk, B = 8, 2, 200
+    g = gen(D)
+    have = list(range(B))
+    table, n_pages = table_for([n + 1 for n in have], 3)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    q = torch.randn(B, 1, H * D, device=DEV, generator=g).bfloat16()
+    got = R.paged_attention_tree(q, H, Hk, D, torch.arange(B, dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve, scale=0.2)
+    want, mag = oracle(q, H, Hk, D, have, [1] * B, None, table, k, v, ke, ve, 0.2)
+    close(got, want, mag, kind)
+    if kind == "bf16":
+        old = P.paged_attention_decode(q[:, 0], H, Hk, D, torch.arange(1, B + 1, dtype=torch.int32, device=DEV), table, k, v, scale=0.2)
+        close(got[:, 0], old.double(), mag[:, 0] * 2, kind)
+
+
+@pytest.mark.parametrize("kind,D,H,Hk,T,lens", [("e4m3", 128, 8, 2, 3, [20011]), ("bf16", 64, 8, 2, 64, [9000, 40]), ("bf16", 128, 2, 1, 1, [5, 30000, 700]), ("e4m3", 64, 4, 1, 20, [64 * 150, 64 * 150 - 20])])
+def test_items_cut_between_ctas(kind, D, H, Hk, T, lens):
+    g = gen(T)
+    table, n_pages = table_for([n + T for n in lens], 5)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    q = torch.randn(len(lens), T, H * D, device=DEV, generator=g).bfloat16()
+    got = R.paged_attention_tree(q, H, Hk, D, torch.tensor(lens, dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, lens, [T] * len(lens), None, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
+    again = R.paged_attention_tree(q, H, Hk, D, torch.tensor(lens, dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("T,G", [(6, 1), (8, 4), (40, 8)])
+def test_no_number_in_a_masked_place(kind, T, G):
+    """A drafted token whose keys and values are no numbers reaches the rows that see it and no other."""
+    D, Hk, len0 = 64, 2, 77
+    H, bad = Hk * G, T // 2
+    g = gen(T)
+    table, n_pages = table_for([len0 + T], 1)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    q = torch.randn(1, T, H * D, device=DEV, generator=g).bfloat16()
+    at = len0 + bad
+    page = int(table[0, at // PAGE])
+    for pool, value in ((k, math.nan), (v, math.inf)):
+        if kind == "bf16":
+            pool[page, :, at % PAGE] = value
+        else:
+            pool.view(torch.uint8)[page, :, at % PAGE] = 0x7f
+    full = torch.tensor([[sum(1 << j for j in range(T) if j != bad)] * T], dtype=torch.int64, device=DEV)
+    lens = torch.tensor([len0], dtype=torch.int32, device=DEV)
+    got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, mask=full, k_exp=ke, v_exp=ve)
+    kz, vz = k.clone(), v.clone()
+    for pool in (kz, vz):
+        R._as_bytes(pool)[page, :, at % PAGE] = 0
+    want, mag = oracle(q, H, Hk, D, [len0], [T], full, table, kz, vz, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
+    full[0, 1] |= 1 << bad
+    got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, mask=full, k_exp=ke, v_exp=ve)
+    assert bool(torch.isnan(got[0, 1]).all())
+    rest = [i for i in range(T) if i != 1]
+    close(got[:, rest], want[:, rest], mag[:, rest], kind)
+
+
+@pytest.mark.parametrize("T", [1, 12, 48])
+def test_exponents_far_apart(T):
+    """Values of very different sizes, keys that are zero, values that are zero where most of the weight lies."""
+    D, H, Hk, n = 128, 4, 2, 500
+    g = gen(T)
+    table, n_pages = table_for([n + T], 1)
+    s = torch.exp2(torch.randint(-30, 31, (n_pages, Hk, PAGE, 1), device=DEV, generator=g).float())
+    k, v, ke, ve = pools(g, n_pages, Hk, D, "e4m3", v_scale=s)
+    first = int(table[0, 0])
+    k.view(torch.uint8)[first, :, :3], v.view(torch.uint8)[first, :, 5:9] = 0, 0
+    ke[first, :, :3], ve[first, :, 5:9] = 63, 63
+    q = torch.randn(1, T, H * D, device=DEV, generator=g).bfloat16() * 3
+    q[0, 0, :D] = 0
+    got = R.paged_attention_tree(q, H, Hk, D, torch.tensor([n], dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, [n], [T], None, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, "bf16")           # scores three times as large: 2^-8 in place of 2^-11 covers 3 * 2^-13 with room
+
+
+def test_rows_between_pieces_other_streams_and_graphs():
+    D, H, Hk, T, n = 64, 4, 2, 5, 130
+    g = gen(1)
+    table, n_pages = table_for([n + T] * 2, 1)
+    k, v, _, _ = pools(g, n_pages, Hk, D, "bf16")
+    lens = torch.tensor([n, n - 9], dtype=torch.int32, device=DEV)
+    wide = torch.randn(2, T, H * D + 24, device=DEV, generator=g).bfloat16()
+    call = lambda q: R.paged_attention_tree(q, H, Hk, D, lens, table, k, v)  # noqa: E731
+    want = call(wide[..., 8:8 + H * D].contiguous())
+    for q in (wide[..., 8:], wide[..., 3:3 + H * D].contiguous()[..., :]):
+        if q.shape[2] == wide.shape[2] - 8:
+            assert torch.equal(call(q), want)
+    odd = torch.randn(2, T, H * D + 3, device=DEV, generator=g).bfloat16()
+    assert torch.equal(call(odd[..., 1:1 + H * D]), call(odd[..., 1:1 + H * D].contiguous()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call(wide[..., 8:8 + H * D].contiguous())
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    # two graphs over the same operands, replayed one after the other: neither disturbs the other's workspace; lengths may change between replays
+    q = wide[..., 8:8 + H * D].contiguous()
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(call(q))
+        graphs.append(gr)
+    for gr in graphs:
+        gr.replay()
+    assert all(torch.equal(o, want) for o in outs)
+    lens.copy_(torch.tensor([3, 100], dtype=torch.int32))
+    for gr in graphs:
+        gr.replay()
+    want = call(q)
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_bad_pages_are_skipped_and_reported():
+    """An id outside the pool, a length beyond the table: nothing is read there, the rest is as if those tokens were not."""
+    D, H, Hk, T = 64, 2, 1, 2
+    g = gen(2)
+    table, n_pages = table_for([200], 1)
+    k, v, _, _ = pools(g, n_pages, Hk, D, "bf16")
+    q = torch.randn(1, T, H * D, device=DEV, generator=g).bfloat16()
+    lens = torch.tensor([190], dtype=torch.int32, device=DEV)
+    bad = table.clone()
+    bad[0, 1] = n_pages
+    got = R.paged_attention_tree(q, H, Hk, D, lens, bad, k, v)
+    with pytest.raises(IndexError):
+        P.check_status(DEV)
+    kept = [0, 2, 3]
+    # without the second page: the same tokens, 64 fewer in front of the drafted ones
+    want, mag = oracle(q, H, Hk, D, [190 - 64], [T], None, table[:, kept].contiguous(), k, v, None, None, D ** -0.5)
+    want2, mag2 = want, mag
+    # the drafted tokens stand at slots 190 and 191: the last page's place is the same
+    close(got, want2, mag2, "bf16")
+    R.paged_attention_tree(q, H, Hk, D, torch.tensor([table.shape[1] * PAGE], dtype=torch.int32, device=DEV), table, k, v)
+    with pytest.raises(IndexError):
+        P.check_status(DEV)
+    P.check_status(DEV)
+
+
+# ---------------------------------------------------------------------------------------------- writing
+def same(a, b):
+    """Equal bytes, NaN codes of either sign counted as one."""
+    if a.dtype == R.E4M3:
+        x, y = a.float(), b.float()
+        return torch.equal(torch.isnan(x), torch.isnan(y)) and torch.equal(torch.nan_to_num(x), torch.nan_to_num(y))
+    return torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("H,Hk,D", [(32, 4, 64), (32, 8, 128), (3, 3, 64), (5, 1, 128), (40, 40, 128)])
+@pytest.mark.parametrize("n,slots", [(1, False), (7, True), (130, False), (515, True)])
+def test_write(kind, H, Hk, D, n, slots):
+    """Bit for bit what the plain form gives: rotation rounded operation by operation, one rounding to the page's type; padding rows are not stored."""
+    g = gen(n + H)
+    req = torch.arange(n, dtype=torch.int32) % 5
+    slot = (torch.arange(n, dtype=torch.int32) // 5)
+    table = torch.randperm(5 * (n // 5 // PAGE + 1), generator=torch.Generator().manual_seed(n)).int().view(5, -1)
+    pos = (slot // 2 + 3) if slots else slot
+    ang = torch.arange(1, n + 10, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+    cos, sin = ang.cos().float(), ang.sin().float()
+    if slots:
+        slot[::4] = -1
+    wide = torch.randn(n, (H + 2 * Hk) * D + 8, device=DEV, generator=g).bfloat16()
+    pool = [torch.zeros(table.numel(), Hk, PAGE, D).bfloat16().to(R.E4M3 if kind == "e4m3" else torch.bfloat16) for _ in range(2)]
+    exps = [torch.full((table.numel(), Hk, PAGE), 9, dtype=torch.uint8) if kind == "e4m3" else None for _ in range(2)]
+    on = lambda t: t.to(DEV) if t is not None else None  # noqa: E731
+    gpu = [on(t) for t in pool + exps]
+    args = (H, Hk, D)
+    for qkv in (wide, wide[:, :-8].contiguous()):
+        q, k = R.paged_write(qkv, *args, on(pos), on(req), on(table), on(cos), on(sin), gpu[0], gpu[1], slot=on(slot) if slots else None, k_exp=gpu[2], v_exp=gpu[3], want_k=True)
+        qc, kc = R.paged_write(qkv.cpu(), *args, pos, req, table, cos, sin, pool[0], pool[1], slot=slot if slots else None, k_exp=exps[0], v_exp=exps[1], want_k=True)
+        P.check_status(DEV)
+        assert torch.equal(q.cpu(), qc) and torch.equal(k.cpu(), kc)
+        for a, b in zip(gpu, pool + exps):
+            if a is not None:
+                assert same(a.cpu(), b)
+
+
+def test_write_of_values_that_are_no_numbers_and_of_any_size():
+    D, H, Hk = 128, 2, 2
+    rows = torch.randn(12, (H + 2 * Hk) * D, generator=torch.Generator().manual_seed(0))
+    rows[0] = 0
+    rows[1, ::7] = math.inf
+    rows[2, 3::9] = -math.inf
+    rows[3, ::5] = math.nan
+    rows[4] *= 2.0 ** 100
+    rows[5] *= 2.0 ** -100
+    rows[6, :] = 448.0
+    rows[7, :] = 449.0
+    rows[8] = math.nan
+    rows[9, 100:] = 0
+    rows[10] *= torch.exp2(torch.arange(rows.shape[1]) % 40 - 20.0)
+    rows = rows.bfloat16()
+    n = rows.shape[0]
+    pos = torch.zeros(n, dtype=torch.int32)
+    slot, req, table = torch.arange(n, dtype=torch.int32), torch.zeros(n, dtype=torch.int32), torch.tensor([[1, 0]], dtype=torch.int32)
+    cos, sin = torch.ones(1, D // 2), torch.zeros(1, D // 2)
+    pool = [torch.zeros(2, Hk, PAGE, D).to(R.E4M3) for _ in range(2)]
+    exps = [torch.zeros(2, Hk, PAGE, dtype=torch.uint8) for _ in range(2)]
+    gpu = [t.to(DEV) for t in pool + exps]
+    R.paged_write(rows.to(DEV), H, Hk, D, pos.to(DEV), req.to(DEV), table.to(DEV), cos.to(DEV), sin.to(DEV), gpu[0], gpu[1], slot=slot.to(DEV), k_exp=gpu[2], v_exp=gpu[3])
+    R.paged_write(rows, H, Hk, D, pos, req, table, cos, sin, pool[0], pool[1], slot=slot, k_exp=exps[0], v_exp=exps[1])
+    v = pool[1][1, :, :n].float()
+    back = R.dequantise_rows(pool[1], exps[1])[1, :, :n]
+    true = rows.view(n, H + 2 * Hk, D)[:, H + Hk:].transpose(0, 1).float()
+    fine = torch.isfinite(true) & (true.abs() < 448 * 2.0 ** 64) & (true.abs() >= back.abs().amax(-1, keepdim=True).nan_to_num(0) * 2.0 ** -14)
+    fine[:, [1, 2, 3, 8]] &= torch.isfinite(true[:, [1, 2, 3, 8]])
+    assert torch.equal(torch.isnan(v), ~torch.isfinite(true))
+    small = true.abs() < 2.0 ** -64
+    assert bool(((back - true).abs() <= 2.0 ** -4 * true.abs())[fine & ~small].all())
+    for a, b in zip(gpu, pool + exps):
+        assert same(a.cpu(), b)
+
+
+def test_write_reports_slots_outside():
+    D, H, Hk = 64, 1, 1
+    qkv = torch.randn(3, 3 * D, device=DEV).bfloat16()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    k, v, _, _ = pools(gen(0), 2, Hk, D, "bf16")
+    before = k.clone()
+    cos = torch.ones(4, D // 2, device=DEV)
+    for pos, slot, req, table in ((i32(0, 1, 2), i32(-1, 128, -1), i32(0, 0, 0), i32(0, 1)), (i32(0, 1, 2), i32(-1, 3, -1), i32(0, 0, 0), i32(7, 1)), (i32(0, 4, 2), i32(-1, 3, -1), i32(0, 0, 0), i32(0, 1)),
+                                  (i32(0, 1, 2), i32(-1, 3, -1), i32(0, 5, 0), i32(0, 1))):
+        R.paged_write(qkv, H, Hk, D, pos, req, table[None], cos, torch.zeros_like(cos), k, v, slot=slot)
+        with pytest.raises(IndexError):
+            P.check_status(DEV)
+        assert torch.equal(k, before)
+
+
+# ---------------------------------------------------------------------------------------------- keeping
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("layers,B,T,Hk,D", [(1, 1, 2, 1, 64), (3, 5, 64, 2, 128), (35, 4, 19, 8, 64), (70, 2, 9, 3, 128)])
+def test_keep(kind, layers, B, T, Hk, D):
+    """Paths within a page and across borders, whole chains (nothing moves), requests without nodes; more layers than one launch takes."""
+    lens = torch.tensor([(60 * b + 61) % 200 for b in range(B)], dtype=torch.int32)
+    table, n_pages = table_for([int(n) + T for n in lens], T)
+    stacks = [pools(gen(l), n_pages, Hk, D, kind) for l in range(layers)]
+    h = torch.Generator().manual_seed(T)
+    path, count = torch.full((B, T), -1, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+    for b in range(B):
+        on = torch.rand(T, generator=h) < (0.5 if b != 1 else 1.1)
+        on[0] = True
+        ids = on.nonzero().flatten().int()
+        path[b, :len(ids)], count[b] = ids, len(ids) - 1
+    if B > 2:
+        count[2], path[2] = -1, -1
+    host = [[t.cpu() if t is not None else None for t in s] for s in stacks]
+    give = (lambda s: s) if kind == "e4m3" else (lambda s: s[:2])
+    R.paged_keep([give(s) for s in stacks], lens.to(DEV), path.to(DEV), count.to(DEV), table)
+    R.paged_keep([give(s) for s in host], lens, path, count, table.cpu())
+    P.check_status(DEV)
+    for s, t in zip(stacks, host):
+        for a, b in zip(s, t):
+            if a is not None:
+                assert torch.equal(R._as_bytes(a).cpu(), R._as_bytes(b))
+
+
+def test_keep_reports_bad_pages_and_paths():
+    k, v, _, _ = pools(gen(0), 3, 1, 64, "bf16")
+    before = k.clone()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    for table, path in (([[0, 9]], [[0, 40]]), ([[0, 1]], [[0, 0]]), ([[0, 1]], [[0, 2]])):
+        R.paged_keep([(k, v)], i32([40]), i32(path), i32([1]), i32(table))
+        with pytest.raises(IndexError):
+            P.check_status(DEV)
+        assert torch.equal(k, before)
