@@ -468,6 +468,15 @@ int ptb_scale_unless_one(void* x, long long n, const float* g, int bf16, cudaStr
 
 int ptb_rmsnorm_bwd_static(const void* x, const void* w, const void* dy, const float* rstd, void* dx, void* dw, int n_ctas, long long rows, int H, const void* dresid, int bf16, cudaStream_t st);
 
+// ---------------------------------------------------------------------------- verify.cu
+// Bytes of workspace that ptb_verify_drafts needs.
+long long ptb_verify_work_bytes(int B, int T, int V);
+
+// Which drafted tokens of B requests stay.  logits [B, T, V] (bf16 or fp32; pitches of a request and of a row in elements), tokens, parents (null: a chain) and u [B, T], nodes [B] (null: T),
+// probs (null, or the draft's probabilities [B, T, V] fp32, row i what node i's child was drawn from; chains only), temperature [B].  Writes path [B, T] (accepted nodes, -1 behind),
+// count [B] (accepted drafted tokens; -1 for a request without nodes) and out [B, T] (their tokens, then the drawn one, -1 behind).
+int ptb_verify_drafts(const void* logits, int bf16, long long l_batch, long long l_row, const float* probs, long long p_batch, long long p_row, const int* tokens, const int* parents, const int* nodes, const float* u, const float* temperature, void* work, int* path, int* count, int* out, int B, int T, int V, cudaStream_t st);
+
 // ---------------------------------------------------------------------------- window_attn.cu
 // After the packed projection x [n, *] (pitch ld; q, k and v rows at the three columns): q_out [n, H, Dp] = q / rms(q) * qw over all H D
 // columns together; k, normed over its G D columns with kw, and v go to the page slot of (req, pos).  Dp, Dvp: sizes as stored,
