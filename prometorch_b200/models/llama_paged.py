@@ -10,6 +10,7 @@ import torch
 import torch.nn.functional as F
 
 from ..ops import paged as P
+from ..ops.paged_tree import paged_attention_tree, paged_write
 from .paged import PagedModel, PromptBatch, register_model
 
 
@@ -127,6 +128,12 @@ class LlamaWeights:
 
 class PagedLlama(PagedModel):
     architecture = "llama"
+    quantises = True
+    trees = True
+
+    @staticmethod
+    def takes_trees(cfg, device, dtype) -> bool:
+        return torch.device(device).type != "cuda" or (dtype == torch.bfloat16 and cfg.head_dim in (64, 128))
 
     def __init__(self, weights: LlamaWeights, device, dtype):
         super().__init__(weights, device, dtype)
@@ -167,9 +174,14 @@ class PagedLlama(PagedModel):
         h = self._norm(x, w.layers[0]["attn_norm"]) if w.layers else self._norm(x, w.final_norm)
         for l, L in enumerate(w.layers):
             qkv = self._linear(h, L["wqkv"]).contiguous()
-            k = P.paged_rope_write(qkv, H, Hk, Dh, batch.pos, batch.req, page_table, self.cos, self.sin, kv.k[l], kv.v[l], want_k=True)
             heads = qkv.view(-1, H + 2 * Hk, Dh)
-            a = flash_attention_varlen(heads[:, :H], k, heads[:, H + Hk:], batch.offs, offs).reshape(-1, H * Dh)
+            if kv.quantised:                               # the prompt itself attends to its keys and values as they were
+                q, k = paged_write(qkv, H, Hk, Dh, batch.pos, batch.req, page_table, self.cos, self.sin, kv.k[l], kv.v[l], k_exp=kv.k_exp[l], v_exp=kv.v_exp[l], want_k=True)
+                q = q.view(-1, H, Dh)
+            else:
+                k = P.paged_rope_write(qkv, H, Hk, Dh, batch.pos, batch.req, page_table, self.cos, self.sin, kv.k[l], kv.v[l], want_k=True)
+                q = heads[:, :H]
+            a = flash_attention_varlen(q, k, heads[:, H + Hk:], batch.offs, offs).reshape(-1, H * Dh)
             h, x = add_rms_norm(self._linear(a, L["wo"]), x, L["ffn_norm"], c.rms_norm_eps)
             nxt = w.layers[l + 1]["attn_norm"] if l + 1 < len(w.layers) else w.final_norm
             h, x = add_rms_norm(self._mlp(h, L), x, nxt, c.rms_norm_eps)
@@ -187,14 +199,37 @@ class PagedLlama(PagedModel):
         req = torch.arange(B, dtype=torch.int32, device=meta.device)
         x = w.tok_emb[ids]
         h = self._norm(x, w.layers[0]["attn_norm"])
+        before = lens - 1                                 # tokens in the cache without the new one
         for l, L in enumerate(w.layers):
-            q = P.qkv_rope_write(h, L["wqkv"], H, Hk, Dh, pos, req, table, self.cos, self.sin, kv.k[l], kv.v[l],
-                                 fuse_sum=True)
-            a = P.paged_attention_decode(q, H, Hk, Dh, lens, table, kv.k[l], kv.v[l], nsplit=nsplit)
+            if kv.quantised:
+                q, _ = paged_write(self._linear(h, L["wqkv"]), H, Hk, Dh, pos, req, table, self.cos, self.sin, kv.k[l], kv.v[l], k_exp=kv.k_exp[l], v_exp=kv.v_exp[l])
+                a = paged_attention_tree(q.view(B, 1, H * Dh), H, Hk, Dh, before, table, kv.k[l], kv.v[l], k_exp=kv.k_exp[l], v_exp=kv.v_exp[l]).view(B, H * Dh)
+            else:
+                q = P.qkv_rope_write(h, L["wqkv"], H, Hk, Dh, pos, req, table, self.cos, self.sin, kv.k[l], kv.v[l],
+                                     fuse_sum=True)
+                a = P.paged_attention_decode(q, H, Hk, Dh, lens, table, kv.k[l], kv.v[l], nsplit=nsplit)
             h, x = linear_add_rms_norm(a, L["wo"], x, L["ffn_norm"], c.rms_norm_eps)
             nxt = w.layers[l + 1]["attn_norm"] if l + 1 < len(w.layers) else w.final_norm
             h, x = linear_add_rms_norm(linear_swiglu(h, L["w_gate_up"]), L["w_down"], x, nxt, c.rms_norm_eps)
         return self._linear(h, w.lm_head).float()
+
+    def tree_pass(self, kv, table, ids, pos, slot, lens, nodes, mask) -> torch.Tensor:
+        from ..ops.gemm import linear_add_rms_norm, linear_swiglu
+        c, w = self.cfg, self.weights
+        H, Hk, Dh = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+        B, T = ids.shape
+        req = torch.arange(B, dtype=torch.int32, device=ids.device).repeat_interleave(T)
+        pos, slot = pos.reshape(-1), slot.reshape(-1)
+        x = w.tok_emb[ids.reshape(-1).long()]
+        h = self._norm(x, w.layers[0]["attn_norm"]) if w.layers else self._norm(x, w.final_norm)
+        for l, L in enumerate(w.layers):
+            cache = dict(k_exp=kv.k_exp[l], v_exp=kv.v_exp[l])
+            q, _ = paged_write(self._linear(h, L["wqkv"]), H, Hk, Dh, pos, req, table, self.cos, self.sin, kv.k[l], kv.v[l], slot=slot, **cache)
+            a = paged_attention_tree(q.view(B, T, H * Dh), H, Hk, Dh, lens, table, kv.k[l], kv.v[l], mask=mask, nodes=nodes, **cache).view(B * T, H * Dh)
+            h, x = linear_add_rms_norm(a, L["wo"], x, L["ffn_norm"], c.rms_norm_eps)
+            nxt = w.layers[l + 1]["attn_norm"] if l + 1 < len(w.layers) else w.final_norm
+            h, x = linear_add_rms_norm(linear_swiglu(h, L["w_gate_up"]), L["w_down"], x, nxt, c.rms_norm_eps)
+        return self._linear(h, w.lm_head).float().view(B, T, -1)
 
 
 register_model(LlamaConfig, LlamaWeights, PagedLlama, "llama", "LlamaForCausalLM", "LlamaModel")

@@ -65,6 +65,8 @@ class PagedModel:
     architecture = ""
     continues_prompts = False          # whether a prompt pass may start behind cached tokens
     rewinds = True                     # whether a decoded token can be taken back by decoding another one at its position
+    quantises = False                  # whether its passes run over e4m3 pages
+    trees = False                      # whether it has a tree_pass
 
     def __init__(self, weights, device, dtype):
         self.cfg = weights.cfg
@@ -88,6 +90,16 @@ class PagedModel:
         """How many of the latest tokens any layer can still read (None: all of them).  Pages that lie behind go back to the
         pool while the sequence runs."""
         return None
+
+    @staticmethod
+    def takes_trees(cfg, device, dtype) -> bool:
+        """Whether the kernels behind ``quantises`` and ``trees`` take this configuration's heads and type on this device."""
+        return False
+
+    def tree_pass(self, kv, table: torch.Tensor, ids: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor, lens: torch.Tensor, nodes: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
+        """Several drafted tokens of each of B requests (``ids``, ``pos``, ``slot [B, T]`` int32; slot -1: padding) behind ``lens [B]`` cached ones, node i in slot lens + i; ``nodes [B]`` of them
+        are there; ``mask [B, T]``: bit j, whether a node sees node j; ``table``: a row of pages for each request.  Logits ``[B, T, V]``."""
+        raise NotImplementedError
 
     def pick_splits(self, rows: int, max_len: int) -> int:
         """Split count of the decode pass's attention (part of the key of its CUDA graph)."""

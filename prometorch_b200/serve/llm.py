@@ -30,6 +30,7 @@ import torch
 from ..models.llama_paged import LlamaConfig, LlamaWeights  # noqa: F401
 from ..models.paged import PagedModel, PromptBatch, entry_of, read_config, resolve_architecture
 from ..ops import paged as P
+from ..ops.paged_tree import E4M3, MAX_NODES
 
 PAGE = P.PAGE
 
@@ -109,12 +110,20 @@ class PagedKVCache:
         (shape, dtype) of what a sequence carries besides its pages; ``slots`` of each are held."""
         n = max_pages + (1 if spare else 0)                # the spare page (id max_pages) is never handed out
         shapes = shapes if shapes is not None else [(num_kv_heads, head_dim, head_dim)] * num_layers
-        self.k = [torch.zeros(n, hk, PAGE, dk, device=device, dtype=dtype) for hk, dk, _ in shapes]
-        self.v = [torch.zeros(n, hk, PAGE, dv, device=device, dtype=dtype) for hk, _, dv in shapes]
+        self.quantised = dtype == E4M3
+        empty = (lambda *d: torch.zeros(*d, device=device, dtype=torch.uint8).view(E4M3)) if self.quantised else (lambda *d: torch.zeros(*d, device=device, dtype=dtype))
+        self.k = [empty(n, hk, PAGE, dk) for hk, dk, _ in shapes]
+        self.v = [empty(n, hk, PAGE, dv) for hk, _, dv in shapes]
+        # e4m3 pages: an exponent for a token's keys and one for its values of every head (ops/paged_tree.py)
+        self.k_exp, self.v_exp = ([torch.zeros(n, hk, PAGE, device=device, dtype=torch.uint8) if self.quantised else None for hk, _, _ in shapes] for _ in range(2))
         self.state = [{k: torch.zeros((slots,) + tuple(shape), device=device, dtype=dt) for k, (shape, dt) in d.items()} for d in states or [{}] * len(shapes)]
         self.max_pages = max_pages
         self.spare_page = max_pages if spare else -1
         self.free_pages: Deque[int] = collections.deque(range(max_pages))
+
+    def layers(self) -> List[tuple]:
+        """Every layer's (keys, values, their exponents or None)."""
+        return list(zip(self.k, self.v, self.k_exp, self.v_exp))
 
     @classmethod
     def for_model(cls, model: PagedModel, max_pages: int, device, dtype, slots: int = 1) -> "PagedKVCache":
@@ -158,10 +167,18 @@ class LLMEngine:
     new ones), ``poll_responses`` hands back what finished."""
 
     def __init__(self, device=None, max_pages: int = 1024, max_active: int = 8, dtype=None, seed: int = 0, use_graphs: bool = True,
-                 spec_tokens: int = 0):
+                 spec_tokens: int = 0, spec_branches: int = 0, kv_dtype=None):
+        """``spec_tokens``: ids drafted for a request and pass by an n-gram look-up.  ``spec_branches``: 0 verifies one continuation, a batch row for each id (greedy
+        requests); 1 or more verifies a tree of up to that many continuations in one attention over the cache, and sampled requests speculate as well (models with
+        ``trees``).  ``kv_dtype``: what the pages hold: None, the compute type; ``"e4m3"`` (or the torch type), quantised on the way in (models with ``quantises``)."""
         self.device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
         self.dtype = dtype if dtype is not None else (torch.bfloat16 if self.device.type == "cuda" else torch.float32)
         self.max_pages, self.max_active = max_pages, max_active
+        if kv_dtype not in (None, "e4m3", E4M3, self.dtype):
+            raise ValueError(f"kv_dtype: None, 'e4m3' or the compute type, not {kv_dtype!r}")
+        self.kv_dtype = E4M3 if kv_dtype in ("e4m3", E4M3) else self.dtype
+        if not 0 <= spec_branches <= 3 or (spec_branches and not 1 <= spec_tokens < MAX_NODES):
+            raise ValueError(f"spec_branches: up to 3 continuations of 1 to {MAX_NODES - 1} drafted ids in all, not {spec_branches} of {spec_tokens}")
         self.cfg = None
         self.model: Optional[PagedModel] = None
         self.tokenizer = ByteTokenizer()
@@ -179,7 +196,7 @@ class LLMEngine:
         self._graphs: Dict[tuple, tuple] = {}
         # speculative decoding for greedy requests of models that can take a token back: up to `spec_tokens` ids proposed by an n-gram look-up in the request's
         # own history are verified in the same decode pass (one extra batch row per proposed id)
-        self.spec_tokens = spec_tokens
+        self.spec_tokens, self.spec_branches = spec_tokens, spec_branches
         self.max_prompt_tokens = 16384           # tokens of new requests that share one prompt pass
         self.spec_drafted = self.spec_accepted = 0
 
@@ -204,9 +221,14 @@ class LLMEngine:
 
     def set_weights(self, w):
         self.cfg = w.cfg
-        self.model = entry_of(w.cfg).model(w, self.device, self.dtype)
+        model = entry_of(w.cfg).model
+        if self.kv_dtype == E4M3 and not (model.quantises and model.takes_trees(w.cfg, self.device, self.dtype)):
+            raise ValueError(f"{model.architecture or model.__name__}: no quantised pages for this model on {self.device.type}")
+        if self.spec_branches and not (model.trees and model.takes_trees(w.cfg, self.device, self.dtype)):
+            raise ValueError(f"{model.architecture or model.__name__}: no trees of drafted ids for this model on {self.device.type}")
+        self.model = model(w, self.device, self.dtype)
         c = self.cfg
-        self.kv = PagedKVCache.for_model(self.model, self.max_pages, self.device, self.dtype, self.max_active + 1)
+        self.kv = PagedKVCache.for_model(self.model, self.max_pages, self.device, self.kv_dtype, self.max_active + 1)
         self.pt_stride = (c.max_position_embeddings + PAGE - 1) // PAGE
         # one row (and one state slot) per active request plus a spare one whose single page absorbs the writes of padding rows
         self.page_table = torch.zeros(self.max_active + 1, self.pt_stride, dtype=torch.int32, device=self.device)
@@ -372,7 +394,9 @@ class LLMEngine:
                 s.prefill_done = True
                 self._emit(s, self._sample([s], logits[i:i + 1])[0])
         running = [s for s in running if self._ensure_pages(s, s.kv_position) or self._finish(s)]
-        if running and self.spec_tokens > 0 and self.model.rewinds:
+        if running and self.spec_branches > 0:
+            self._step_tree(running)
+        elif running and self.spec_tokens > 0 and self.model.rewinds:
             self._step_speculative(running)
         elif running:                                          # one batched decode pass for everyone else
             logits = self._forward_decode(running)
@@ -393,6 +417,11 @@ class LLMEngine:
         history and propose the ids that followed it (the reference drafts the same way on the CPU,
         torch/io/speculative_draft.h).  The request keeps an index from n-gram to the position after its latest
         occurrence, extended by the ids that arrived since the last call, so a look-up costs O(new ids)."""
+        found = self._continuations(s, k)
+        return found[0] if found else []
+
+    def _continuations(self, s: RequestState, k: int) -> List[List[int]]:
+        """The ids that followed the latest earlier occurrence of the last 3, of the last 2 and of the last id, up to k each, as far as there is one."""
         hist = s.prompt_ids + s.output_ids if s.ngram_hist is None else s.ngram_hist
         if s.ngram_hist is None:
             s.ngram_hist, s.ngram_index, s.ngram_done = hist, {}, 0
@@ -404,12 +433,137 @@ class LLMEngine:
                 if q + 1 >= n:
                     s.ngram_index[tuple(hist[q + 1 - n:q + 1])] = q + 1
         s.ngram_done = max(s.ngram_done, L - 1)
+        found = []
         for n in (3, 2, 1):
             if L > n:
                 at = s.ngram_index.get(tuple(hist[L - n:]))
                 if at is not None:
-                    return hist[at:at + k]
-        return []
+                    found.append(hist[at:at + k])
+        return found
+
+    def _draft_tree(self, s: RequestState, budget: int) -> tuple:
+        """(ids, parents) of up to ``budget`` drafted nodes behind node 0, the latest id: the continuations' common beginnings shared, level by level, so that each
+        continuation gets its share of the budget."""
+        lines = self._continuations(s, budget)[:self.spec_branches]
+        ids, parents, child, at = [], [], {}, [0] * len(lines)
+        for level in range(budget):
+            for i, line in enumerate(lines):
+                if level >= len(line) or at[i] is None:
+                    continue
+                key = (at[i], line[level])
+                if key not in child:
+                    if len(ids) == budget:
+                        at[i] = None
+                        continue
+                    ids.append(line[level])
+                    parents.append(at[i])
+                    child[key] = len(ids)
+                at[i] = child[key]
+        return ids, parents
+
+    # -------------------------------------------------------------------------------------- trees
+    def _step_tree(self, running: List[RequestState]):
+        """One pass in which a request contributes its latest id and a tree of drafted ones: node i stands in slot kv_position + i of its pages and at the position of its depth, one
+        attention over the cache serves all nodes, and :func:`~prometorch_b200.ops.verify.verify_drafts` walks the tree for greedy and for sampled requests.  The entries of the nodes on the
+        path move to the front.  Requests with a repetition penalty have no distribution before their tokens are known: they go on by one id."""
+        from ..ops.paged_tree import paged_keep, tree_mask
+        from ..ops.verify import verify_drafts
+        T, B, dev = self.spec_tokens + 1, len(running), self.device
+        Bb = 1
+        while Bb < B and dev.type == "cuda" and self.use_graphs:
+            Bb *= 2
+        Bb = max(Bb, B)
+        ids, pos, slot, parents = (torch.full((Bb, T), x, dtype=torch.int32) for x in (0, 0, -1, -1))
+        rows, lens, nodes = torch.full((Bb,), self.max_active, dtype=torch.int32), torch.zeros(Bb, dtype=torch.int32), torch.zeros(Bb, dtype=torch.int32)
+        temperature = torch.zeros(Bb)
+        walked, branched = [], False
+        for b, s in enumerate(running):
+            walk = s.config.repetition_penalty == 1.0
+            room = min(s.config.max_new_tokens - len(s.output_ids) - 1, self.cfg.max_position_embeddings - 2 - s.kv_position)
+            new, up = self._draft_tree(s, min(self.spec_tokens, room)) if walk and room > 0 else ([], [])
+            while new and not self._ensure_pages(s, s.kv_position + len(new)):
+                new.pop(), up.pop()
+            n = 1 + len(new)
+            depth = [0]
+            for p in up:
+                depth.append(depth[p] + 1)
+            ids[b, :n] = torch.tensor([s.input_ids[-1]] + new)
+            pos[b, :n] = torch.tensor(depth) + s.kv_position
+            slot[b, :n] = torch.arange(n) + s.kv_position
+            parents[b, 1:n] = torch.tensor(up)
+            rows[b], lens[b], nodes[b] = s.row, s.kv_position, n
+            temperature[b] = max(s.config.temperature, 0.0) if walk else 0.0
+            walked.append(walk)
+            branched |= up != list(range(len(up)))
+        self.launch_log.append(B)
+        packed = torch.cat([ids, pos, slot, parents, rows[:, None], lens[:, None], nodes[:, None]], 1)
+        logits, (ids_d, parents_d, table, lens_d, nodes_d) = self._forward_trees(packed, tree_mask(parents))
+        heads = logits[:B, 0].clone() if not all(walked) else None          # before any is cut down
+        logits = self._truncate(logits, running, walked)
+        u = torch.rand(Bb, T, generator=self._gen).to(dev)
+        path, count, out = verify_drafts(logits, ids_d, u, temperature.to(dev), parents=parents_d, nodes=nodes_d)
+        if branched:
+            paged_keep(self.kv.layers(), lens_d, path, count, table)
+        said = torch.cat([count[:, None], out], 1).tolist()                 # the pass's one synchronisation
+        for b, s in enumerate(running):
+            toks = said[b][1:said[b][0] + 2] if walked[b] else self._sample([s], heads[b:b + 1])
+            for tok in toks:
+                s.kv_position += 1
+                self._emit(s, tok)
+                if s.done:
+                    break
+            self.spec_drafted += int(nodes[b]) - 1
+            self.spec_accepted += len(toks) - 1
+
+    def _truncate(self, logits: torch.Tensor, running: List[RequestState], walked: List[bool]) -> torch.Tensor:
+        """Sets what top-k and top-p of a sampled request leave out to -inf: the k largest, of these the shortest run from the top that holds ``top_p``."""
+        for b, s in enumerate(running):
+            c, V = s.config, logits.shape[2]
+            if not walked[b] or c.temperature <= 0.0 or not (1 <= c.top_k < V or 0.0 < c.top_p < 1.0):
+                continue
+            vals, at = torch.topk(logits[b], c.top_k if 1 <= c.top_k < V else V, dim=-1)
+            e = torch.exp((vals - vals[:, :1]) / c.temperature)
+            if 0.0 < c.top_p < 1.0:
+                vals = vals.masked_fill(e.cumsum(-1) - e >= c.top_p * e.sum(-1, keepdim=True), -float("inf"))
+            logits[b] = torch.full_like(logits[b], -float("inf")).scatter_(1, at, vals)
+        return logits
+
+    def _tree_layers(self, packed: torch.Tensor, mask: torch.Tensor) -> tuple:
+        """The device work of a pass over trees: logits ``[B, T, V]`` and what the verification reads."""
+        T = mask.shape[1]
+        ids, pos, slot, parents = (packed[:, i * T:(i + 1) * T].contiguous() for i in range(4))
+        rows, lens, nodes = (packed[:, 4 * T + i].contiguous() for i in range(3))
+        table = self.page_table[rows.long()]
+        logits = self.model.tree_pass(self.kv, table, ids, pos, slot, lens, nodes, mask)
+        return logits, (ids, parents, table, lens, nodes)
+
+    def _forward_trees(self, packed: torch.Tensor, mask: torch.Tensor) -> tuple:
+        """On a GPU a CUDA graph for each batch bucket; padding requests have no nodes."""
+        if self.device.type != "cuda" or not self.use_graphs:
+            return self._tree_layers(packed.to(self.device), mask.to(self.device))
+        key = ("tree", packed.shape[0])
+        if key not in self._graphs:
+            held = [t.clone().pin_memory() for t in (packed, mask)]
+            on = [t.to(self.device) for t in held]
+            idle = on[0].clone()
+            idle[:, -1] = 0                                                 # warm-up without nodes: it writes nothing
+            idle[:, 2 * mask.shape[1]:3 * mask.shape[1]] = -1
+            side = torch.cuda.Stream(device=self.device)
+            side.wait_stream(torch.cuda.current_stream(self.device))
+            with torch.cuda.stream(side):
+                self._tree_layers(idle, on[1])
+            torch.cuda.current_stream(self.device).wait_stream(side)
+            torch.cuda.synchronize(self.device)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = self._tree_layers(*on)
+            self._graphs[key] = (graph, on, held, out)
+        graph, on, held, out = self._graphs[key]
+        for h, d, t in zip(held, on, (packed, mask)):
+            h.copy_(t)
+            d.copy_(h, non_blocking=True)
+        graph.replay()
+        return out
 
     def _step_speculative(self, running: List[RequestState]):
         """One decode pass in which a greedy request contributes 1 + d rows: its last id and d proposed ids at the next

@@ -1,0 +1,84 @@
+"""The batching engine with trees of drafted ids and quantised pages on the GPU: writing, attention, verification and keeping together, in graphs, as a server runs them."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def setup(D, kv):
+    from prometorch_b200.serve.llm import LlamaConfig, LlamaWeights
+    cfg = LlamaConfig(vocab_size=1024, hidden_size=4 * D, intermediate_size=1024, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=512, eos_token_id=-1)
+    g = torch.Generator().manual_seed(7)
+    piece = torch.randint(3, 1024, (10,), generator=g).tolist()
+    prompts = [[1] + piece * 6, [1] + torch.randint(3, 1024, (40,), generator=g).tolist(), [1] + piece[:4] * 20 + piece[2:8] + piece[:3]]
+    return LlamaWeights.random(cfg, seed=2, dtype=torch.bfloat16), prompts
+
+
+def serve(w, prompts, config, **kw):
+    from prometorch_b200.serve.llm import GenerationConfig, LLMEngine, Request
+    e = LLMEngine(device="cuda", max_pages=64, max_active=4, seed=1, **kw)
+    e.set_weights(w)
+    for i, p in enumerate(prompts):
+        e.submit_request(Request(i, p, GenerationConfig(**config)))
+    res = {}
+    while e.num_active():
+        e.step()
+        res.update({r.request_id: r.token_ids for r in e.poll_responses()})
+    assert e.kv.pages_in_use == 0
+    return res, e
+
+
+@pytest.mark.parametrize("kv", [None, "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_greedy_tokens_of_trees(D, kv):
+    """Every id that comes out is the arg-max of what the plain decode step says behind the ids before it, up to the noise of bf16 sums in another order: 3e-2 of a row's
+    root mean square (the bound the engine's logits are held to against fp32), five of those on either of two logits."""
+    from prometorch_b200.serve.llm import LLMEngine
+    w, prompts = setup(D, kv)
+    config = dict(max_new_tokens=40, temperature=0.0, repetition_penalty=1.0, top_k=1)
+    for graphs in (True, False):
+        got, eng = serve(w, prompts, config, spec_tokens=6, spec_branches=3, kv_dtype=kv, use_graphs=graphs)
+        assert all(len(got[i]) == 40 for i in range(3)) and eng.spec_accepted > 0 and eng.steps <= 40          # a request that nothing is accepted for takes 40
+        plain = LLMEngine(device="cuda", max_pages=64, max_active=4, kv_dtype=kv)
+        plain.set_weights(w)
+        for i, p in enumerate(prompts):
+            s = plain.open_sequence()
+            row = plain.feed([(s, p, [len(p) - 1])])[0]
+            for t in got[i]:
+                assert float(row.max() - row[t]) <= 2 * 5 * 3e-2 * float(row.square().mean().sqrt()), (i, t)
+                row = plain.feed([(s, [t], [0])])[0]
+            plain.close_sequence(s)
+
+
+@pytest.mark.parametrize("kv", [None, "e4m3"])
+def test_sampled_requests_speculate(kv):
+    w, prompts = setup(64, kv)
+    got, eng = serve(w, prompts, dict(max_new_tokens=30, temperature=0.05, repetition_penalty=1.0, top_k=3, top_p=0.9), spec_tokens=6, spec_branches=2, kv_dtype=kv)
+    assert all(len(got[i]) == 30 for i in range(3)) and eng.spec_accepted > 0
+    got, eng = serve(w, prompts, dict(max_new_tokens=9), spec_tokens=6, spec_branches=2, kv_dtype=kv)          # a penalty: one id a pass
+    assert all(len(got[i]) == 9 for i in range(3)) and eng.spec_drafted == 0
+
+
+def test_quantised_logits_against_the_cpu_engine():
+    """The same passes in fp32 on the host over pages quantised the same way."""
+    from prometorch_b200.serve.llm import LLMEngine
+    w, prompts = setup(128, "e4m3")
+    rows = []
+    for dev in ("cuda", "cpu"):
+        e = LLMEngine(device=dev, max_pages=16, max_active=2, kv_dtype="e4m3", dtype=torch.bfloat16 if dev == "cuda" else torch.float32)
+        e.set_weights(w)
+        s = e.open_sequence()
+        e.feed([(s, prompts[0], [])])
+        rows.append(torch.cat([e.feed([(s, [t], [0])]) for t in (5, 6, 7)]).float().cpu())
+        e.close_sequence(s)
+    a, b = rows
+    assert float((a - b).norm() / b.norm()) < 5e-2          # 3e-2 as without quantising; a value near a tie of e4m3 may round either way, 2^-4 of few values
+
+
+def test_head_sizes_without_kernels_are_refused():
+    from prometorch_b200.serve.llm import LlamaConfig, LlamaWeights, LLMEngine
+    cfg = LlamaConfig(vocab_size=64, hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=2, max_position_embeddings=64)
+    w = LlamaWeights.random(cfg, seed=0, dtype=torch.bfloat16)
+    for kw in (dict(kv_dtype="e4m3"), dict(spec_tokens=3, spec_branches=1)):
+        with pytest.raises(ValueError):
+            LLMEngine(device="cuda", max_pages=4, max_active=1, **kw).set_weights(w)
