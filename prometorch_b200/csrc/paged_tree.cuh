@@ -5,9 +5,9 @@
 // Node i of a request stands in slot lens[b] + i.  All nodes and all query heads of a kv head are rows of one matrix, row = node * G + head, so that
 // a page is fetched once for all of them.
 //
-// Work is dealt on the device: an item is a (request, tile of rows, kv head), a unit one of its pages; the units of all items, in order, are cut into equal
-// runs, one for each CTA.  Lengths differ as they like, the host knows none of them, and a captured graph serves all.  A CTA writes the rows of an
-// item that lies in its run as a whole; of one that is cut it leaves (accumulators, maximum, sum) for paged_tree_merge_kernel.
+// Work is dealt on the device: an item is a (request, tile of rows, kv head), a unit 64 or 128 of its tokens; the units of all items, in order, are cut into equal
+// runs, one for each CTA.  Lengths differ as they like, the host knows none of them, and a captured graph serves all.  Of an item that is cut every CTA leaves
+// a partial result (accumulators, maximum, sum) for paged_tree_merge_kernel.
 #pragma once
 #include "common.cuh"
 #include <cuda.h>
@@ -32,9 +32,12 @@ struct Params {
     int pt_stride, n_pages;
     const uint8_t* k_exp;                // [n_pages, Hk, 64] biased exponents, null: bf16 pages
     const uint8_t* v_exp;
+    const uint8_t* v_raw;                // the pool of values, as bytes
     float* work;                         // partials of cut items
     int B, T, H, Hk, G;
     int tile_rows, tiles;                // rows of a tile, tiles of T nodes
+    int unit;                            // tokens of a unit
+    int parts;                           // partial results that a CTA leaves of an item (of which some may be empty)
     int ctas;
     float scale_log2;
     int* status;
@@ -45,17 +48,17 @@ __host__ __device__ constexpr size_t partial_floats(int rows, int D) { return (s
 __device__ __forceinline__ int nodes_of(const Params& P, int b) { return P.nodes ? max(0, min(P.nodes[b], P.T)) : P.T; }
 __device__ __forceinline__ int cached_of(const Params& P, int b, int n) { return max(0, min(P.lens[b], P.pt_stride * PAGE - n)); }
 
-// What a request asks for: tiles with rows, pages of an item.
-struct Req { int nodes, len, tiles, pages; };
+// What a request asks for: tiles with rows, units of an item.
+struct Req { int nodes, len, tiles, units; };
 __device__ __forceinline__ Req req_of(const Params& P, int b) {
     Req r;
     r.nodes = nodes_of(P, b);
     r.len = cached_of(P, b, r.nodes);
     r.tiles = (r.nodes * P.G + P.tile_rows - 1) / P.tile_rows;
-    r.pages = (r.len + r.nodes + PAGE - 1) / PAGE;
+    r.units = (r.len + r.nodes + P.unit - 1) / P.unit;
     return r;
 }
-__device__ __forceinline__ int units_of(const Params& P, const Req& r) { return r.tiles * P.Hk * r.pages; }
+__device__ __forceinline__ int units_of(const Params& P, const Req& r) { return r.tiles * P.Hk * r.units; }
 
 // starts[b]: units before request b (starts[B]: all).  The block's N threads, with `part` of N / 32 ints.
 template <int N>
@@ -88,8 +91,48 @@ __device__ __forceinline__ void plan(const Params& P, int* starts, int* part) {
 // The run of units of a CTA: `per` each.
 __device__ __forceinline__ int units_per_cta(int all, int ctas) { return max(1, (all + ctas - 1) / ctas); }
 
-// Partials: a CTA leaves at most two, of the item its run begins in (slot 0) and of the one it ends in (slot 1; where both are the same item, slot 0).
-__device__ __forceinline__ size_t partial_at(const Params& P, int cta, int slot, int D) { return ((size_t)cta * 2 + slot) * partial_floats(P.tile_rows, D); }
+// A CTA leaves partial results of at most two items: the one its run begins in (slot 0) and the one it ends in (slot 1; where both are the same, slot 0).
+// One is [rows][D] accumulators, then [rows] (maximum, sum).
+__device__ __forceinline__ size_t partial_at(const Params& P, int cta, int slot, int part, int D) { return (size_t)((cta * 2 + slot) * P.parts + part) * partial_floats(P.tile_rows, D); }
+
+// An item and the part of it in a CTA's run: n units from `first` on.
+struct Item { int b, tile, kvh, first, n; Req r; };
+__device__ __forceinline__ Item item_at(const Params& P, const int* starts, int u, int u1) {
+    int lo = 0, hi = P.B;                                // the last request that starts at or before u (empty ones share a start with the next)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= u) lo = mid; else hi = mid;
+    }
+    Item it;
+    it.b = lo;
+    it.r = req_of(P, lo);
+    const int in = u - starts[lo], i = in / it.r.units;
+    it.first = in - i * it.r.units;
+    it.n = min(it.r.units - it.first, u1 - u);
+    it.tile = i / P.Hk;
+    it.kvh = i - it.tile * P.Hk;
+    return it;
+}
+
+// Weights are 2^(s - m + up): fp16, whose smallest step is 2^-24, holds what a long context's many small weights add up to.  m is the reference, a maximum that
+// was passed by less than 2^8; the largest weight is 2^15.
+template <bool Q8> __device__ __forceinline__ constexpr float weight_up() { return Q8 ? 7.f : 0.f; }
+
+// Two e4m3 values (the low 16 bits) as fp16, exactly.
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t two) {
+    uint32_t h;
+    asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(h) : "r"(two));
+    return h;
+}
+template <bool Q8>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    uint32_t r;
+    if constexpr (Q8) { const __half2 h = __floats2half2_rn(x, y); memcpy(&r, &h, 4); }
+    else { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); memcpy(&r, &h, 4); }
+    return r;
+}
+
+template <int D, bool Q8> int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);      // paged_tree_sm100.cu
 
 }  // namespace tree
 }  // namespace ptb

@@ -1,0 +1,568 @@
+// More than sixteen rows of drafted tokens against a paged cache, both products on the 5th-generation tensor cores; see paged_tree.cuh.
+//
+// One CTA per SM walks its run of units, blocks of 128 tokens (two pages).  Rows lie along the 128 lanes of tensor memory.  Sixteen warps:
+//   warp 0      brings pages: bf16 keys and values straight to the tiles the products read; e4m3 ones, and their exponents, to a ring of raw pages;
+//   warp 1      owns tensor memory and issues S(j) = Q K_j^T and O += P(j) V_j;
+//   warps 4-11  softmax, two groups of four warps that take every other block, each with a score buffer, a running maximum and sum and an output accumulator of its
+//               own: while one group works on its scores the tensor cores work for the other.  A thread owns a row, so nothing is exchanged.  Weights go back to
+//               tensor memory, over the scores they came from, as the first operand of the second product.  The accumulator is scaled, by its own threads, only
+//               when a row's maximum has grown by 2^8;
+//   warps 12-15 e4m3: the raw page to fp16 tiles.  bf16: of a block with drafted tokens they clear the values that must not meet a weight.
+//
+// e4m3 values times a power of two are exact in fp16, which has five more exponents than they need: a block's keys are brought to the largest exponent among them (which
+// then scales the block's scores), the values to a reference that only grows and that the accumulator follows.  A key or a value more than 2^30 below those loses bits that
+// the scores and the sums do not hold either.
+//
+// What bounds it: the cache's bytes up to 128 rows (a block of 128 keys of 128 elements is 64 KB in bf16 and takes an SM's share of the memory 1.5 us; exponentials, products and
+// softmax instructions take about 0.6 us each, side by side); with more tiles of rows, which fetch the pages again, the products and exponentials.
+//
+// A drafted token that a row does not see must not reach it, whatever it holds: its weight is zero, and zero times a value that is no number is none.  So such values are
+// cleared in the tile and the rows that do see the token take them at the end.  What lies behind a request's last token is cleared as well.
+#include "paged_tree.cuh"
+#include "gemm_sm100.cuh"
+
+namespace ptb {
+namespace tree {
+namespace {
+
+using namespace ptb::gemm;
+
+constexpr int BQ = 128, BLOCK = 128, THREADS = 512;
+constexpr int SOFTMAX_WARP = 4, CONVERT_WARP = 12;
+
+template <int D, bool Q8>
+struct Sm {
+    static constexpr int Q_BYTES = BQ * D * 2, TILE = BLOCK * D * 2, RAW = BLOCK * D, PAGE_RAW = RAW / 2;
+    static constexpr int NK = Q8 ? 1 : D == 128 ? 2 : 3, NV = Q8 ? 2 : D == 128 ? 3 : 4, NR = Q8 ? (D == 128 ? 2 : 4) : 0;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NK * TILE, OFF_R = OFF_V + NV * TILE, OFF_E = OFF_R + NR * 2 * RAW;
+    static constexpr int OFF_BAR = OFF_E + NR * 2 * BLOCK, OFF_PLAN = OFF_BAR + 1024;
+    static constexpr int TOTAL = OFF_PLAN + 1024;                      // and (B + 1) ints
+    static_assert(TOTAL + MAX_B * 4 + 4 <= 227 * 1024, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) { tmem_st16(taddr, r); tmem_st16(taddr + 16, r + 16); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Loads have arrived; the registers are not read before.
+__device__ __forceinline__ void tmem_ld_done(uint32_t* r) {
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])::"memory");
+}
+__device__ __forceinline__ void convert_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// fp16 or bf16 operands, fp32 accumulators.
+template <bool Q8>
+constexpr uint32_t idesc(int n, int b_mn) { return instr_desc(BQ, n, 0, b_mn) & (Q8 ? ~((1u << 7) | (1u << 10)) : ~0u); }
+
+// Which of 32 tokens from `d0` behind the cached ones on (negative: still cached) a row sees; seen: its mask, of nodes that are there.
+__device__ __forceinline__ uint32_t visible32(unsigned long long seen, int d0) {
+    if (d0 >= 0) return d0 < 64 ? (uint32_t)(seen >> d0) : 0u;
+    if (d0 <= -32) return ~0u;
+    return ((1u << -d0) - 1) | (uint32_t)(seen << -d0);
+}
+__device__ __forceinline__ uint32_t byte_max(uint32_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = __vmaxu4(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return max(max(v & 255, (v >> 8) & 255), max((v >> 16) & 255, v >> 24));
+}
+// 2^e as two fp16 (zero below what fp16 has).
+__device__ __forceinline__ __half2 half2_pow2(int e) {
+    const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+    const uint32_t w = h | (h << 16);
+    return *reinterpret_cast<const __half2*>(&w);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
+
+constexpr int V_ROOM = 3;                // fp16 values stand for value * 2^(reference - V_ROOM): the reference may be passed by 2^4 before it has to grow
+constexpr int K_ROOM = 7;                // 448 * 2^7 fits fp16
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params P) {
+    using S = Sm<D, Q8>;
+    constexpr int NK = S::NK, NV = S::NV, NR = Q8 ? S::NR : 1;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *sq = smem, *sk = smem + S::OFF_K, *sv = smem + S::OFF_V, *sr = smem + S::OFF_R, *se = smem + S::OFF_E;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
+    uint64_t *q_full = bars, *q_free = bars + 1, *s_full = bars + 2, *p_ready = bars + 4, *o_full = bars + 6;            // [1], [1], [2], [2], [2]
+    uint64_t *k_full = bars + 8, *k_empty = bars + 12, *v_full = bars + 16, *v_empty = bars + 20, *v_ready = bars + 24;  // [NK], [NK], [NV], [NV], [NV]
+    uint64_t *raw_full = bars + 28, *raw_empty = bars + 32;                                                              // [NR], [NR]
+    unsigned long long* taint = reinterpret_cast<unsigned long long*>(bars + 36);          // [8] by item: drafted tokens whose values were cleared
+    int* bad_pages = reinterpret_cast<int*>(bars + 44);                // [8] by block: bits of pages that are none of the pool's
+    int* k_ref = bad_pages + 8;                                        // [8] by block: biased exponent that its keys were brought to
+    int* v_ref = k_ref + 8;                                            // [8] by block: that of its values' reference
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ref + 8);
+    int* part = reinterpret_cast<int*>(tmem_slot + 1);                 // [16]
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(part + 16);
+    int* starts = reinterpret_cast<int*>(smem + S::OFF_PLAN);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 4);
+        mbar_init(q_free, 1);
+        for (int g = 0; g < 2; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_ready[g], 4); mbar_init(&o_full[g], 1); }
+        for (int s = 0; s < NK; ++s) { mbar_init(&k_full[s], Q8 ? 4 : 1); mbar_init(&k_empty[s], 1); }
+        for (int s = 0; s < NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); mbar_init(&v_ready[s], 4); }
+        for (int s = 0; s < NR; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 4); }
+        *abort_flag = 0;
+        mbar_fence_init();
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    constexpr uint32_t TM_S = 0, TM_O = 256;             // two buffers of 128 columns, two of D
+    pdl_wait();
+    pdl_launch_dependents();
+    plan<THREADS>(P, starts, part);
+    __syncthreads();
+    const int all = starts[P.B], per = units_per_cta(all, P.ctas);
+    const int u0 = (int)min((long long)all, (long long)blockIdx.x * per), u1 = min(all, u0 + per);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int turn) { return ok && !*abort_flag && mbar_wait(bar, (uint32_t)(turn & 1), P.status); };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------------------------ pages
+        int n = 0;                                       // block of the run
+        for (int u = u0; u < u1 && ok;) {
+            const Item it = item_at(P, starts, u, u1);
+            const int pages = (it.r.len + it.r.nodes + PAGE - 1) / PAGE;
+            for (int j = 0; j < it.n && ok; ++j, ++n) {
+                int id = 0;
+                const int p0 = 2 * (it.first + j);
+                static_assert(PAGE * 2 == BLOCK, "two pages a block");
+                if (lane < 2) {
+                    id = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : -2;        // -2: behind the last page
+                    if (id != -2 && (id < 0 || id >= P.n_pages)) {
+                        id = -1;
+                        if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
+                    }
+                }
+                const int page[2] = {__shfl_sync(0xffffffffu, id, 0), __shfl_sync(0xffffffffu, id, 1)};
+                if (lane == 0) {
+                    const int there = page[1] == -2 ? 1 : 2;
+                    if constexpr (Q8) {
+                        const int s = n % NR;
+                        if (n >= NR) ok = wait(&raw_empty[s], n / NR - 1);
+                        if (ok) {
+                            bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
+                            mbar_expect_tx(&raw_full[s], there * (2 * S::PAGE_RAW + 2 * PAGE));
+                            for (int x = 0; x < there; ++x) {
+                                const int head = max(page[x], 0) * P.Hk + it.kvh;        // a page that is none of the pool's: any other in its place, which no row sees
+                                tma_load_2d(sr + s * 2 * S::RAW + x * S::PAGE_RAW, &tmK, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
+                                tma_load_2d(sr + s * 2 * S::RAW + S::RAW + x * S::PAGE_RAW, &tmV, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
+                                bulk_g2s(se + s * 2 * BLOCK + x * PAGE, P.k_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
+                                bulk_g2s(se + s * 2 * BLOCK + BLOCK + x * PAGE, P.v_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
+                            }
+                        }
+                    } else {
+                        const int sK = n % NK, sV = n % NV;
+                        if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
+                        if (ok) {
+                            bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
+                            mbar_expect_tx(&k_full[sK], there * (S::TILE / 2));
+                            for (int x = 0; x < there; ++x)
+                                for (int c = 0; c < D / 64; ++c)
+                                    tma_load_2d(sk + sK * S::TILE + c * (BLOCK * 128) + x * 8192, &tmK, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &k_full[sK]);
+                            if (n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
+                        }
+                        if (ok) {
+                            mbar_expect_tx(&v_full[sV], there * (S::TILE / 2));
+                            for (int x = 0; x < there; ++x)
+                                for (int c = 0; c < D / 64; ++c)
+                                    tma_load_2d(sv + sV * S::TILE + (x * (D / 64) + c) * 8192, &tmV, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &v_full[sV]);
+                        }
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            }
+            u += it.n;
+        }
+        if (!ok) *abort_flag = 1;
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------------------------ products
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc<Q8>(BLOCK, 0), id_o = idesc<Q8>(D, 1);
+            int base = 0, item = 0, p_turn[2] = {0, 0};  // base: block of the run that the item begins with
+            for (int u = u0; u < u1 && ok; ++item) {
+                const Item it = item_at(P, starts, u, u1);
+                const int total = it.r.len + it.r.nodes;
+                auto issue_s = [&](int j) {
+                    const int n = base + j, s = n % NK;
+                    ok = wait(&k_full[s], n / NK);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(sq), b0 = smem_u32(sk + s * S::TILE);
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_bf16(tmem + TM_S + (uint32_t)((j & 1) * BLOCK), smem_desc(a0 + c * (BQ * 128) + k * 32, 16, 1024), smem_desc(b0 + c * (BLOCK * 128) + k * 32, 16, 1024), id_s,
+                                      (c > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(&k_empty[s]);
+                    umma_commit(&s_full[j & 1]);
+                    if (j + 1 == it.n) umma_commit(q_free);
+                };
+                ok = wait(q_full, item);
+                if (ok) issue_s(0);
+                if (ok && it.n > 1) issue_s(1);
+                for (int j = 0; j < it.n && ok; ++j) {
+                    const int g = j & 1, n = base + j, s = n % NV, t0 = (it.first + j) * BLOCK;
+                    ok = wait(&p_ready[g], p_turn[g]++);
+                    if (ok) ok = wait(&v_ready[s], n / NV);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t b0 = smem_u32(sv + s * S::TILE);
+                    const int halves = t0 + PAGE < total ? 2 : 1;      // the second page is there
+                    for (int x = 0; x < halves; ++x)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_ts(tmem + TM_O + (uint32_t)(g * D), tmem + TM_S + (uint32_t)(g * BLOCK + (x * 4 + k) * 8), smem_desc(b0 + x * (D / 64) * 8192 + k * 2048, 8192, 1024), id_o,
+                                    (j > 1 || x > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(&v_empty[s]);
+                    if (j + 2 >= it.n) umma_commit(&o_full[g]);
+                    if (j + 2 < it.n) issue_s(j + 2);
+                }
+                base += it.n;
+                u += it.n;
+            }
+            if (!ok) *abort_flag = 1;
+        }
+    } else if (warp >= SOFTMAX_WARP && warp < CONVERT_WARP) {
+        // ------------------------------------------------------------------------------------ softmax
+        const int g = (warp - SOFTMAX_WARP) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + TM_S + (uint32_t)(g * BLOCK), to = lanes + TM_O + (uint32_t)(g * D);
+        int base = 0, item = 0, s_turn = 0, o_turn = 0;
+        for (int u = u0; u < u1; ++item) {
+            const Item it = item_at(P, starts, u, u1);
+            const int len = it.r.len, nodes = it.r.nodes, rows = min(BQ, nodes * P.G - it.tile * BQ);
+            const bool live = (warp & 3) * 32 < rows, on = row < rows;
+            const int at = it.tile * BQ + row, node = on ? at / P.G : 0, head = on ? at - node * P.G : 0;
+            unsigned long long seen = 0;
+            if (on) seen = (P.mask ? P.mask[(size_t)it.b * P.T + node] : (2ull << node) - 1) & (nodes < 64 ? (1ull << nodes) - 1 : ~0ull);
+            float fac = P.scale_log2;
+            if (Q8 || g == 0) {                          // the row of q: both groups want its scale, the first puts it into the tile
+                const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)it.b * P.q_batch + (size_t)node * P.q_row + (size_t)(it.kvh * P.G + head) * D);
+                uint4 raw[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) raw[i] = on ? q[i] : make_uint4(0, 0, 0, 0);
+                if constexpr (Q8) {                      // to fp16, its largest magnitude in [1, 2)
+                    uint32_t a = 0;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) a = max(a, max(w[x] & 0x7fffu, (w[x] >> 16) & 0x7fffu));
+                    }
+                    const int k = min(253, max(1, (int)(a >> 7)));           // biased exponent
+                    const float down = __uint_as_float((uint32_t)(254 - k) << 23);
+                    fac *= __uint_as_float((uint32_t)k << 23);
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&raw[i]);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[x]));
+                            w[x] = pack2<true>(f.x * down, f.y * down);
+                        }
+                    }
+                }
+                if (g == 0) {
+                    if (item > 0) ok = wait(q_free, item - 1);               // the products of the last item have read theirs
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(sq + (i / 8) * (BQ * 128) + row * 128 + (((i & 7) ^ (row & 7)) * 16)) = raw[i];
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q_full);
+                }
+            }
+            float m = -INFINITY, l = 0.f;
+            int ref = 0;                                 // of the values that the accumulator holds
+            for (int j = g; j < it.n; j += 2) {
+                const int n = base + j, t0 = (it.first + j) * BLOCK;
+                ok = wait(&s_full[g], s_turn++);
+                tc_fence_after();
+                if (live && ok) {
+                    const int bad = bad_pages[n & 7];
+                    const bool some = t0 + BLOCK > len || bad;               // not every row sees every token
+                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    if (some) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) vis[c] = (bad >> (c >> 1)) & 1 ? 0u : visible32(seen, t0 + 32 * c - len);
+                    }
+                    const float f = Q8 ? fac * pow2(k_ref[n & 7] - 127 - K_ROOM) : fac;
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    uint32_t r[2][32];
+                    tmem_ld32(ts, r[0]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_ld_done(r[c & 1]);
+                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), r[(c + 1) & 1]);
+                        if (some) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], (vis[c] >> i) & 1 ? __uint_as_float(r[c & 1][i]) : -INFINITY);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[c & 1][i]));
+                        }
+                    }
+                    tmem_ld32(ts, r[0]);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+                    float alpha = 1.f;
+                    if (mx > m + 8.f) {
+                        alpha = exp2f(m - mx);
+                        m = mx;
+                        l *= alpha;
+                    }
+                    if constexpr (Q8) {
+                        const int to_ref = v_ref[n & 7];
+                        alpha *= pow2(j > 1 ? ref - to_ref : 0);
+                        ref = to_ref;
+                    }
+                    const float mu = m == -INFINITY ? 0.f : m - weight_up<Q8>();
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_ld_done(r[c & 1]);
+                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), r[(c + 1) & 1]);
+                        uint32_t p[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float x = fmaf(__uint_as_float(r[c & 1][2 * i]), f, -mu), y = fmaf(__uint_as_float(r[c & 1][2 * i + 1]), f, -mu);
+                            if (some) {
+                                if (!((vis[c] >> (2 * i)) & 1)) x = -INFINITY;
+                                if (!((vis[c] >> (2 * i + 1)) & 1)) y = -INFINITY;
+                            }
+                            x = exp2f(x);
+                            y = exp2f(y);
+                            l4[i & 3] += x + y;
+                            p[i] = pack2<Q8>(x, y);
+                        }
+                        tmem_st16(ts + 16 * c, p);                           // over scores that have been read
+                    }
+                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    if (j > 1 && __any_sync(0xffffffffu, alpha != 1.f)) {    // these scores are there, so the product before them is done
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            tmem_ld32(to + 32 * c, r[0]);
+                            tmem_ld_done(r[0]);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) r[0][i] = __float_as_uint(__uint_as_float(r[0][i]) * alpha);
+                            tmem_st32(to + 32 * c, r[0]);
+                        }
+                    }
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[g]);
+            }
+            // ---- the item's part of this group
+            float* wk = P.work + partial_at(P, blockIdx.x, u == u0 ? 0 : 1, g, D);
+            float2* ml = reinterpret_cast<float2*>(wk + (size_t)BQ * D) + row;
+            if (it.n > g) {
+                ok = wait(&o_full[g], o_turn++);
+                tc_fence_after();
+                if (live && ok) {
+                    const unsigned long long meets = taint[item & 7] & seen;
+                    const float down = Q8 ? pow2(ref - 127 - V_ROOM) : 1.f;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32(to + 32 * c, r);
+                        tmem_ld_done(r);
+                        if constexpr (Q8) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * down);
+                        }
+                        for (unsigned long long left = meets; left; left &= left - 1) {          // values that were cleared, of a token that this row sees
+                            const int t = len + __ffsll((long long)left) - 1;
+                            if (t / BLOCK < it.first || t / BLOCK >= it.first + it.n || ((t / BLOCK - it.first) & 1) != g) continue;
+                            const int page = P.page_table[(size_t)it.b * P.pt_stride + t / PAGE];
+                            if (page < 0 || page >= P.n_pages) continue;
+                            const size_t v = (((size_t)page * P.Hk + it.kvh) * PAGE + t % PAGE) * D + 32 * c;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                if constexpr (Q8) {
+                                    if ((P.v_raw[v + i] & 0x7f) == 0x7f) r[i] = 0x7fffffffu;
+                                } else {
+                                    const uint32_t w = (uint32_t)reinterpret_cast<const uint16_t*>(P.v_raw)[v + i] << 16;
+                                    if ((w & 0x7f800000u) == 0x7f800000u) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(w));
+                                }
+                            }
+                        }
+                        if (on) {
+                            float* dst = wk + (size_t)row * D + 32 * c;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) st_global_32(dst + i, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]), make_uint4(r[i + 4], r[i + 5], r[i + 6], r[i + 7]));
+                        }
+                    }
+                    *ml = on ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+                }
+            } else if (live) {
+                *ml = make_float2(-INFINITY, 0.f);
+            }
+            base += it.n;
+            u += it.n;
+        }
+        if (!ok) *abort_flag = 1;
+    } else if (warp >= CONVERT_WARP) {
+        // ------------------------------------------------------------------------------------ tiles
+        const int cw = warp - CONVERT_WARP, tid = threadIdx.x - CONVERT_WARP * 32;
+        int n = 0, item = 0;
+        for (int u = u0; u < u1; ++item) {               // after a wait that ran out as well: the four warps meet at every item
+            const Item it = item_at(P, starts, u, u1);
+            const int len = it.r.len, total = len + it.r.nodes;
+            if (tid == 0) taint[item & 7] = 0;           // eight items back: nobody reads it any more
+            convert_sync();
+            int ref = 0;
+            for (int j = 0; j < it.n; ++j, ++n) {
+                const int t0 = (it.first + j) * BLOCK, sV = n % NV;
+                if constexpr (!Q8) {
+                    ok = wait(&v_full[sV], n / NV);
+                    const int t = t0 + tid;
+                    if (ok && t0 + BLOCK > len && t >= len) {
+                        uint8_t* v = sv + sV * S::TILE + (tid >> 6) * (D / 64) * 8192 + (tid & 63) * 128;
+                        bool odd = false;
+                        for (int i = 0; i < D / 8; ++i) {
+                            uint4* w = reinterpret_cast<uint4*>(v + (i / 8) * 8192 + (i & 7) * 16);
+                            if (t >= total) { *w = make_uint4(0, 0, 0, 0); continue; }
+                            uint4 x = *w;
+                            uint32_t* y = reinterpret_cast<uint32_t*>(&x);
+                            uint32_t any = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t no = __vcmpeq2(y[k] & 0x7f807f80u, 0x7f807f80u);
+                                any |= no;
+                                y[k] &= ~no;
+                            }
+                            if (any) { *w = x; odd = true; }
+                        }
+                        if (odd) atomicOr(&taint[item & 7], 1ull << (t - len));
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_ready[sV]);
+                } else {
+                    const int sR = n % NR, sK = n % NK;
+                    ok = wait(&raw_full[sR], n / NR);
+                    const uint8_t *ke = se + sR * 2 * BLOCK, *ve = ke + BLOCK;
+                    uint32_t kw = 0, vw = 0;
+                    if (ok) { kw = reinterpret_cast<const uint32_t*>(ke)[lane]; vw = reinterpret_cast<const uint32_t*>(ve)[lane]; }
+                    const int past = t0 + 4 * lane - total + 4;              // how many of these four lie behind the last token
+                    if (past > 0) {
+                        const uint32_t keep = past >= 4 ? 0u : 0xffffffffu >> (8 * past);
+                        kw &= keep;
+                        vw &= keep;
+                    }
+                    const int top_k = (int)byte_max(kw), top_v = (int)byte_max(vw);
+                    if (j == 0 || top_v > ref + K_ROOM - V_ROOM) ref = top_v;
+                    // eight tokens and 64 of their elements at a time: lane (token, 16-byte piece).  Two tokens of a phase differ in the bits that part their pieces in the raw
+                    // lines and in the tile's, so that neither meets in a bank
+                    constexpr int HALVES = D / 64, TURNS = BLOCK / 8 * HALVES / 4;
+                    const int pr = lane >> 3, sel = (lane >> 2) & 1, c4 = lane & 3, in8 = D == 128 ? (sel ? pr ^ 5 : pr) : 2 * pr + sel;
+                    auto convert = [&](const uint8_t* raw, const uint8_t* exps, uint8_t* tile, bool values, int top) {
+#pragma unroll 2
+                        for (int i = 0; i < TURNS; ++i) {
+                            const int turn = cw * TURNS + i, half = turn % HALVES, token = turn / HALVES * 8 + in8, x = token >> 6, t = token & 63;
+                            const uint32_t at = D == 128 ? t * 128 + (((half * 4 + c4) ^ (t & 7)) * 16) : (t >> 1) * 128 + ((((t & 1) * 4 + c4) ^ ((t >> 1) & 7)) * 16);
+                            const uint4 w = *reinterpret_cast<const uint4*>(raw + x * S::PAGE_RAW + at);
+                            uint32_t y[4] = {w.x, w.y, w.z, w.w};
+                            __half2 by = half2_pow2(min((int)exps[token] - top, 0) + (values ? min(top - ref + V_ROOM, K_ROOM) : K_ROOM));
+                            if (values && t0 + token >= len) {
+                                const bool gone = t0 + token >= total;
+                                uint32_t any = 0;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint32_t no = gone ? ~0u : __vcmpeq4(y[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                                    any |= no;
+                                    y[k] &= ~no;
+                                }
+                                if (gone) by = half2_pow2(0);
+                                else if (any) atomicOr(&taint[item & 7], 1ull << (t0 + token - len));
+                            }
+                            uint32_t h[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const uint32_t two = e4m3x2(k & 1 ? y[k >> 1] >> 16 : y[k >> 1]);
+                                const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&two), by);
+                                h[k] = *reinterpret_cast<const uint32_t*>(&z);
+                            }
+                            uint8_t* dst = tile + (values ? (x * HALVES + half) * 8192 : half * (BLOCK * 128) + x * 8192) + t * 128;
+                            *reinterpret_cast<uint4*>(dst + (((2 * c4) ^ (t & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4*>(dst + (((2 * c4 + 1) ^ (t & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+                        }
+                    };
+                    if (ok && n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
+                    if (ok) convert(sr + sR * 2 * S::RAW, ke, sk + sK * S::TILE, false, top_k);
+                    if (tid == 0) { k_ref[n & 7] = top_k; v_ref[n & 7] = ref; }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&k_full[sK]);
+                    if (ok && n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
+                    if (ok) convert(sr + sR * 2 * S::RAW + S::RAW, ve, sv + sV * S::TILE, true, top_v);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(&v_ready[sV]); mbar_arrive(&raw_empty[sR]); }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            u += it.n;
+        }
+        if (!ok) *abort_flag = 1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace
+
+// All items' partial results, two for each CTA and item.
+template <int D, bool Q8>
+int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
+    using S = Sm<D, Q8>;
+    CUtensorMap mk, mv;
+    if constexpr (Q8) {                                  // raw pages as 128-byte lines
+        constexpr int LINES = PAGE * D / 128;
+        const long long lines = (long long)p.n_pages * p.Hk * LINES;
+        if (ptb_make_tmap_bf16(&mk, k_pages, 64, lines, 64, 64, LINES) || ptb_make_tmap_bf16(&mv, v_pages, 64, lines, 64, 64, LINES)) return -1;
+    } else {
+        const long long rows = (long long)p.n_pages * p.Hk * PAGE;
+        if (ptb_make_tmap_bf16(&mk, k_pages, D, rows, D, 64, PAGE) || ptb_make_tmap_bf16(&mv, v_pages, D, rows, D, 64, PAGE)) return -1;
+    }
+    static bool attr[64];
+    int dev = 0;
+    PTB_CUDA_OK(cudaGetDevice(&dev));
+    if (dev >= 64 || !attr[dev]) {
+        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_tiles_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL + MAX_B * 4 + 4));
+        if (dev < 64) attr[dev] = true;
+    }
+    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D, Q8>, dim3(p.ctas), dim3(THREADS), (size_t)S::TOTAL + (p.B + 1) * 4, st, ptb_pdl_enabled(), mk, mv, p));
+    PTB_CUDA_OK(cudaGetLastError());
+    return 0;
+}
+template int launch_tiles<64, false>(const Params&, const void*, const void*, cudaStream_t);
+template int launch_tiles<64, true>(const Params&, const void*, const void*, cudaStream_t);
+template int launch_tiles<128, false>(const Params&, const void*, const void*, cudaStream_t);
+template int launch_tiles<128, true>(const Params&, const void*, const void*, cudaStream_t);
+
+}  // namespace tree
+}  // namespace ptb

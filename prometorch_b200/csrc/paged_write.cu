@@ -168,72 +168,68 @@ __global__ void __launch_bounds__(PW_THREADS) paged_write_kernel(const __grid_co
     }
 }
 
-constexpr int KEEP_LAYERS = 32, KEEP_THREADS = 128, KEEP_TOGETHER = 8;
+constexpr int KEEP_LAYERS = 36, KEEP_THREADS = 256, KEEP_AT_ONCE = 4;
+static_assert(KEEP_THREADS == 64 * KEEP_AT_ONCE, "a thread for each layer and token");
 
 struct KeepParams {
-    uint8_t* pool[KEEP_LAYERS][4];       // keys, values, their exponents (or null)
+    uint8_t* pool[4][KEEP_LAYERS];       // keys, values, their exponents (or null)
     const int* lens;                     // [B]
     const int* path;                     // [B, T]
     const int* count;                    // [B]
     const int* page_table;
-    int pt_stride, n_pages, Hk, row, T;  // row: bytes of a token's keys of a head
+    int pt_stride, n_pages, Hk, row, T, layers;        // row: bytes of a token's keys of a head
     int* status;
 };
 
-// A thread owns one 16-byte piece (or one exponent byte) of every token and walks the path in order.  A path ascends, so a token never moves behind its own
-// place and no later one reads a slot that an earlier one filled: eight are read before the first is written.  Latency bounds it (a path is a few
-// dozen kilobytes a layer), so all layers go in one launch.
+// A block moves the keys (or the values) of one head in up to four layers: threads are (token of the path, 16-byte piece), as many tokens at a time as fit.  A path ascends, so a token never
+// moves behind its own place and no later one reads a slot that an earlier one filled; within a group all are read before the first is written.  Latency
+// bounds it (a request's path is a few dozen kilobytes a layer), so all layers go in one launch and a move is one chain of four loads.
 __global__ void __launch_bounds__(KEEP_THREADS) paged_keep_kernel(const __grid_constant__ KeepParams P) {
+    __shared__ int at[2][64];            // where a token comes from and goes to: page * 64 + place, or -1
     pdl_wait();
     pdl_launch_dependents();
-    const int b = blockIdx.y, layer = blockIdx.z;
-    const int n = min(P.count[b], P.T - 1), len = P.lens[b];
-    const int per = P.row / 16, pieces = P.Hk * per, bytes = P.pool[layer][2] ? P.Hk : 0;
-    int e = blockIdx.x * KEEP_THREADS + threadIdx.x;
-    if (n <= 0 || e >= 2 * pieces + 2 * bytes) return;
-    const bool wide = e < 2 * pieces;
-    int which;
-    if (wide) { which = e >= pieces; e -= which * pieces; }
-    else { e -= 2 * pieces; which = 2 + (e >= bytes); e -= (which - 2) * bytes; }
-    uint8_t* pool = P.pool[layer][which];
-    const int head = wide ? e / per : e, unit = wide ? 16 : 1, row = wide ? P.row : 1, in_row = wide ? (e - head * per) * 16 : 0;
-    const int* table = P.page_table + (size_t)b * P.pt_stride;
-    auto place = [&](int slot) -> uint8_t* {
-        const int page = slot >= 0 && slot / PW_PAGE < P.pt_stride ? table[slot / PW_PAGE] : -1;
-        if (page < 0 || page >= P.n_pages) {
-            if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
-            return nullptr;
-        }
-        return pool + (((size_t)page * P.Hk + head) * PW_PAGE + slot % PW_PAGE) * row + in_row;
-    };
-    for (int j0 = 1; j0 <= n; j0 += KEEP_TOGETHER) {
-        uint4 v[KEEP_TOGETHER];
-        uint8_t* to[KEEP_TOGETHER];
-#pragma unroll
-        for (int u = 0; u < KEEP_TOGETHER; ++u) {
-            to[u] = nullptr;
-            const int j = j0 + u;
-            if (j > n) continue;
+    const int b = blockIdx.y, layer0 = blockIdx.z * KEEP_AT_ONCE, which = blockIdx.x & 1, head = blockIdx.x >> 1, tid = threadIdx.x;
+    const int n = min(P.count[b], P.T - 1);
+    if (n <= 0) return;
+    if (tid < 128) {                     // thread (end, token): looks one place up
+        const int end = tid >> 6, j = tid & 63;
+        int x = -1;
+        if (j >= 1 && j <= n) {
             const int from = P.path[(size_t)b * P.T + j];
-            if (from == j) continue;
             if (from < j || from >= P.T) {
                 if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
-                continue;
-            }
-            const uint8_t* src = place(len + from);
-            to[u] = place(len + j);
-            if (!src) to[u] = nullptr;
-            if (to[u]) {
-                if (unit == 16) v[u] = *reinterpret_cast<const uint4*>(src);
-                else v[u].x = *src;
+            } else if (from != j) {
+                const int slot = P.lens[b] + (end ? j : from);
+                const int page = slot >= 0 && slot / PW_PAGE < P.pt_stride ? P.page_table[(size_t)b * P.pt_stride + slot / PW_PAGE] : -1;
+                if (page >= 0 && page < P.n_pages) x = page * PW_PAGE + slot % PW_PAGE;
+                else if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
             }
         }
+        at[end][j] = x;
+    }
+    __syncthreads();
+    const int per = P.row / 16, together = KEEP_THREADS / per, j0 = tid / per, piece = tid - j0 * per;
+    auto spot = [&](int x, int row) { return ((size_t)(x / PW_PAGE) * P.Hk + head) * PW_PAGE * row + (size_t)(x % PW_PAGE) * row; };
+    for (int g = 1; g <= n; g += together) {
+        const int j = g + j0;
+        const bool on = j0 < together && j <= n && at[0][j] >= 0 && at[1][j] >= 0;
+        uint4 v[KEEP_AT_ONCE];
 #pragma unroll
-        for (int u = 0; u < KEEP_TOGETHER; ++u)
-            if (to[u]) {
-                if (unit == 16) *reinterpret_cast<uint4*>(to[u]) = v[u];
-                else *to[u] = (uint8_t)v[u].x;
-            }
+        for (int l = 0; l < KEEP_AT_ONCE; ++l)
+            if (on && layer0 + l < P.layers) v[l] = *reinterpret_cast<const uint4*>(P.pool[which][layer0 + l] + spot(at[0][j], P.row) + piece * 16);
+        __syncthreads();
+#pragma unroll
+        for (int l = 0; l < KEEP_AT_ONCE; ++l)
+            if (on && layer0 + l < P.layers) *reinterpret_cast<uint4*>(P.pool[which][layer0 + l] + spot(at[1][j], P.row) + piece * 16) = v[l];
+        __syncthreads();
+    }
+    if (P.pool[2][0]) {                  // thread (layer, token) moves an exponent
+        const int l = layer0 + (tid >> 6), j = tid & 63;
+        const bool on = l < P.layers && j >= 1 && j <= n && at[0][j] >= 0 && at[1][j] >= 0;
+        uint8_t v = 0;
+        if (on) v = P.pool[2 + which][l][spot(at[0][j], 1)];
+        __syncthreads();
+        if (on) P.pool[2 + which][l][spot(at[1][j], 1)] = v;
     }
 }
 
@@ -266,25 +262,25 @@ PTB_API int ptb_paged_write(const void* qkv, long long ld, int n, int H, int Hk,
 }
 
 // The cache entries of each request's accepted drafted tokens, moved from slot lens[b] + path[b][j] to lens[b] + j for j in 1 .. count[b], in every
-// layer.  pools: [layers][4] device pointers (keys, values, their exponents or null), row: bytes of a token's keys of a head; path [B, T] ascends.
+// layer.  pools: [4][layers] device pointers (keys, values, their exponents or null), row: bytes of a token's keys of a head; path [B, T] ascends.
 PTB_API int ptb_paged_keep(void* const* pools, int layers, int B, int T, int Hk, int row, int n_pages, const int* lens, const int* path, const int* count, const int* page_table,
                            int pt_stride, int* status, cudaStream_t st) {
     if (B <= 0 || layers <= 0 || T <= 1) return 0;
-    if (Hk <= 0 || row <= 0 || row % 16 || B > 65535) { ptb_set_error("paged_keep: %d kv heads of %d bytes, %d requests", Hk, row, B); return -1; }
+    if (Hk <= 0 || row <= 0 || row % 16 || row > 16 * KEEP_THREADS || B > 65535 || T > 64 || n_pages > 0x7fffffff / PW_PAGE) {
+        ptb_set_error("paged_keep: %d kv heads of %d bytes, %d requests of %d nodes (up to 64), %d pages", Hk, row, B, T, n_pages);
+        return -1;
+    }
     for (int l0 = 0; l0 < layers; l0 += KEEP_LAYERS) {
         const int m = layers - l0 < KEEP_LAYERS ? layers - l0 : KEEP_LAYERS;
         KeepParams p;
         memset(&p, 0, sizeof(p));
-        for (int l = 0; l < m; ++l)
-            for (int w = 0; w < 4; ++w) {
-                p.pool[l][w] = (uint8_t*)pools[(size_t)(l0 + l) * 4 + w];
-                if (w < 2 && (!p.pool[l][w] || off16(p.pool[l][w]))) { ptb_set_error("paged_keep: the pools need to be 16-byte aligned"); return -1; }
-            }
-        for (int l = 0; l < m; ++l)
-            if (!p.pool[l][2] != !p.pool[0][2] || !p.pool[l][3] != !p.pool[0][2]) { ptb_set_error("paged_keep: some pools have exponents and some have none"); return -1; }
-        p.lens = lens; p.path = path; p.count = count; p.page_table = page_table; p.pt_stride = pt_stride; p.n_pages = n_pages; p.Hk = Hk; p.row = row; p.T = T; p.status = status;
-        const int pieces = 2 * Hk * (row / 16) + (p.pool[0][2] ? 2 * Hk : 0);
-        PTB_CUDA_OK(ptb_launch(paged_keep_kernel, dim3((pieces + KEEP_THREADS - 1) / KEEP_THREADS, B, m), dim3(KEEP_THREADS), 0, st, ptb_pdl_enabled(), p));
+        for (int l = 0; l < m; ++l) {
+            for (int w = 0; w < 4; ++w) p.pool[w][l] = (uint8_t*)pools[(size_t)w * layers + l0 + l];
+            if (!p.pool[0][l] || !p.pool[1][l] || off16(p.pool[0][l]) || off16(p.pool[1][l])) { ptb_set_error("paged_keep: the pools need to be 16-byte aligned"); return -1; }
+            if (!p.pool[2][l] != !p.pool[2][0] || !p.pool[3][l] != !p.pool[2][0]) { ptb_set_error("paged_keep: some pools have exponents and some have none"); return -1; }
+        }
+        p.lens = lens; p.path = path; p.count = count; p.page_table = page_table; p.pt_stride = pt_stride; p.n_pages = n_pages; p.Hk = Hk; p.row = row; p.T = T; p.layers = m; p.status = status;
+        PTB_CUDA_OK(ptb_launch(paged_keep_kernel, dim3(2 * Hk, B, (m + KEEP_AT_ONCE - 1) / KEEP_AT_ONCE), dim3(KEEP_THREADS), 0, st, ptb_pdl_enabled(), p));
     }
     PTB_CUDA_OK(cudaGetLastError());
     return 0;

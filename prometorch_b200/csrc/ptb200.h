@@ -315,7 +315,7 @@ int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_row, void*
 int ptb_paged_write(const void* qkv, long long ld, int n, int H, int Hk, int D, const int* pos, const int* slot, const int* req, const int* page_table, int pt_stride, int pt_rows, int n_pages, const float* cos, const float* sin, int max_pos, void* q_out, void* k_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, int* status, cudaStream_t st);
 
 // The cache entries of each request's accepted drafted tokens, moved from slot lens[b] + path[b][j] to lens[b] + j for j in 1 .. count[b], in every
-// layer.  pools: [layers][4] device pointers (keys, values, their exponents or null), row: bytes of a token's keys of a head; path [B, T] ascends.
+// layer.  pools: [4][layers] device pointers (keys, values, their exponents or null), row: bytes of a token's keys of a head; path [B, T] ascends.
 int ptb_paged_keep(void* const* pools, int layers, int B, int T, int Hk, int row, int n_pages, const int* lens, const int* path, const int* count, const int* page_table, int pt_stride, int* status, cudaStream_t st);
 
 // ---------------------------------------------------------------------------- prompt_layers.cu

@@ -16,9 +16,10 @@
 namespace ptb {
 namespace {
 
-constexpr int VF_THREADS = 256, VF_EACH = 16, VF_CHUNK = VF_THREADS * VF_EACH;
+constexpr int VF_THREADS = 256, VF_EACH = 32, VF_CHUNK = VF_THREADS * VF_EACH;
+constexpr int VF_WALKERS = 1024;            // threads of the walk: fp64 exponentials and sums are long chains, so many run side by side
 constexpr int VF_NODES = 64;                 // nodes of a request
-constexpr int VF_CLUSTER = 16;
+constexpr int VF_CLUSTER = 16, VF_TOGETHER = 4;
 constexpr int VF_SLICE = 27 * 1024;          // weights a CTA can hold
 
 struct VerifyParams {
@@ -38,7 +39,7 @@ struct VerifyParams {
     int B, T, V, chunks, slice;      // slice: weights per CTA of the cluster
 };
 
-__device__ __forceinline__ float clean(float l) { return l == l ? l : -INFINITY; }         // NaN is no token's logit
+__device__ __forceinline__ float clean(float l) { return fmaxf(l, -INFINITY); }         // NaN is no token's logit
 
 template <bool BF16>
 __device__ __forceinline__ float logit_at(const VerifyParams& P, int b, int i, int v) {
@@ -47,91 +48,71 @@ __device__ __forceinline__ float logit_at(const VerifyParams& P, int b, int i, i
 }
 __device__ __forceinline__ int nodes_of(const VerifyParams& P, int b) { return P.nodes ? max(0, min(P.nodes[b], P.T)) : P.T; }
 
-struct Top { float m, s; int at; };          // maximum, sum of exp((x - m) / temperature), place of the maximum
-// Two parts as one: the greater maximum, of equals the earlier place.
-__device__ __forceinline__ Top join(const Top& a, const Top& b, float inv) {
-    const bool second = b.m > a.m || (b.m == a.m && b.at < a.at);
-    Top r;
-    r.m = second ? b.m : a.m;
-    r.at = second ? b.at : a.at;
-    r.s = (a.m == r.m ? a.s : a.s * __expf((a.m - r.m) * inv)) + (b.m == r.m ? b.s : b.s * __expf((b.m - r.m) * inv));
-    return r;
-}
-
-// One chunk of one row.  VEC: rows start on 16 bytes.
+// One chunk of one row: maximum, its first place, sum of exp((l - maximum) / temperature).  VEC: rows start on 16 bytes.  Bound by the logits' bytes as long as an element
+// costs few instructions: the place is looked for only in the warps that hold the chunk's maximum.
 template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(const __grid_constant__ VerifyParams P) {
+    __shared__ float part_m[VF_THREADS / 32], part_s[VF_THREADS / 32];
+    __shared__ int place;
     pdl_wait();
     pdl_launch_dependents();
-    const int row = blockIdx.y, b = row / P.T, i = row - b * P.T, chunk = blockIdx.x;
+    const int row = blockIdx.y, b = row / P.T, i = row - b * P.T, chunk = blockIdx.x, tid = threadIdx.x;
     if (i >= nodes_of(P, b)) return;
-    const float t = P.temperature[b], inv = t > 0.f ? __frcp_rn(t) : 1.f;
+    if (tid == 0) place = 0x7fffffff;
+    const float t = P.temperature[b], scale = (t > 0.f ? __frcp_rn(t) : 1.f) * 1.4426950408889634f;
     const size_t base = (size_t)b * P.l_batch + (size_t)i * P.l_row;
     const int v0 = chunk * VF_CHUNK;
+    constexpr int W = !VEC ? 1 : BF16 ? 8 : 4;                 // neighbours that a thread has at once: element k stands at v0 + ((k / W) * VF_THREADS + tid) * W + k % W
     float l[VF_EACH];
-    int at[VF_EACH];
-    if constexpr (VEC && BF16) {
-        const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(P.logits) + base;
 #pragma unroll
-        for (int k = 0; k < VF_EACH / 8; ++k) {
-            const int v = v0 + (k * VF_THREADS + threadIdx.x) * 8;
-            uint4 raw = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);      // -inf
-            if (v + 8 <= P.V) raw = *reinterpret_cast<const uint4*>(p + v);
-            else
-                for (int x = 0; x < 8; ++x)
-                    if (v + x < P.V) reinterpret_cast<__nv_bfloat16*>(&raw)[x] = p[v + x];
-            const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    for (int g = 0; g < VF_EACH / W; ++g) {
+        const int v = v0 + (g * VF_THREADS + tid) * W;
+        if (VEC && v + W <= P.V) {
+            if constexpr (BF16) {
+                const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(P.logits) + base + v);
+                const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) { const float2 f = __bfloat1622float2(h2[x]); l[8 * k + 2 * x] = clean(f.x); l[8 * k + 2 * x + 1] = clean(f.y); }
+                for (int x = 0; x < W / 2; ++x) { const float2 f = __bfloat1622float2(h2[x]); l[g * W + 2 * x] = f.x; l[g * W + (2 * x + 1) % W] = f.y; }
+            } else if constexpr (VEC) {
+                const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(P.logits) + base + v);
+                l[g * W] = f.x; l[g * W + 1 % W] = f.y; l[g * W + 2 % W] = f.z; l[g * W + 3 % W] = f.w;
+            }
+        } else {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) at[8 * k + x] = v + x;
-        }
-    } else if constexpr (VEC) {
-        const float* p = static_cast<const float*>(P.logits) + base;
-#pragma unroll
-        for (int k = 0; k < VF_EACH / 4; ++k) {
-            const int v = v0 + (k * VF_THREADS + threadIdx.x) * 4;
-            float4 raw = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (v + 4 <= P.V) raw = *reinterpret_cast<const float4*>(p + v);
-            else
-                for (int x = 0; x < 4; ++x)
-                    if (v + x < P.V) reinterpret_cast<float*>(&raw)[x] = p[v + x];
-            l[4 * k] = clean(raw.x); l[4 * k + 1] = clean(raw.y); l[4 * k + 2] = clean(raw.z); l[4 * k + 3] = clean(raw.w);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) at[4 * k + x] = v + x;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < VF_EACH; ++k) {
-            const int v = v0 + k * VF_THREADS + threadIdx.x;
-            at[k] = v;
-            l[k] = -INFINITY;
-            if (v < P.V) l[k] = clean(BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(P.logits)[base + v]) : static_cast<const float*>(P.logits)[base + v]);
+            for (int x = 0; x < W; ++x) l[g * W + x] = v + x < P.V ? logit_at<BF16>(P, b, i, v + x) : -INFINITY;
         }
     }
-    Top a;
-    a.m = l[0]; a.at = at[0];
+    float m = -INFINITY;
 #pragma unroll
-    for (int k = 1; k < VF_EACH; ++k)
-        if (l[k] > a.m) { a.m = l[k]; a.at = at[k]; }
-    a.s = 0.f;
+    for (int k = 0; k < VF_EACH; ++k) { l[k] = clean(l[k]); m = fmaxf(m, l[k]); }
+    const float mine = m;
+    m = warp_max(m);                                           // the reference of the warp's exponentials
+    float s = 0.f;
+    if (fabsf(m) < INFINITY) {
 #pragma unroll
-    for (int k = 0; k < VF_EACH; ++k) a.s += l[k] == a.m ? 1.f : __expf((l[k] - a.m) * inv);
-    if (a.m == -INFINITY) a.s = 0.f;
-    __shared__ Top part[VF_THREADS / 32];
+        for (int k = 0; k < VF_EACH; ++k) s += exp2f((l[k] - m) * scale);
+    } else if (m > 0.f) {                                      // of infinite logits each counts as one, the others as none
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Top c;
-        c.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        c.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        c.at = __shfl_xor_sync(0xffffffffu, a.at, o);
-        a = join(a, c, inv);
+        for (int k = 0; k < VF_EACH; ++k) s += l[k] == m ? 1.f : 0.f;
     }
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+    s = warp_sum(s);
+    if ((tid & 31) == 0) { part_m[tid >> 5] = m; part_s[tid >> 5] = s; }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < VF_THREADS / 32; ++w) a = join(a, part[w], inv);
-        P.stats[(size_t)row * P.chunks + chunk] = make_float4(a.m, a.s, __int_as_float(a.at), 0.f);
+    float top = part_m[0], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < VF_THREADS / 32; ++w) top = fmaxf(top, part_m[w]);
+    if (mine == top) {
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int k = VF_EACH - 1; k >= 0; --k)
+            if (l[k] == top) at = v0 + ((k / W) * VF_THREADS + tid) * W + k % W;
+        atomicMin(&place, at);
+    }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 0; w < VF_THREADS / 32; ++w) sum += part_m[w] == top ? part_s[w] : part_s[w] * exp2f((part_m[w] - top) * scale);
+        P.stats[(size_t)row * P.chunks + chunk] = make_float4(top, sum, __int_as_float(place), 0.f);
     }
 }
 
@@ -151,16 +132,17 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    double s = 0;
-    for (int w = 0; w < VF_THREADS / 32; ++w) s += part[w];
-    return s;
+    v = part[threadIdx.x & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // One cluster a request; each CTA of it walks by itself (the tree is small) and holds the weights of `slice` tokens of the row that the last token is drawn from.
 template <bool BF16>
-__global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_constant__ VerifyParams P) {
+__global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid_constant__ VerifyParams P) {
     extern __shared__ double w[];
-    __shared__ double node_z[VF_NODES], node_w[VF_NODES], part[VF_THREADS / 32], total_s[2];
+    __shared__ double node_z[VF_NODES], node_w[VF_NODES], part[32], total_s[2];
     __shared__ float node_m[VF_NODES];
     __shared__ int node_at[VF_NODES], parent[VF_NODES], token[VF_NODES], next[VF_NODES], path[VF_NODES], gone[VF_NODES];
     __shared__ int length, n_gone, finder;
@@ -170,7 +152,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_co
     const int rank = (int)cluster_rank(), ranks = (int)cluster_size();
     if (n == 0) {                                        // the whole cluster agrees
         if (rank == 0) {
-            for (int i = tid; i < T; i += VF_THREADS) { P.path[(size_t)b * T + i] = -1; P.out[(size_t)b * T + i] = -1; }
+            for (int i = tid; i < T; i += VF_WALKERS) { P.path[(size_t)b * T + i] = -1; P.out[(size_t)b * T + i] = -1; }
             if (tid == 0) P.count[b] = -1;
         }
         return;
@@ -184,8 +166,8 @@ __global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_co
         token[tid] = P.tokens[(size_t)b * T + tid];
         next[tid] = VF_NODES;
     }
-    if (tid == 0) { n_gone = 0; finder = VF_THREADS; }
-    for (int i = warp; i < n; i += VF_THREADS / 32) {    // the chunks of a node's row
+    if (tid == 0) { n_gone = 0; finder = VF_WALKERS; }
+    for (int i = warp; i < n; i += VF_WALKERS / 32) {    // the chunks of a node's row
         const float4* st = P.stats + ((size_t)b * T + i) * P.chunks;
         float m = -INFINITY;
         int at = 0x7fffffff;
@@ -243,7 +225,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_co
     __syncthreads();
     const int last = length, end = path[last];
     if (rank == 0) {
-        for (int i = tid; i < T; i += VF_THREADS) {
+        for (int i = tid; i < T; i += VF_WALKERS) {
             P.path[(size_t)b * T + i] = i <= last ? path[i] : -1;
             if (i != last) P.out[(size_t)b * T + i] = i < last ? token[path[i + 1]] : -1;
             else if (greedy) P.out[(size_t)b * T + i] = node_at[end];
@@ -254,26 +236,37 @@ __global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_co
     if (child && parent[tid] == end) gone[atomicAdd(&n_gone, 1)] = token[tid];
     const int v0 = rank * P.slice, len = max(0, min(P.slice, P.V - v0));
     const float m = node_m[end];
-    for (int k = tid; k < len; k += VF_THREADS) w[k] = weight(logit_at<BF16>(P, b, end, v0 + k), m, inv);
+    for (int k0 = tid; k0 < len; k0 += VF_TOGETHER * VF_WALKERS) {          // several at a time: loads and exponentials overlap
+        float l[VF_TOGETHER];
+        double x[VF_TOGETHER];
+#pragma unroll
+        for (int i = 0; i < VF_TOGETHER; ++i) l[i] = k0 + i * VF_WALKERS < len ? logit_at<BF16>(P, b, end, v0 + k0 + i * VF_WALKERS) : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VF_TOGETHER; ++i) x[i] = exp(((double)l[i] - (double)m) * inv);
+#pragma unroll
+        for (int i = 0; i < VF_TOGETHER; ++i)
+            if (k0 + i * VF_WALKERS < len) w[k0 + i * VF_WALKERS] = l[i] == -INFINITY ? 0.0 : l[i] == m ? 1.0 : x[i];
+    }
     __syncthreads();
     if (P.probs && n_gone > 0) {                         // what the draft's distribution leaves of the target's
         double s = 0;
-        for (int k = tid; k < len; k += VF_THREADS) s += w[k];
+        for (int k = tid; k < len; k += VF_WALKERS) s += w[k];
         s = block_sum(s, part);
         if (tid == 0) total_s[0] = s;
         cluster_sync();
         double z = 0;
         for (int r = 0; r < ranks; ++r) z += ld_cluster_f64(smem_u32(&total_s[0]), r);
         const float* q = P.probs + (size_t)b * P.p_batch + (size_t)end * P.p_row + v0;
-        for (int k = tid; k < len; k += VF_THREADS) w[k] = fmax(w[k] / z - (double)q[k], 0.0);
+        for (int k = tid; k < len; k += VF_WALKERS) w[k] = fmax(w[k] / z - (double)q[k], 0.0);
     } else if (tid < n_gone) {
         const int g = gone[tid] - v0;
         if (g >= 0 && g < len) w[g] = 0;
     }
     __syncthreads();
     // each thread sums a run of neighbours (an odd number: no two lanes of a warp meet in a bank), the block scans the sums
-    const int run = ((P.slice + VF_THREADS - 1) / VF_THREADS) | 1, k0 = min(len, tid * run), k1 = min(len, k0 + run);
+    const int run = ((P.slice + VF_WALKERS - 1) / VF_WALKERS) | 1, k0 = min(len, tid * run), k1 = min(len, k0 + run);
     double mine = 0;
+#pragma unroll 4
     for (int k = k0; k < k1; ++k) mine += w[k];
     double upto = mine;
 #pragma unroll
@@ -283,22 +276,31 @@ __global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_co
     }
     if (lane == 31) part[warp] = upto;
     __syncthreads();
-    double before = 0, sum = 0;
-    for (int x = 0; x < VF_THREADS / 32; ++x) {
-        if (x == warp) before = sum;
-        sum += part[x];
+    if (warp == 0) {                                     // the warps' sums, scanned by one of them
+        double x = part[lane], up = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += y;
+        }
+        part[lane] = up - x;
+        if (lane == 31) total_s[1] = up;
     }
-    if (tid == 0) total_s[1] = sum;
+    __syncthreads();
+    const double before = part[warp];
     cluster_sync();
-    double all = 0;
-    for (int r = 0; r < ranks; ++r) all += ld_cluster_f64(smem_u32(&total_s[1]), r);
+    double sums[VF_CLUSTER], all = 0;
+#pragma unroll
+    for (int r = 0; r < VF_CLUSTER; ++r) sums[r] = r < ranks ? ld_cluster_f64(smem_u32(&total_s[1]), r) : 0.0;
+#pragma unroll
+    for (int r = 0; r < VF_CLUSTER; ++r) all += sums[r];
     const double target = (double)P.u[(size_t)b * T] * all;
     int owner = -1;
     double base = 0, run_sum = 0;
-    for (int r = 0; r < ranks; ++r) {
-        const double s = ld_cluster_f64(smem_u32(&total_s[1]), r);
-        if (s > 0 && (owner < 0 || run_sum <= target)) { owner = r; base = run_sum; }       // the last part that starts at or below the target
-        run_sum += s;
+#pragma unroll
+    for (int r = 0; r < VF_CLUSTER; ++r) {
+        if (sums[r] > 0 && (owner < 0 || run_sum <= target)) { owner = r; base = run_sum; }       // the last part that starts at or below the target
+        run_sum += sums[r];
     }
     cluster_sync();                                      // nobody leaves while its sums are read
     if (owner < 0) {                                     // nothing is left to draw from
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_walk_kernel(const __grid_co
     const double aim = target - base;
     if (mine > 0 && before + upto > aim) atomicMin(&finder, tid);
     __syncthreads();
-    if (finder == VF_THREADS) {                          // rounding put the target behind the last sum: the last run with weight
+    if (finder == VF_WALKERS) {                          // rounding put the target behind the last sum: the last run with weight
         __syncthreads();
         if (tid == 0) finder = -1;
         __syncthreads();
@@ -342,7 +344,7 @@ int launch_walk(const VerifyParams& p, int cluster, cudaStream_t st) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(cluster, p.B);
-    cfg.blockDim = dim3(VF_THREADS);
+    cfg.blockDim = dim3(VF_WALKERS);
     cfg.dynamicSmemBytes = (size_t)p.slice * 8;
     cfg.stream = st;
     cudaLaunchAttribute at[2];

@@ -12,8 +12,10 @@ CUDA tensors go through csrc/paged_write.cu and csrc/paged_tree.cu; CPU tensors 
 slot outside its extent skips the access and reports it: ``ops.paged.check_status`` raises."""
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
+import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -40,41 +42,35 @@ def _decls(L):
         L.ptb_paged_tree_work_floats.restype = ll
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _index(t: torch.Tensor, like: torch.Tensor, shape: tuple, name: str) -> None:
-    """int32, contiguous, on the device of ``like``."""
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device:
-        raise ValueError(f"{name}: a contiguous int32 tensor {list(shape)} on {like.device} is needed, not {t.dtype} {list(t.shape)} on {t.device}")
+def _index(t: torch.Tensor, dev: torch.device, shape: tuple, name: str) -> None:
+    """int32, contiguous, on the device."""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name}: a contiguous int32 tensor {list(shape)} on {dev} is needed, not {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _pools(like, Hk: int, D: int, k_pages, v_pages, k_exp, v_exp) -> bool:
     """Checks a layer's pools; whether they are quantised."""
-    quant = k_pages.dtype == E4M3
-    _need(k_pages.dtype == v_pages.dtype and (quant or k_pages.dtype == like.dtype), f"pages: {k_pages.dtype} and {v_pages.dtype} for {like.dtype} tokens")
-    _need(k_pages.dim() == 4 and tuple(k_pages.shape[1:]) == (Hk, PAGE, D) and k_pages.shape == v_pages.shape,
-          f"pages: [page, {Hk}, {PAGE}, {D}] is needed, not {list(k_pages.shape)} and {list(v_pages.shape)}")
-    _need((k_exp is not None) == quant and (v_exp is not None) == quant, "pages: e4m3 pages come with exponents of keys and of values, others without")
-    for t in (k_pages, v_pages) + ((k_exp, v_exp) if quant else ()):
-        _need(t.is_contiguous() and t.device == like.device, f"pages: contiguous pools on {like.device} are needed")
+    quant, shape, dev = k_pages.dtype == E4M3, k_pages.shape, like.device
+    if k_pages.dtype != v_pages.dtype or not (quant or k_pages.dtype == like.dtype):
+        raise ValueError(f"pages: {k_pages.dtype} and {v_pages.dtype} for {like.dtype} tokens")
+    if len(shape) != 4 or shape[1] != Hk or shape[2] != PAGE or shape[3] != D or v_pages.shape != shape:
+        raise ValueError(f"pages: [page, {Hk}, {PAGE}, {D}] is needed, not {list(shape)} and {list(v_pages.shape)}")
+    if (k_exp is not None) != quant or (v_exp is not None) != quant:
+        raise ValueError("pages: e4m3 pages come with exponents of keys and of values, others without")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.device == dev and v_pages.device == dev):
+        raise ValueError(f"pages: contiguous pools on {dev} are needed")
     if quant:
-        _need(k_exp.dtype == v_exp.dtype == torch.uint8 and k_exp.shape == v_exp.shape == k_pages.shape[:3], "pages: exponents are uint8 [page, kv head, 64]")
+        for t in (k_exp, v_exp):
+            if t.dtype != torch.uint8 or t.shape != shape[:3] or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"pages: exponents are contiguous uint8 [page, kv head, 64] on {dev}")
     return quant
 
 
-def _on(t: torch.Tensor):
-    """The current stream of the tensor's device, for a launch on it."""
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
 class _Device:
-    """Makes a tensor's device the current one for the length of a launch, if it is not."""
+    """Makes a device the current one for the length of a launch, if it is not."""
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
 
     def __enter__(self):
         self.old = torch.cuda.current_device()
@@ -84,6 +80,10 @@ class _Device:
     def __exit__(self, *_):
         if self.old != self.index:
             torch.cuda.set_device(self.old)
+
+
+_looks = operator.attrgetter("shape", "dtype", "device")
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
 # ---------------------------------------------------------------------------------------------- e4m3 with an exponent a row
@@ -121,26 +121,35 @@ def paged_write(qkv: torch.Tensor, H: int, Hk: int, D: int, pos: torch.Tensor, r
     """Rotates q and k of the ``n`` tokens of ``qkv [n, >= (H + 2 Hk) D]`` (pairs (j, j + D/2)) to the positions ``pos`` and stores k and v at
     ``page_table[req[i], slot[i] // 64]``, place ``slot[i] % 64``.  ``slot`` None: the position; a negative one is not stored (padding).  No two tokens have one slot.  e4m3 pages
     come with ``k_exp`` and ``v_exp``.  Returns the rotated ``q [n, H D]`` and, if asked for, the rotated keys ``[n, Hk, D]`` as they were before quantising."""
+    width, dev = (H + 2 * Hk) * D, qkv.device
+    if qkv.dim() != 2 or qkv.shape[1] < width or H < 0 or Hk <= 0 or D <= 0 or D % 2:
+        raise ValueError(f"paged_write: rows of {width} values for {H} + 2 x {Hk} heads of {D} are needed, not {list(qkv.shape)}")
     n = qkv.shape[0]
-    _need(qkv.dim() == 2 and qkv.shape[1] >= (H + 2 * Hk) * D and H >= 0 and Hk > 0 and D > 0 and D % 2 == 0,
-          f"paged_write: rows of {(H + 2 * Hk) * D} values for {H} + 2 x {Hk} heads of {D} are needed, not {list(qkv.shape)}")
     quant = _pools(qkv, Hk, D, k_pages, v_pages, k_exp, v_exp)
-    for t, name in ((pos, "pos"), (req, "req")) + (((slot, "slot"),) if slot is not None else ()):
-        _index(t, qkv, (n,), "paged_write: " + name)
-    _need(page_table.dim() == 2, "paged_write: page_table [requests, pages]")
-    _index(page_table, qkv, tuple(page_table.shape), "paged_write: page_table")
-    _need(cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == D // 2 and cos.is_contiguous() and sin.is_contiguous()
-          and cos.device == sin.device == qkv.device, f"paged_write: contiguous fp32 tables [positions, {D // 2}] on {qkv.device} are needed")
+    _index(pos, dev, (n,), "paged_write: pos")
+    _index(req, dev, (n,), "paged_write: req")
+    if slot is not None:
+        _index(slot, dev, (n,), "paged_write: slot")
+    if page_table.dim() != 2:
+        raise ValueError("paged_write: page_table [requests, pages]")
+    _index(page_table, dev, page_table.shape, "paged_write: page_table")
+    if not (cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == D // 2 and cos.is_contiguous() and sin.is_contiguous()
+            and cos.device == dev and sin.device == dev):
+        raise ValueError(f"paged_write: contiguous fp32 tables [positions, {D // 2}] on {dev} are needed")
     if qkv.is_cuda:
-        _need(qkv.dtype == torch.bfloat16 and D in (64, 128), f"paged_write: bf16 tokens with heads of 64 or 128 are needed, not {qkv.dtype} and {D}")
-        if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) < (H + 2 * Hk) * D or qkv.data_ptr() % 16:      # a row starts on 16 bytes
-            qkv = qkv[:, :(H + 2 * Hk) * D].contiguous() if qkv.stride(1) != 1 or qkv.shape[1] != (H + 2 * Hk) * D else qkv.clone(memory_format=torch.contiguous_format)
-        q = torch.empty(n, H * D, dtype=qkv.dtype, device=qkv.device)
-        k = torch.empty(n, Hk, D, dtype=qkv.dtype, device=qkv.device) if want_k else None
-        with _Device(qkv):
-            N.check(N.lib().ptb_paged_write(qkv.data_ptr(), qkv.stride(0), n, H, Hk, D, pos.data_ptr(), N.ptr(slot), req.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                                            page_table.shape[0], k_pages.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), N.ptr(k), k_pages.data_ptr(),
-                                            v_pages.data_ptr(), N.ptr(k_exp), N.ptr(v_exp), _status(qkv.device).data_ptr(), _on(qkv)), "paged_write")
+        if qkv.dtype != torch.bfloat16 or D not in (64, 128):
+            raise ValueError(f"paged_write: bf16 tokens with heads of 64 or 128 are needed, not {qkv.dtype} and {D}")
+        ld, one = qkv.stride()
+        if one != 1 or ld % 8 or ld < width or qkv.data_ptr() % 16:      # a row starts on 16 bytes
+            qkv, ld = torch.empty(n, width, dtype=qkv.dtype, device=dev).copy_(qkv[:, :width]), width
+        q = torch.empty(n, H * D, dtype=torch.bfloat16, device=dev)
+        k = torch.empty(n, Hk, D, dtype=torch.bfloat16, device=dev) if want_k else None
+        with _Device(dev):
+            rc = N.lib().ptb_paged_write(qkv.data_ptr(), ld, n, H, Hk, D, pos.data_ptr(), N.ptr(slot), req.data_ptr(), page_table.data_ptr(), page_table.shape[1], page_table.shape[0],
+                                         k_pages.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), N.ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp),
+                                         N.ptr(v_exp), _status(dev).data_ptr(), _stream(dev.index))
+        if rc:
+            N.check(rc, "paged_write")
         return q, k
     x = qkv[:, :(H + 2 * Hk) * D].reshape(n, H + 2 * Hk, D).float()
     c, s = cos[pos.long()][:, None], sin[pos.long()][:, None]
@@ -162,10 +171,12 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
     """``parents [B, T]`` (a node before the node, -1 for the first) -> ``[B, T]`` int64: bit j of node i, whether i is j or has it among its ancestors.  On the
     host this is a few operations for each node; keep it there."""
     B, T = parents.shape
-    _need(1 <= T <= MAX_NODES, f"tree_mask: 1 to {MAX_NODES} nodes, not {T}")
+    if not 1 <= T <= MAX_NODES:
+        raise ValueError(f"tree_mask: 1 to {MAX_NODES} nodes, not {T}")
     mask = torch.zeros(B, T, dtype=torch.int64, device=parents.device)
     p = parents.long()
-    _need(bool(((p < torch.arange(T, device=p.device)) & (p >= -1)).all()), "tree_mask: a parent is a node before its child, or -1")
+    if not bool(((p < torch.arange(T, device=p.device)) & (p >= -1)).all()):
+        raise ValueError("tree_mask: a parent is a node before its child, or -1")
     for i in range(T):
         bit = (1 << i) - (1 << 64 if i == 63 else 0)
         up = mask.gather(1, p[:, i:i + 1].clamp_min(0)).squeeze(1)
@@ -179,30 +190,40 @@ def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.T
     """``q [B, T, >= H D]``: up to 64 drafted tokens of each request (heads packed along the row), node i of request b in slot ``lens[b] + i`` of the pages
     ``page_table[b]``.  It sees the ``lens[b]`` cached tokens and the nodes j of its request whose bit j is set in ``mask[b, i]`` (int64; None: a chain, nodes 0 to i).  ``nodes [B]``: how
     many of the T are there (None: all).  Returns ``[B, T, H D]``; rows behind ``nodes[b]`` and rows that see nothing are zeros.  e4m3 pages come with ``k_exp`` and ``v_exp``."""
-    _need(q.dim() == 3 and q.shape[2] >= H * D and Hk > 0 and H > 0 and H % Hk == 0, f"paged_attention_tree: [B, T, {H} x {D}] over {Hk} kv heads, not {list(q.shape)}")
-    B, T = q.shape[:2]
-    _need(1 <= T <= MAX_NODES, f"paged_attention_tree: 1 to {MAX_NODES} nodes a request, not {T}")
-    quant = _pools(q, Hk, D, k_pages, v_pages, k_exp, v_exp)
-    _index(lens, q, (B,), "paged_attention_tree: lens")
+    if q.dim() != 3 or Hk <= 0 or H <= 0 or H % Hk or q.shape[2] < H * D:
+        raise ValueError(f"paged_attention_tree: [B, T, {H} x {D}] over {Hk} kv heads, not {list(q.shape)}")
+    B, T, _ = q.shape
+    dev = q.device
+    if not 1 <= T <= MAX_NODES:
+        raise ValueError(f"paged_attention_tree: 1 to {MAX_NODES} nodes a request, not {T}")
+    _pools(q, Hk, D, k_pages, v_pages, k_exp, v_exp)
+    _index(lens, dev, (B,), "paged_attention_tree: lens")
     if nodes is not None:
-        _index(nodes, q, (B,), "paged_attention_tree: nodes")
-    _need(page_table.dim() == 2 and page_table.shape[0] == B, f"paged_attention_tree: a row of pages for each of {B} requests, not {list(page_table.shape)}")
-    _index(page_table, q, tuple(page_table.shape), "paged_attention_tree: page_table")
-    if mask is not None:
-        _need(mask.dtype == torch.int64 and tuple(mask.shape) == (B, T) and mask.is_contiguous() and mask.device == q.device,
-              f"paged_attention_tree: a contiguous int64 mask [{B}, {T}] on {q.device} is needed")
+        _index(nodes, dev, (B,), "paged_attention_tree: nodes")
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError(f"paged_attention_tree: a row of pages for each of {B} requests, not {list(page_table.shape)}")
+    _index(page_table, dev, page_table.shape, "paged_attention_tree: page_table")
+    if mask is not None and not (mask.dtype == torch.int64 and mask.shape == (B, T) and mask.is_contiguous() and mask.device == dev):
+        raise ValueError(f"paged_attention_tree: a contiguous int64 mask [{B}, {T}] on {dev} is needed")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"paged_attention_tree: a scale above zero is needed, not {scale}")
     if q.is_cuda:
-        _need(q.dtype == torch.bfloat16 and D in (64, 128), f"paged_attention_tree: bf16 queries with heads of 64 or 128 are needed, not {q.dtype} and {D}")
-        if q.stride(2) != 1 or q.stride(1) % 8 or q.stride(0) % 8 or q.data_ptr() % 16:
-            q = q.clone(memory_format=torch.contiguous_format) if (q.shape[2] % 8 == 0) else q[:, :, :H * D].clone(memory_format=torch.contiguous_format)
-        out = torch.empty(B, T, H * D, dtype=q.dtype, device=q.device)
+        if q.dtype != torch.bfloat16 or D not in (64, 128):
+            raise ValueError(f"paged_attention_tree: bf16 queries with heads of 64 or 128 are needed, not {q.dtype} and {D}")
+        s0, s1, s2 = q.stride()
+        if s2 != 1 or s1 % 8 or s0 % 8 or q.data_ptr() % 16:             # a row starts on 16 bytes
+            q = torch.empty(B, T, H * D, dtype=q.dtype, device=dev).copy_(q[:, :, :H * D])
+            s0, s1, s2 = q.stride()
+        out = torch.empty(B, T, H * D, dtype=torch.bfloat16, device=dev)
         L = N.lib()
-        with _Device(q):
-            work = torch.empty(L.ptb_paged_tree_work_floats(T, H, Hk, D), dtype=torch.float32, device=q.device)
-            N.check(L.ptb_paged_attn_tree(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), B, T, H, Hk, D, lens.data_ptr(), N.ptr(nodes), N.ptr(mask), page_table.data_ptr(),
-                                          page_table.stride(0), k_pages.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp), N.ptr(v_exp), scale, work.data_ptr(),
-                                          _status(q.device).data_ptr(), _on(q)), "paged_attention_tree")
+        with _Device(dev):
+            work = torch.empty(L.ptb_paged_tree_work_floats(T, H, Hk, D), dtype=torch.float32, device=dev)
+            rc = L.ptb_paged_attn_tree(q.data_ptr(), s0, s1, out.data_ptr(), B, T, H, Hk, D, lens.data_ptr(), N.ptr(nodes), N.ptr(mask), page_table.data_ptr(), page_table.shape[1],
+                                       k_pages.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp), N.ptr(v_exp), scale, work.data_ptr(), _status(dev).data_ptr(),
+                                       _stream(dev.index))
+        if rc:
+            N.check(rc, "paged_attention_tree")
         return out
     return paged_attention_tree_reference(q, H, Hk, D, lens, page_table, k_pages, v_pages, mask, nodes, k_exp, v_exp, scale)
 
@@ -241,34 +262,44 @@ def paged_keep(layers: Sequence[Sequence[Optional[torch.Tensor]]], lens: torch.T
     """Moves the cache entries of each request's accepted drafted tokens from slot ``lens[b] + path[b, j]`` to ``lens[b] + j`` for j = 1 .. ``count[b]``, in every layer's
     pools.  ``layers``: (k_pages, v_pages) or (k_pages, v_pages, k_exp, v_exp) of each layer, of one shape; ``path [B, T]`` and ``count [B]`` are what
     :func:`~prometorch_b200.ops.verify.verify_drafts` gives (a path ascends; a count below one moves nothing); ``page_table [B, pages]``: a row for each request."""
-    if not len(layers):
+    n = len(layers)
+    if not n:
         return
-    flat = []
-    k0 = layers[0][0]
-    Hk, D, quant = k0.shape[1], k0.shape[3], k0.dtype == E4M3
-    for l in layers:
-        k, v, ke, ve = l if len(l) == 4 else (*l, None, None)
-        if k.shape != k0.shape or k.dtype != k0.dtype or v.shape != k0.shape or v.dtype != k0.dtype or not k.is_contiguous() or not v.is_contiguous() or k.device != k0.device \
-                or v.device != k0.device or (ke is None) == quant or (ve is None) == quant:
-            raise ValueError("paged_keep: layers need contiguous pools of one shape, type and device, with exponents if they are e4m3 and only then")
-        if quant and not (ke.dtype == ve.dtype == torch.uint8 and ke.shape == ve.shape == k0.shape[:3] and ke.is_contiguous() and ve.is_contiguous()
-                          and ke.device == ve.device == k0.device):
-            raise ValueError("paged_keep: exponents are contiguous uint8 [page, kv head, 64]")
-        flat += [k, v, ke, ve]
-    _need(k0.dim() == 4 and k0.shape[2] == PAGE and path.dim() == 2, "paged_keep: pages [page, kv head, 64, D] and a path [B, T]")
+    ks, vs, kes, ves = zip(*[l if len(l) == 4 else (*l, None, None) for l in layers])
+    k0 = ks[0]
+    dev, quant = k0.device, k0.dtype == E4M3
+    if k0.dim() != 4 or k0.shape[2] != PAGE:
+        raise ValueError(f"paged_keep: pages [page, kv head, {PAGE}, D], not {list(k0.shape)}")
+    pools, exps = ks + vs, kes + ves
+    if list(map(_looks, pools)).count(_looks(k0)) != 2 * n or not all(map(torch.Tensor.is_contiguous, pools)):
+        raise ValueError("paged_keep: layers need contiguous pools of one shape, type and device")
+    none = sum(e is None for e in exps)
+    if not quant and none != 2 * n:
+        raise ValueError("paged_keep: only e4m3 pools have exponents")
+    if quant and (none or list(map(_looks, exps)).count((k0.shape[:3], torch.uint8, dev)) != 2 * n or not all(map(torch.Tensor.is_contiguous, exps))):
+        raise ValueError(f"paged_keep: exponents are contiguous uint8 [page, kv head, {PAGE}] on {dev}, for e4m3 pools all of them")
+    if path.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] != path.shape[0]:
+        raise ValueError(f"paged_keep: a path [B, T] and a row of pages for each request, not {list(path.shape)} and {list(page_table.shape)}")
     B, T = path.shape
-    _index(path, k0, (B, T), "paged_keep: path")
-    _index(lens, k0, (B,), "paged_keep: lens")
-    _index(count, k0, (B,), "paged_keep: count")
-    _need(page_table.dim() == 2 and page_table.shape[0] == B, f"paged_keep: a row of pages for each of {B} requests, not {list(page_table.shape)}")
-    _index(page_table, k0, tuple(page_table.shape), "paged_keep: page_table")
+    if T > MAX_NODES:
+        raise ValueError(f"paged_keep: up to {MAX_NODES} nodes a request, not {T}")
+    _index(path, dev, (B, T), "paged_keep: path")
+    _index(lens, dev, (B,), "paged_keep: lens")
+    _index(count, dev, (B,), "paged_keep: count")
+    _index(page_table, dev, page_table.shape, "paged_keep: page_table")
     if k0.is_cuda:
-        _need(D * k0.element_size() % 16 == 0, f"paged_keep: rows of 16-byte pieces are needed, not {D} x {k0.element_size()} bytes")
-        ptrs = (C.c_void_p * len(flat))(*[t.data_ptr() if t is not None else None for t in flat])
-        with _Device(k0):
-            N.check(N.lib().ptb_paged_keep(ptrs, len(layers), B, T, Hk, D * k0.element_size(), k0.shape[0], lens.data_ptr(), path.data_ptr(), count.data_ptr(), page_table.data_ptr(),
-                                           page_table.stride(0), _status(k0.device).data_ptr(), _on(k0)), "paged_keep")
+        row = k0.shape[3] * k0.element_size()
+        if row % 16:
+            raise ValueError(f"paged_keep: rows of 16-byte pieces are needed, not {row} bytes")
+        at = list(map(torch.Tensor.data_ptr, pools + exps)) if quant else list(map(torch.Tensor.data_ptr, pools)) + [0] * (2 * n)
+        ptrs = array.array("Q", at)                  # all keys, all values, all exponents of keys, all of values
+        with _Device(dev):
+            rc = N.lib().ptb_paged_keep(ptrs.buffer_info()[0], n, B, T, k0.shape[1], row, k0.shape[0], lens.data_ptr(), path.data_ptr(), count.data_ptr(), page_table.data_ptr(),
+                                        page_table.shape[1], _status(dev).data_ptr(), _stream(dev.index))
+        if rc:
+            N.check(rc, "paged_keep")
         return
+    flat = pools + exps
     for b in range(B):
         n = min(int(count[b]), T - 1)
         if n < 1:

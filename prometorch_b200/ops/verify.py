@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native as N
-from .paged_tree import _Device, _index, _need, _on
+from .paged_tree import _Device, _index, _stream
 
 MAX_NODES = 64
 
@@ -28,6 +28,11 @@ def _decls(L):
         L.ptb_verify_work_bytes.restype = ll
 
 
+def _floats(t: torch.Tensor, dev: torch.device, shape: tuple, name: str) -> None:
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"verify_drafts: {name} is a contiguous fp32 tensor {list(shape)} on {dev}, not {t.dtype} {list(t.shape)} on {t.device}")
+
+
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor, parents: Optional[torch.Tensor] = None,
                   nodes: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``logits [B, T, V]`` (fp32 or bf16): what the target says behind each of a request's T nodes; node 0 is the latest token, the others are drafted.  ``tokens [B, T]`` (int32):
@@ -40,31 +45,41 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, t
 
     A logit of -inf (or NaN) is a token of probability zero; where nothing is left to draw from, the arg-max of the row is taken.  Siblings with one token count
     once.  A token outside the vocabulary is rejected, a node whose parent does not come before it is never reached."""
-    _need(logits.dim() == 3 and logits.dtype in (torch.float32, torch.bfloat16), f"verify_drafts: fp32 or bf16 logits [B, T, V] are needed, not {logits.dtype} {list(logits.shape)}")
+    if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"verify_drafts: fp32 or bf16 logits [B, T, V] are needed, not {logits.dtype} {list(logits.shape)}")
     B, T, V = logits.shape
-    _need(1 <= T <= MAX_NODES and V >= 1, f"verify_drafts: 1 to {MAX_NODES} nodes a request and a vocabulary, not {T} and {V}")
-    _index(tokens, logits, (B, T), "verify_drafts: tokens")
+    dev = logits.device
+    if not 1 <= T <= MAX_NODES or V < 1:
+        raise ValueError(f"verify_drafts: 1 to {MAX_NODES} nodes a request and a vocabulary, not {T} and {V}")
+    _index(tokens, dev, (B, T), "verify_drafts: tokens")
     if parents is not None:
-        _index(parents, logits, (B, T), "verify_drafts: parents")
-        _need(draft_probs is None, "verify_drafts: draft probabilities go with chains")
+        _index(parents, dev, (B, T), "verify_drafts: parents")
+        if draft_probs is not None:
+            raise ValueError("verify_drafts: draft probabilities go with chains")
     if nodes is not None:
-        _index(nodes, logits, (B,), "verify_drafts: nodes")
-    for t, shape, name in ((u, (B, T), "u"), (temperature, (B,), "temperature")) + (((draft_probs, (B, T, V), "draft_probs"),) if draft_probs is not None else ()):
-        _need(t.dtype == torch.float32 and tuple(t.shape) == shape and t.device == logits.device and (t.is_contiguous() or t is draft_probs),
-              f"verify_drafts: {name} is fp32 {list(shape)} on {logits.device}, not {t.dtype} {list(t.shape)} on {t.device}")
+        _index(nodes, dev, (B,), "verify_drafts: nodes")
+    _floats(u, dev, (B, T), "u")
+    _floats(temperature, dev, (B,), "temperature")
+    if draft_probs is not None and (draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape or draft_probs.device != dev):
+        raise ValueError(f"verify_drafts: draft_probs are fp32 {[B, T, V]} on {dev}, not {draft_probs.dtype} {list(draft_probs.shape)} on {draft_probs.device}")
     if logits.is_cuda:
-        logits = logits if logits.stride(2) == 1 else logits.contiguous()
-        draft_probs = draft_probs if draft_probs is None or draft_probs.stride(2) == 1 else draft_probs.contiguous()
-        dev = logits.device
-        path, out = torch.empty(B, T, dtype=torch.int32, device=dev), torch.empty(B, T, dtype=torch.int32, device=dev)
-        count = torch.empty(B, dtype=torch.int32, device=dev)
+        if logits.stride(2) != 1:
+            logits = logits.contiguous()
+        p_batch = p_row = 0
+        if draft_probs is not None:
+            if draft_probs.stride(2) != 1:
+                draft_probs = draft_probs.contiguous()
+            p_batch, p_row, _ = draft_probs.stride()
+        l_batch, l_row, _ = logits.stride()
         L = N.lib()
-        work = torch.empty(L.ptb_verify_work_bytes(B, T, V), dtype=torch.uint8, device=dev)
-        with _Device(logits):
-            N.check(L.ptb_verify_drafts(logits.data_ptr(), int(logits.dtype == torch.bfloat16), logits.stride(0), logits.stride(1), N.ptr(draft_probs),
-                                        draft_probs.stride(0) if draft_probs is not None else 0, draft_probs.stride(1) if draft_probs is not None else 0, tokens.data_ptr(),
-                                        N.ptr(parents), N.ptr(nodes), u.data_ptr(), temperature.data_ptr(), work.data_ptr(), path.data_ptr(), count.data_ptr(), out.data_ptr(), B, T, V,
-                                        _on(logits)), "verify_drafts")
+        ints = torch.empty((2 * T + 1) * B, dtype=torch.int32, device=dev)
+        path, out, count = ints[:B * T].view(B, T), ints[B * T:2 * B * T].view(B, T), ints[2 * B * T:]
+        with _Device(dev):
+            work = torch.empty(L.ptb_verify_work_bytes(B, T, V), dtype=torch.uint8, device=dev)
+            rc = L.ptb_verify_drafts(logits.data_ptr(), int(logits.dtype == torch.bfloat16), l_batch, l_row, N.ptr(draft_probs), p_batch, p_row, tokens.data_ptr(), N.ptr(parents),
+                                     N.ptr(nodes), u.data_ptr(), temperature.data_ptr(), work.data_ptr(), path.data_ptr(), count.data_ptr(), out.data_ptr(), B, T, V, _stream(dev.index))
+        if rc:
+            N.check(rc, "verify_drafts")
         return path, count, out
     return verify_drafts_reference(logits, tokens, u, temperature, parents, nodes, draft_probs)
 

@@ -126,7 +126,7 @@ def call_attend(**kw):
                                 dict(page_table=i32(0, 1)), dict(page_table=i32(0, 1, 0, 1).view(2, 2)), dict(nodes=i32(1, 1)), dict(mask=torch.zeros(1, 3, dtype=torch.int32)),
                                 dict(mask=torch.zeros(1, 2, dtype=torch.int64)), dict(k_exp=torch.zeros(2, 2, 64, dtype=torch.uint8)), dict(k_pages=torch.zeros(2, 2, 64, 32)),
                                 dict(v_pages=torch.zeros(3, 2, 64, 64)), dict(quant=True, k_exp=None), dict(quant=True, v_exp=torch.zeros(2, 2, 64)), dict(k_pages=torch.zeros(2, 2, 64, 64).bfloat16()),
-                                dict(k_pages=torch.zeros(2, 64, 2, 64).transpose(1, 2))])
+                                dict(k_pages=torch.zeros(2, 64, 2, 64).transpose(1, 2)), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf)])
 def test_attention_refuses(kw):
     with pytest.raises(ValueError):
         call_attend(**kw)
@@ -187,7 +187,7 @@ def test_native_entries_refuse():
 
     def attend(q=BASE, q_batch=1024, q_row=512, B=1, T=2, H=4, Hk=2, D=128, stride=4, pages=8, k=BASE, v=BASE, ke=None, ve=None, work=BASE):
         return refused(L.ptb_paged_attn_tree(q, q_batch, q_row, BASE, B, T, H, Hk, D, BASE, None, None, BASE, stride, pages, k, v, ke, ve, 1.0, work, BASE, None))
-    for kw, word in ((dict(T=65), "nodes"), (dict(T=0), "nodes"), (dict(B=5000), "requests"), (dict(H=5), "heads"), (dict(D=96), "head size"), (dict(q=BASE + 4), "8 bytes"), (dict(q_row=514), "8 bytes"),
+    for kw, word in ((dict(T=65), "nodes"), (dict(T=0), "nodes"), (dict(B=5000), "requests"), (dict(H=5), "heads"), (dict(D=96), "head size"), (dict(q=BASE + 8), "16 bytes"), (dict(q_row=516), "16 bytes"),
                      (dict(k=BASE + 8), "16-byte"), (dict(v=BASE + 4), "16-byte"), (dict(ke=BASE), "belong together"), (dict(work=BASE + 8), "16-byte"), (dict(stride=0), "no pages"),
                      (dict(pages=1 << 28), "31 bits")):
         assert word in (attend(**kw) or ""), kw
