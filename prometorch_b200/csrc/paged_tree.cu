@@ -105,6 +105,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
     __syncthreads();
     const int all = starts[P.B], per = units_per_cta(all, P.ctas);
     const int u0 = (int)min((long long)all, (long long)blockIdx.x * per), u1 = min(all, u0 + per);
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= P.B; b += THREADS) P.starts[b] = starts[b];
     if (u0 >= u1) return;
 
     // ---- fetching: stage s of the ring takes the pieces s, s + STAGES, ... of this warp
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                     a = max(a, max(max(raw[s].x & 0x7fffu, (raw[s].x >> 16) & 0x7fffu), max(raw[s].y & 0x7fffu, (raw[s].y >> 16) & 0x7fffu)));
                 a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
                 a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-                const int k = min(253, max(1, (int)(a >> 7)));               // biased exponent
+                const int k = min(253, max(40, (int)(a >> 7)));              // biased exponent
                 const float down = __uint_as_float((uint32_t)(254 - k) << 23);
                 fac[x] *= __uint_as_float((uint32_t)k << 23);
 #pragma unroll
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                     o[v_elem<D, Q8>(i / 8, i % 8 + 1)] = __float2bfloat16_rn(on ? o1 / L : 0.f);
                 }
             } else {
-                *reinterpret_cast<float2*>(wk + (size_t)row * D + i) = make_float2(o0, o1);
+                *reinterpret_cast<float2*>(wk + ((i / 8) * ROWS + row) * 8 + i % 8) = make_float2(o0, o1);
                 if (i == 0) *reinterpret_cast<float2*>(wk + (size_t)ROWS * D + 2 * row) = make_float2(M, L);
             }
         }
@@ -440,84 +442,81 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
     }
 }
 
-// The partial results of items: one block per (sixteen rows of an item, 32 columns); and the rows that no unit belongs to, which are zeros.  NATURAL: partial rows are in the
-// order of the head, and every item has partial results; else place i of a row is column i % 8 of tile i / 8, and an item of one CTA is written already.
-constexpr int MERGE_THREADS = 256;
+// The partial results of items: one block per sixteen rows of an item, a thread (row, eight columns); and the rows that no unit belongs to, which are zeros.  NATURAL: partial
+// columns are in the order of the head, and every item has partial results; else place i of a row is column i % 8 of tile i / 8, and an item of one CTA is written already.
 template <int D, bool Q8, bool NATURAL>
-__global__ void __launch_bounds__(MERGE_THREADS) paged_tree_merge_kernel(const __grid_constant__ Params P) {
-    __shared__ int part[2][MERGE_THREADS / 32];
+__global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_constant__ Params P) {
     pdl_wait();
     pdl_launch_dependents();
-    const int b = blockIdx.y, groups = min(P.tile_rows, (P.T * P.G + 15) / 16 * 16) / 16, per_item = groups * (D / 32);
-    const int i = blockIdx.x / per_item, sub = blockIdx.x - i * per_item, row0 = sub / (D / 32) * 16, col0 = sub % (D / 32) * 32;
+    const int b = blockIdx.y, groups = min(P.tile_rows, (P.T * P.G + 15) / 16 * 16) / 16;
+    const int i = blockIdx.x / groups, row0 = (blockIdx.x - i * groups) * 16;
     const int tile = i / P.Hk, kvh = i - tile * P.Hk;
     const Req r = req_of(P, b);
-    const int row = threadIdx.x / 16, col = col0 + (threadIdx.x % 16) * 2, at = tile * P.tile_rows + row0 + row, node = at / P.G, g = at - node * P.G;
-    const bool empty = tile >= r.tiles || (tile * P.tile_rows + row0) / P.G >= r.nodes;          // none of the sixteen rows is there
-    float o0 = 0.f, o1 = 0.f, L = 0.f, M = -INFINITY;
-    if (!empty) {
-        // this request's first unit, and all units
-        int before = 0, all = 0;
-        for (int x = threadIdx.x; x < P.B; x += MERGE_THREADS) {
-            const int u = units_of(P, req_of(P, x));
-            all += u;
-            if (x < b) before += u;
-        }
+    const int row = row0 + threadIdx.x % 16, c8 = threadIdx.x / 16, at = tile * P.tile_rows + row, node = at / P.G, g = at - node * P.G;
+    float o[8], L = 0.f, M = -INFINITY;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) { before += __shfl_xor_sync(0xffffffffu, before, o); all += __shfl_xor_sync(0xffffffffu, all, o); }
-        if ((threadIdx.x & 31) == 0) { part[0][threadIdx.x >> 5] = before; part[1][threadIdx.x >> 5] = all; }
-        __syncthreads();
-        before = all = 0;
-        for (int w = 0; w < MERGE_THREADS / 32; ++w) { before += part[0][w]; all += part[1][w]; }
-        const int per = units_per_cta(all, P.ctas), a = before + i * r.units, e = a + r.units;
+    for (int x = 0; x < 8; ++x) o[x] = 0.f;
+    if (tile < r.tiles && (tile * P.tile_rows + row0) / P.G < r.nodes) {     // some of the sixteen rows are there
+        const int per = units_per_cta(P.starts[P.B], P.ctas), a = P.starts[b] + i * r.units, e = a + r.units;
         const int c0 = a / per, c1 = (e - 1) / per, n = (c1 - c0 + 1) * P.parts;
         if (!NATURAL && c0 == c1) return;                // written already
-        // sixteen parts at a time: thread (row, k) fetches the maximum and the sum of part k, and every thread its two columns of all sixteen, before any of them is needed
         auto from = [&](int k) {                         // slot 0: the run begins in (or with) this item
             const int c = c0 + k / P.parts;
             return P.work + partial_at(P, c, c * per >= a ? 0 : 1, k % P.parts, D);
         };
-        for (int k0 = 0; k0 < n; k0 += 16) {
-            const int k = k0 + threadIdx.x % 16;
-            float2 ml = make_float2(-INFINITY, 0.f), v[16];
-            if (k < n) ml = *reinterpret_cast<const float2*>(from(k) + (size_t)P.tile_rows * D + 2 * (row0 + row));
+        constexpr int AT_ONCE = 4;                       // fetched together, before any of them is needed
+        for (int k0 = 0; k0 < n; k0 += AT_ONCE) {
+            float2 ml[AT_ONCE];
+            float4 v[AT_ONCE][2];
 #pragma unroll
-            for (int x = 0; x < 16; ++x)
-                if (k0 + x < n) v[x] = *reinterpret_cast<const float2*>(from(k0 + x) + (size_t)(row0 + row) * D + col);
-            float mx = ml.x;
+            for (int x = 0; x < AT_ONCE; ++x)
+                if (k0 + x < n) {
+                    const float* p = from(k0 + x);
+                    ml[x] = *reinterpret_cast<const float2*>(p + (size_t)P.tile_rows * D + 2 * row);
+                    const float4* q = reinterpret_cast<const float4*>(p + (size_t)(c8 * P.tile_rows + row) * 8);
+                    v[x][0] = q[0];
+                    v[x][1] = q[1];
+                } else {
+                    ml[x] = make_float2(-INFINITY, 0.f);
+                }
+            float mn = M;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float mn = fmaxf(M, mx), old = M == -INFINITY ? 0.f : exp2f(M - mn), f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-            float s = ml.x == -INFINITY ? 0.f : ml.y * f;
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            L = L * old + s;
-            o0 *= old;
-            o1 *= old;
+            for (int x = 0; x < AT_ONCE; ++x) mn = fmaxf(mn, ml[x].x);
+            const float old = M == -INFINITY ? 0.f : exp2f(M - mn);
             M = mn;
+            L *= old;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const float w = __shfl_sync(0xffffffffu, f, (threadIdx.x & 16) + x);
-                if (k0 + x < n && w != 0.f) { o0 += v[x].x * w; o1 += v[x].y * w; }
+            for (int x = 0; x < 8; ++x) o[x] *= old;
+#pragma unroll
+            for (int x = 0; x < AT_ONCE; ++x) {
+                if (ml[x].x == -INFINITY) continue;      // that part saw nothing, and may not have written its accumulators
+                const float w = exp2f(ml[x].x - mn);
+                L += ml[x].y * w;
+                o[0] += v[x][0].x * w; o[1] += v[x][0].y * w; o[2] += v[x][0].z * w; o[3] += v[x][0].w * w;
+                o[4] += v[x][1].x * w; o[5] += v[x][1].y * w; o[6] += v[x][1].z * w; o[7] += v[x][1].w * w;
             }
         }
     }
     if (node >= P.T) return;
     const bool on = node < r.nodes && L != 0.f;
-    __nv_bfloat16* o = P.out + (((size_t)b * P.T + node) * P.H + kvh * P.G + g) * D;
-    const float r0 = on ? o0 / L : 0.f, r1 = on ? o1 / L : 0.f;
+    const float inv = on ? 1.f / L : 0.f;
+    __nv_bfloat16* out = P.out + (((size_t)b * P.T + node) * P.H + kvh * P.G + g) * D;
     if constexpr (NATURAL) {
-        *reinterpret_cast<__nv_bfloat162*>(o + col) = __floats2bfloat162_rn(r0, r1);
+        uint4 w;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) h[x] = __floats2bfloat162_rn(on ? o[2 * x] * inv : 0.f, on ? o[2 * x + 1] * inv : 0.f);
+        *reinterpret_cast<uint4*>(out + 8 * c8) = w;
     } else {
-        o[v_elem<D, Q8>(col / 8, col % 8)] = __float2bfloat16_rn(r0);
-        o[v_elem<D, Q8>(col / 8, col % 8 + 1)] = __float2bfloat16_rn(r1);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) out[v_elem<D, Q8>(c8, x)] = __float2bfloat16_rn(on ? o[x] * inv : 0.f);
     }
 }
 
 template <int D, bool Q8, bool NATURAL>
 int launch_merge(const Params& p, cudaStream_t st) {
     const int groups = (p.T * p.G + 15) / 16 < p.tile_rows / 16 ? (p.T * p.G + 15) / 16 : p.tile_rows / 16;
-    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, Q8, NATURAL>, dim3(p.tiles * p.Hk * groups * (D / 32), p.B), dim3(MERGE_THREADS), 0, st, ptb_pdl_enabled(), p));
+    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, Q8, NATURAL>, dim3(p.tiles * p.Hk * groups, p.B), dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }
@@ -565,10 +564,10 @@ int parts_of(int tile_rows) { return tile_rows == ROWS ? 1 : 2; }
 using namespace ptb;
 
 // Floats of workspace that ptb_paged_attn_tree needs.
-PTB_API long long ptb_paged_tree_work_floats(int T, int H, int Hk, int D) {
+PTB_API long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D) {
     if (Hk <= 0 || T <= 0) return 0;
     const int rows = tree::tile_rows_of(T * (H / Hk));
-    return (long long)tree::sm_count() * 2 * tree::parts_of(rows) * (long long)tree::partial_floats(rows, D);
+    return (long long)tree::sm_count() * 2 * tree::parts_of(rows) * (long long)tree::partial_floats(rows, D) + B + 1;
 }
 
 // T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with
@@ -588,7 +587,7 @@ PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_ro
         return -1;
     }
     if (!k_exp != !v_exp) { ptb_set_error("paged attention of trees: exponents of keys and of values belong together"); return -1; }
-    if (!(scale > 0.f) || !(scale < 3e38f)) { ptb_set_error("paged attention of trees: a scale above zero is needed"); return -1; }
+    if (!(scale > 1e-30f) || !(scale < 1e30f)) { ptb_set_error("paged attention of trees: a scale between 1e-30 and 1e30 is needed"); return -1; }
     if (pt_stride < 1 || n_pages < 1) { ptb_set_error("paged attention of trees: no pages"); return -1; }
     tree::Params p;
     memset(&p, 0, sizeof(p));
@@ -600,6 +599,7 @@ PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_ro
     p.unit = p.tile_rows == tree::ROWS ? tree::PAGE : 128;
     p.parts = tree::parts_of(p.tile_rows);
     p.ctas = tree::sm_count();
+    p.starts = reinterpret_cast<int*>(work + (size_t)p.ctas * 2 * p.parts * tree::partial_floats(p.tile_rows, D));
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = status;
     if ((long long)B * p.tiles * Hk * pt_stride > 0x7fffffffll || (long long)n_pages * Hk * 128 > 0x7fffffffll) { ptb_set_error("paged attention of trees: more pages than 31 bits count"); return -1; }

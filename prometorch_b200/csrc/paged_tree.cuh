@@ -33,7 +33,8 @@ struct Params {
     const uint8_t* k_exp;                // [n_pages, Hk, 64] biased exponents, null: bf16 pages
     const uint8_t* v_exp;
     const uint8_t* v_raw;                // the pool of values, as bytes
-    float* work;                         // partials of cut items
+    float* work;                         // partial results of items
+    int* starts;                         // [B + 1], behind them: units before each request
     int B, T, H, Hk, G;
     int tile_rows, tiles;                // rows of a tile, tiles of T nodes
     int unit;                            // tokens of a unit
@@ -92,7 +93,7 @@ __device__ __forceinline__ void plan(const Params& P, int* starts, int* part) {
 __device__ __forceinline__ int units_per_cta(int all, int ctas) { return max(1, (all + ctas - 1) / ctas); }
 
 // A CTA leaves partial results of at most two items: the one its run begins in (slot 0) and the one it ends in (slot 1; where both are the same, slot 0).
-// One is [rows][D] accumulators, then [rows] (maximum, sum).
+// One is [D / 8][rows][8] accumulators (threads that own a row each then write whole lines), then [rows] (maximum, sum).
 __device__ __forceinline__ size_t partial_at(const Params& P, int cta, int slot, int part, int D) { return (size_t)((cta * 2 + slot) * P.parts + part) * partial_floats(P.tile_rows, D); }
 
 // An item and the part of it in a CTA's run: n units from `first` on.

@@ -1,13 +1,13 @@
 // More than sixteen rows of drafted tokens against a paged cache, both products on the 5th-generation tensor cores; see paged_tree.cuh.
 //
-// One CTA per SM walks its run of units, blocks of 128 tokens (two pages).  Rows lie along the 128 lanes of tensor memory.  Sixteen warps:
+// One CTA per SM walks its run of units, blocks of 128 tokens (two pages).  Rows lie along the 128 lanes of tensor memory.  Sixteen warps, or (e4m3) twenty:
 //   warp 0      brings pages: bf16 keys and values straight to the tiles the products read; e4m3 ones, and their exponents, to a ring of raw pages;
 //   warp 1      owns tensor memory and issues S(j) = Q K_j^T and O += P(j) V_j;
 //   warps 4-11  softmax, two groups of four warps that take every other block, each with a score buffer, a running maximum and sum and an output accumulator of its
 //               own: while one group works on its scores the tensor cores work for the other.  A thread owns a row, so nothing is exchanged.  Weights go back to
 //               tensor memory, over the scores they came from, as the first operand of the second product.  The accumulator is scaled, by its own threads, only
 //               when a row's maximum has grown by 2^8;
-//   warps 12-15 e4m3: the raw page to fp16 tiles.  bf16: of a block with drafted tokens they clear the values that must not meet a weight.
+//   warps 12-19 e4m3: raw pages to fp16 tiles, four warps the keys and four the values.  12-15, bf16: of a block with drafted tokens they clear the values that must not meet a weight.
 //
 // e4m3 values times a power of two are exact in fp16, which has five more exponents than they need: a block's keys are brought to the largest exponent among them (which
 // then scales the block's scores), the values to a reference that only grows and that the accumulator follows.  A key or a value more than 2^30 below those loses bits that
@@ -27,8 +27,13 @@ namespace {
 
 using namespace ptb::gemm;
 
-constexpr int BQ = 128, BLOCK = 128, THREADS = 512;
-constexpr int SOFTMAX_WARP = 4, CONVERT_WARP = 12;
+constexpr int BQ = 128, BLOCK = 128;
+constexpr int SOFTMAX_WARP = 4, CONVERT_WARP = 12;       // four warps of converters behind the latter, or (e4m3) eight
+// Threads, and registers a thread of the softmax and of the other warps: the launch's shared out anew (512 x 128 = 256 x 184 + 256 x 72; 640 x 96 = 256 x 120 + 384 x 80).  A softmax
+// thread holds its 128 scores (64 of them): one wait for tensor memory a block, or three, in place of eight; 4900 clocks from the scores to the weights became 2000.
+template <bool Q8> struct Split { static constexpr int THREADS = Q8 ? 640 : 512, SOFTMAX = Q8 ? 120 : 184, OTHER = Q8 ? 80 : 72; };
+template <int R> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
 template <int D, bool Q8>
 struct Sm {
@@ -61,6 +66,14 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t* r) {
 }
 __device__ __forceinline__ void convert_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y)); return r; }
+__device__ __forceinline__ uint64_t both(float x) { return pair(__float_as_uint(x), __float_as_uint(x)); }
+__device__ __forceinline__ void apart(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
 // fp16 or bf16 operands, fp32 accumulators.
 template <bool Q8>
 constexpr uint32_t idesc(int n, int b_mn) { return instr_desc(BQ, n, 0, b_mn) & (Q8 ? ~((1u << 7) | (1u << 10)) : ~0u); }
@@ -84,11 +97,12 @@ __device__ __forceinline__ __half2 half2_pow2(int e) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
 
+template <bool X> struct Flag { static constexpr bool value = X; };
 constexpr int V_ROOM = 3;                // fp16 values stand for value * 2^(reference - V_ROOM): the reference may be passed by 2^4 before it has to grow
 constexpr int K_ROOM = 7;                // 448 * 2^7 fits fp16
 
 template <int D, bool Q8>
-__global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params P) {
     using S = Sm<D, Q8>;
     constexpr int NK = S::NK, NV = S::NV, NR = Q8 ? S::NR : 1;
     extern __shared__ uint8_t smem_raw[];
@@ -103,8 +117,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
     int* k_ref = bad_pages + 8;                                        // [8] by block: biased exponent that its keys were brought to
     int* v_ref = k_ref + 8;                                            // [8] by block: that of its values' reference
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ref + 8);
-    int* part = reinterpret_cast<int*>(tmem_slot + 1);                 // [16]
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(part + 16);
+    int* part = reinterpret_cast<int*>(tmem_slot + 1);                 // [20]
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(part + 20);
     int* starts = reinterpret_cast<int*>(smem + S::OFF_PLAN);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -114,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
         for (int g = 0; g < 2; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_ready[g], 4); mbar_init(&o_full[g], 1); }
         for (int s = 0; s < NK; ++s) { mbar_init(&k_full[s], Q8 ? 4 : 1); mbar_init(&k_empty[s], 1); }
         for (int s = 0; s < NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); mbar_init(&v_ready[s], 4); }
-        for (int s = 0; s < NR; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 4); }
+        for (int s = 0; s < NR; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 8); }
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tmK);
@@ -129,158 +143,168 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     constexpr uint32_t TM_S = 0, TM_O = 256;             // two buffers of 128 columns, two of D
+    constexpr uint32_t TM_P = Q8 ? 64 : 0;               // weights lie in the half of the scores that is in registers when they are written
     pdl_wait();
     pdl_launch_dependents();
-    plan<THREADS>(P, starts, part);
+    plan<Split<Q8>::THREADS>(P, starts, part);
     __syncthreads();
     const int all = starts[P.B], per = units_per_cta(all, P.ctas);
     const int u0 = (int)min((long long)all, (long long)blockIdx.x * per), u1 = min(all, u0 + per);
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= P.B; b += Split<Q8>::THREADS) P.starts[b] = starts[b];
     bool ok = true;
-    auto wait = [&](uint64_t* bar, int turn) { return ok && !*abort_flag && mbar_wait(bar, (uint32_t)(turn & 1), P.status); };
+    auto wait = [&](uint64_t* bar, int turn) { return ok && (mbar_try_wait(bar, (uint32_t)(turn & 1)) || (!*abort_flag && mbar_wait(bar, (uint32_t)(turn & 1), P.status))); };
 
-    if (warp == 0) {
-        // ------------------------------------------------------------------------------------ pages
-        int n = 0;                                       // block of the run
-        for (int u = u0; u < u1 && ok;) {
-            const Item it = item_at(P, starts, u, u1);
-            const int pages = (it.r.len + it.r.nodes + PAGE - 1) / PAGE;
-            for (int j = 0; j < it.n && ok; ++j, ++n) {
-                int id = 0;
-                const int p0 = 2 * (it.first + j);
-                static_assert(PAGE * 2 == BLOCK, "two pages a block");
-                if (lane < 2) {
-                    id = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : -2;        // -2: behind the last page
-                    if (id != -2 && (id < 0 || id >= P.n_pages)) {
-                        id = -1;
-                        if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
+    if (warp < SOFTMAX_WARP) {
+        regs_dec<Split<Q8>::OTHER>();                          // one instruction for the warp group
+        if (warp == 0) {
+            // ------------------------------------------------------------------------------------ pages
+            int n = 0;                                       // block of the run
+            for (int u = u0; u < u1 && ok;) {
+                const Item it = item_at(P, starts, u, u1);
+                const int pages = (it.r.len + it.r.nodes + PAGE - 1) / PAGE;
+                for (int j = 0; j < it.n && ok; ++j, ++n) {
+                    int id = 0;
+                    const int p0 = 2 * (it.first + j);
+                    static_assert(PAGE * 2 == BLOCK, "two pages a block");
+                    if (lane < 2) {
+                        id = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : -2;        // -2: behind the last page
+                        if (id != -2 && (id < 0 || id >= P.n_pages)) {
+                            id = -1;
+                            if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
+                        }
                     }
-                }
-                const int page[2] = {__shfl_sync(0xffffffffu, id, 0), __shfl_sync(0xffffffffu, id, 1)};
-                if (lane == 0) {
-                    const int there = page[1] == -2 ? 1 : 2;
-                    if constexpr (Q8) {
-                        const int s = n % NR;
-                        if (n >= NR) ok = wait(&raw_empty[s], n / NR - 1);
-                        if (ok) {
-                            bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
-                            mbar_expect_tx(&raw_full[s], there * (2 * S::PAGE_RAW + 2 * PAGE));
-                            for (int x = 0; x < there; ++x) {
-                                const int head = max(page[x], 0) * P.Hk + it.kvh;        // a page that is none of the pool's: any other in its place, which no row sees
-                                tma_load_2d(sr + s * 2 * S::RAW + x * S::PAGE_RAW, &tmK, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
-                                tma_load_2d(sr + s * 2 * S::RAW + S::RAW + x * S::PAGE_RAW, &tmV, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
-                                bulk_g2s(se + s * 2 * BLOCK + x * PAGE, P.k_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
-                                bulk_g2s(se + s * 2 * BLOCK + BLOCK + x * PAGE, P.v_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
+                    const int page[2] = {__shfl_sync(0xffffffffu, id, 0), __shfl_sync(0xffffffffu, id, 1)};
+                    if (lane == 0) {
+                        const int there = page[1] == -2 ? 1 : 2;
+                        if constexpr (Q8) {
+                            const int s = n % NR;
+                            if (n >= NR) ok = wait(&raw_empty[s], n / NR - 1);
+                            if (ok) {
+                                bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
+                                mbar_expect_tx(&raw_full[s], there * (2 * S::PAGE_RAW + 2 * PAGE));
+                                for (int x = 0; x < there; ++x) {
+                                    const int head = max(page[x], 0) * P.Hk + it.kvh;        // a page that is none of the pool's: any other in its place, which no row sees
+                                    tma_load_2d(sr + s * 2 * S::RAW + x * S::PAGE_RAW, &tmK, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
+                                    tma_load_2d(sr + s * 2 * S::RAW + S::RAW + x * S::PAGE_RAW, &tmV, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
+                                    bulk_g2s(se + s * 2 * BLOCK + x * PAGE, P.k_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
+                                    bulk_g2s(se + s * 2 * BLOCK + BLOCK + x * PAGE, P.v_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
+                                }
+                            }
+                        } else {
+                            const int sK = n % NK, sV = n % NV;
+                            if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
+                            if (ok) {
+                                bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
+                                mbar_expect_tx(&k_full[sK], there * (S::TILE / 2));
+                                for (int x = 0; x < there; ++x)
+                                    for (int c = 0; c < D / 64; ++c)
+                                        tma_load_2d(sk + sK * S::TILE + c * (BLOCK * 128) + x * 8192, &tmK, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &k_full[sK]);
+                                if (n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
+                            }
+                            if (ok) {
+                                mbar_expect_tx(&v_full[sV], there * (S::TILE / 2));
+                                for (int x = 0; x < there; ++x)
+                                    for (int c = 0; c < D / 64; ++c)
+                                        tma_load_2d(sv + sV * S::TILE + (x * (D / 64) + c) * 8192, &tmV, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &v_full[sV]);
                             }
                         }
-                    } else {
-                        const int sK = n % NK, sV = n % NV;
-                        if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
-                        if (ok) {
-                            bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
-                            mbar_expect_tx(&k_full[sK], there * (S::TILE / 2));
-                            for (int x = 0; x < there; ++x)
-                                for (int c = 0; c < D / 64; ++c)
-                                    tma_load_2d(sk + sK * S::TILE + c * (BLOCK * 128) + x * 8192, &tmK, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &k_full[sK]);
-                            if (n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
-                        }
-                        if (ok) {
-                            mbar_expect_tx(&v_full[sV], there * (S::TILE / 2));
-                            for (int x = 0; x < there; ++x)
-                                for (int c = 0; c < D / 64; ++c)
-                                    tma_load_2d(sv + sV * S::TILE + (x * (D / 64) + c) * 8192, &tmV, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &v_full[sV]);
-                        }
                     }
+                    ok = __shfl_sync(0xffffffffu, (int)ok, 0);
                 }
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-            }
-            u += it.n;
-        }
-        if (!ok) *abort_flag = 1;
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------------------------ products
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc<Q8>(BLOCK, 0), id_o = idesc<Q8>(D, 1);
-            int base = 0, item = 0, p_turn[2] = {0, 0};  // base: block of the run that the item begins with
-            for (int u = u0; u < u1 && ok; ++item) {
-                const Item it = item_at(P, starts, u, u1);
-                const int total = it.r.len + it.r.nodes;
-                auto issue_s = [&](int j) {
-                    const int n = base + j, s = n % NK;
-                    ok = wait(&k_full[s], n / NK);
-                    if (!ok) return;
-                    tc_fence_after();
-                    const uint32_t a0 = smem_u32(sq), b0 = smem_u32(sk + s * S::TILE);
-#pragma unroll
-                    for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_bf16(tmem + TM_S + (uint32_t)((j & 1) * BLOCK), smem_desc(a0 + c * (BQ * 128) + k * 32, 16, 1024), smem_desc(b0 + c * (BLOCK * 128) + k * 32, 16, 1024), id_s,
-                                      (c > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(&k_empty[s]);
-                    umma_commit(&s_full[j & 1]);
-                    if (j + 1 == it.n) umma_commit(q_free);
-                };
-                ok = wait(q_full, item);
-                if (ok) issue_s(0);
-                if (ok && it.n > 1) issue_s(1);
-                for (int j = 0; j < it.n && ok; ++j) {
-                    const int g = j & 1, n = base + j, s = n % NV, t0 = (it.first + j) * BLOCK;
-                    ok = wait(&p_ready[g], p_turn[g]++);
-                    if (ok) ok = wait(&v_ready[s], n / NV);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t b0 = smem_u32(sv + s * S::TILE);
-                    const int halves = t0 + PAGE < total ? 2 : 1;      // the second page is there
-                    for (int x = 0; x < halves; ++x)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_ts(tmem + TM_O + (uint32_t)(g * D), tmem + TM_S + (uint32_t)(g * BLOCK + (x * 4 + k) * 8), smem_desc(b0 + x * (D / 64) * 8192 + k * 2048, 8192, 1024), id_o,
-                                    (j > 1 || x > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(&v_empty[s]);
-                    if (j + 2 >= it.n) umma_commit(&o_full[g]);
-                    if (j + 2 < it.n) issue_s(j + 2);
-                }
-                base += it.n;
                 u += it.n;
             }
             if (!ok) *abort_flag = 1;
+        } else if (warp == 1) {
+            // ------------------------------------------------------------------------------------ products
+            if (lane == 0) {
+                constexpr uint32_t id_s = idesc<Q8>(BLOCK, 0), id_o = idesc<Q8>(D, 1);
+                int base = 0, item = 0, p_turn[2] = {0, 0};  // base: block of the run that the item begins with
+                for (int u = u0; u < u1 && ok; ++item) {
+                    const Item it = item_at(P, starts, u, u1);
+                    const int total = it.r.len + it.r.nodes;
+                    auto issue_s = [&](int j) {
+                        const int n = base + j, s = n % NK;
+                        ok = wait(&k_full[s], n / NK);
+                        if (!ok) return;
+                        tc_fence_after();
+                        const uint64_t a0 = smem_desc(smem_u32(sq), 16, 1024), b0 = smem_desc(smem_u32(sk + s * S::TILE), 16, 1024);          // an address in a descriptor counts 16 bytes
+    #pragma unroll
+                        for (int c = 0; c < D / 64; ++c)
+    #pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                umma_bf16(tmem + TM_S + (uint32_t)((j & 1) * BLOCK), a0 + (c * (BQ * 128) + k * 32) / 16, b0 + (c * (BLOCK * 128) + k * 32) / 16, id_s, (c > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(&k_empty[s]);
+                        umma_commit(&s_full[j & 1]);
+                        if (j + 1 == it.n) umma_commit(q_free);
+                    };
+                    ok = wait(q_full, item);
+                    if (ok) issue_s(0);
+                    if (ok && it.n > 1) issue_s(1);
+                    for (int j = 0; j < it.n && ok; ++j) {
+                        const int g = j & 1, n = base + j, s = n % NV, t0 = (it.first + j) * BLOCK;
+                        ok = wait(&p_ready[g], p_turn[g]++);
+                        if (ok) ok = wait(&v_ready[s], n / NV);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t b0 = smem_desc(smem_u32(sv + s * S::TILE), 8192, 1024);
+                        const uint32_t d = tmem + TM_O + (uint32_t)(g * D), p = tmem + TM_S + (uint32_t)(g * BLOCK) + TM_P;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+                            if (x == 0 || t0 + PAGE < total)               // the second page is there
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) umma_ts(d, p + (x * 4 + k) * 8, b0 + (x * (D / 64) * 8192 + k * 2048) / 16, id_o, (j > 1 || x > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(&v_empty[s]);
+                        if (j + 2 >= it.n) umma_commit(&o_full[g]);
+                        if (j + 2 < it.n) issue_s(j + 2);
+                    }
+                    base += it.n;
+                    u += it.n;
+                }
+                if (!ok) *abort_flag = 1;
+            }
         }
-    } else if (warp >= SOFTMAX_WARP && warp < CONVERT_WARP) {
+    } else if (warp < CONVERT_WARP) {
         // ------------------------------------------------------------------------------------ softmax
+        regs_inc<Split<Q8>::SOFTMAX>();
         const int g = (warp - SOFTMAX_WARP) >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + TM_S + (uint32_t)(g * BLOCK), to = lanes + TM_O + (uint32_t)(g * D);
-        int base = 0, item = 0, s_turn = 0, o_turn = 0;
-        for (int u = u0; u < u1; ++item) {
-            const Item it = item_at(P, starts, u, u1);
-            const int len = it.r.len, nodes = it.r.nodes, rows = min(BQ, nodes * P.G - it.tile * BQ);
-            const bool live = (warp & 3) * 32 < rows, on = row < rows;
-            const int at = it.tile * BQ + row, node = on ? at / P.G : 0, head = on ? at - node * P.G : 0;
-            unsigned long long seen = 0;
-            if (on) seen = (P.mask ? P.mask[(size_t)it.b * P.T + node] : (2ull << node) - 1) & (nodes < 64 ? (1ull << nodes) - 1 : ~0ull);
-            float fac = P.scale_log2;
+        int base = 0, s_turn = 0, o_turn = 0;
+        // what a thread knows of its row in an item
+        struct Row { Item it; bool live, on; unsigned long long seen; float fac; };
+        auto enter = [&](int u, int item) {
+            Row w;
+            w.it = item_at(P, starts, u, u1);
+            const int rows = min(BQ, w.it.r.nodes * P.G - w.it.tile * BQ), at = w.it.tile * BQ + row;
+            w.live = (warp & 3) * 32 < rows;
+            w.on = row < rows;
+            const int node = w.on ? at / P.G : 0, head = w.on ? at - node * P.G : 0;
+            w.seen = 0;
+            if (w.on) w.seen = (P.mask ? P.mask[(size_t)w.it.b * P.T + node] : (2ull << node) - 1) & (w.it.r.nodes < 64 ? (1ull << w.it.r.nodes) - 1 : ~0ull);
+            w.fac = P.scale_log2;
             if (Q8 || g == 0) {                          // the row of q: both groups want its scale, the first puts it into the tile
-                const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)it.b * P.q_batch + (size_t)node * P.q_row + (size_t)(it.kvh * P.G + head) * D);
+                const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)w.it.b * P.q_batch + (size_t)node * P.q_row + (size_t)(w.it.kvh * P.G + head) * D);
                 uint4 raw[D / 8];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) raw[i] = on ? q[i] : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < D / 8; ++i) raw[i] = w.on ? q[i] : make_uint4(0, 0, 0, 0);
                 if constexpr (Q8) {                      // to fp16, its largest magnitude in [1, 2)
                     uint32_t a = 0;
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                        const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) a = max(a, max(w[x] & 0x7fffu, (w[x] >> 16) & 0x7fffu));
+                        for (int k = 0; k < 4; ++k) a = max(a, max(x[k] & 0x7fffu, (x[k] >> 16) & 0x7fffu));
                     }
-                    const int k = min(253, max(1, (int)(a >> 7)));           // biased exponent
+                    const int k = min(253, max(40, (int)(a >> 7)));          // biased exponent
                     const float down = __uint_as_float((uint32_t)(254 - k) << 23);
-                    fac *= __uint_as_float((uint32_t)k << 23);
+                    w.fac *= __uint_as_float((uint32_t)k << 23);
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i) {
-                        uint32_t* w = reinterpret_cast<uint32_t*>(&raw[i]);
+                        uint32_t* x = reinterpret_cast<uint32_t*>(&raw[i]);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[x]));
-                            w[x] = pack2<true>(f.x * down, f.y * down);
+                        for (int y = 0; y < 4; ++y) {
+                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[y]));
+                            x[y] = pack2<true>(f.x * down, f.y * down);
                         }
                     }
                 }
@@ -293,6 +317,16 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                     if (lane == 0) mbar_arrive(q_full);
                 }
             }
+            return w;
+        };
+        Row w;
+        if (u0 < u1) w = enter(u0, 0);
+        for (int u = u0, item = 0; u < u1; ++item) {
+            const Item& it = w.it;
+            const int len = it.r.len;
+            const bool live = w.live, on = w.on;
+            const unsigned long long seen = w.seen;
+            const float fac = w.fac;
             float m = -INFINITY, l = 0.f;
             int ref = 0;                                 // of the values that the accumulator holds
             for (int j = g; j < it.n; j += 2) {
@@ -302,28 +336,36 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                 if (live && ok) {
                     const int bad = bad_pages[n & 7];
                     const bool some = t0 + BLOCK > len || bad;               // not every row sees every token
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-                    if (some) {
+                    const float f = Q8 ? fmaxf(fac * pow2(k_ref[n & 7] - 127 - K_ROOM), 1e-30f) : fac;      // above zero: it meets -infinity
+                    // HOLD scores at a time in registers: all of a block, or (e4m3) halves, the first fetched a second time
+                    constexpr int HOLD = Q8 ? BLOCK / 2 : BLOCK;
+                    uint32_t r[HOLD];
+                    auto fetch = [&](int from) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) vis[c] = (bad >> (c >> 1)) & 1 ? 0u : visible32(seen, t0 + 32 * c - len);
-                    }
-                    const float f = Q8 ? fac * pow2(k_ref[n & 7] - 127 - K_ROOM) : fac;
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    uint32_t r[2][32];
-                    tmem_ld32(ts, r[0]);
+                        for (int c = 0; c < HOLD / 32; ++c) tmem_ld32(ts + from + 32 * c, r + 32 * c);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld_done(r[c & 1]);
-                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), r[(c + 1) & 1]);
+                        for (int c = 0; c < HOLD / 32; ++c) tmem_ld_done(r + 32 * c);
                         if (some) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], (vis[c] >> i) & 1 ? __uint_as_float(r[c & 1][i]) : -INFINITY);
-                        } else {
+                            for (int c = 0; c < HOLD / 32; ++c) {
+                                const uint32_t vis = (bad >> ((from + 32 * c) / PAGE)) & 1 ? 0u : visible32(seen, t0 + from + 32 * c - len);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[c & 1][i]));
+                                for (int i = 0; i < 32; ++i)
+                                    if (!((vis >> i) & 1)) r[32 * c + i] = 0xff800000u;      // -infinity
+                            }
                         }
+                    };
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto top = [&] {
+#pragma unroll
+                        for (int i = 0; i < HOLD; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                    };
+                    fetch(0);
+                    top();
+                    if constexpr (Q8) {
+                        fetch(HOLD);
+                        top();
                     }
-                    tmem_ld32(ts, r[0]);
                     const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
                     float alpha = 1.f;
                     if (mx > m + 8.f) {
@@ -337,35 +379,40 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                         ref = to_ref;
                     }
                     const float mu = m == -INFINITY ? 0.f : m - weight_up<Q8>();
-                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint64_t f2 = both(f), mu2 = both(-mu);
+                    uint64_t l2[2] = {0, 0};
+                    auto weigh = [&](int from) {                             // the packed weights take the place of the scores, in registers and in tensor memory
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld_done(r[c & 1]);
-                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), r[(c + 1) & 1]);
-                        uint32_t p[16];
+                        for (int c = 0; c < HOLD / 32; ++c) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float x = fmaf(__uint_as_float(r[c & 1][2 * i]), f, -mu), y = fmaf(__uint_as_float(r[c & 1][2 * i + 1]), f, -mu);
-                            if (some) {
-                                if (!((vis[c] >> (2 * i)) & 1)) x = -INFINITY;
-                                if (!((vis[c] >> (2 * i + 1)) & 1)) y = -INFINITY;
+                            for (int i = 0; i < 16; ++i) {
+                                float x, y;
+                                apart(fma2(pair(r[32 * c + 2 * i], r[32 * c + 2 * i + 1]), f2, mu2), x, y);
+                                x = exp2f(x);
+                                y = exp2f(y);
+                                l2[i & 1] = add2(l2[i & 1], pair(__float_as_uint(x), __float_as_uint(y)));
+                                r[16 * c + i] = pack2<Q8>(x, y);
                             }
-                            x = exp2f(x);
-                            y = exp2f(y);
-                            l4[i & 3] += x + y;
-                            p[i] = pack2<Q8>(x, y);
+                            tmem_st16(ts + TM_P + from / 2 + 16 * c, r + 16 * c);
                         }
-                        tmem_st16(ts + 16 * c, p);                           // over scores that have been read
+                    };
+                    if constexpr (Q8) {
+                        weigh(HOLD);
+                        fetch(0);
                     }
-                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    weigh(0);
+                    float lx[4];
+                    apart(l2[0], lx[0], lx[1]);
+                    apart(l2[1], lx[2], lx[3]);
+                    l += (lx[0] + lx[1]) + (lx[2] + lx[3]);
                     if (j > 1 && __any_sync(0xffffffffu, alpha != 1.f)) {    // these scores are there, so the product before them is done
 #pragma unroll
                         for (int c = 0; c < D / 32; ++c) {
-                            tmem_ld32(to + 32 * c, r[0]);
-                            tmem_ld_done(r[0]);
+                            tmem_ld32(to + 32 * c, r);
+                            tmem_ld_done(r);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) r[0][i] = __float_as_uint(__uint_as_float(r[0][i]) * alpha);
-                            tmem_st32(to + 32 * c, r[0]);
+                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                            tmem_st32(to + 32 * c, r);
                         }
                     }
                     tmem_st_wait();
@@ -374,9 +421,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[g]);
             }
-            // ---- the item's part of this group
+            // ---- the item's part of this group; the next item's scores are computed meanwhile
             float* wk = P.work + partial_at(P, blockIdx.x, u == u0 ? 0 : 1, g, D);
             float2* ml = reinterpret_cast<float2*>(wk + (size_t)BQ * D) + row;
+            Row next = w;
+            if (u + it.n < u1) next = enter(u + it.n, item + 1);
             if (it.n > g) {
                 ok = wait(&o_full[g], o_turn++);
                 tc_fence_after();
@@ -409,9 +458,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                             }
                         }
                         if (on) {
-                            float* dst = wk + (size_t)row * D + 32 * c;
+                            float* dst = wk + (4 * c * BQ + row) * 8;
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) st_global_32(dst + i, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]), make_uint4(r[i + 4], r[i + 5], r[i + 6], r[i + 7]));
+                            for (int i = 0; i < 32; i += 8) st_global_32(dst + i * BQ, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]), make_uint4(r[i + 4], r[i + 5], r[i + 6], r[i + 7]));
                         }
                     }
                     *ml = on ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
@@ -421,17 +470,22 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
             }
             base += it.n;
             u += it.n;
+            w = next;
         }
         if (!ok) *abort_flag = 1;
-    } else if (warp >= CONVERT_WARP) {
+    } else {
         // ------------------------------------------------------------------------------------ tiles
-        const int cw = warp - CONVERT_WARP, tid = threadIdx.x - CONVERT_WARP * 32;
+        regs_dec<Split<Q8>::OTHER>();
+        const int cw = (warp - CONVERT_WARP) & 3, tid = (threadIdx.x - CONVERT_WARP * 32) & 127;
+        const bool values = !Q8 || warp >= CONVERT_WARP + 4;                 // e4m3: keys are the first four warps' matter, values the others'
         int n = 0, item = 0;
         for (int u = u0; u < u1; ++item) {               // after a wait that ran out as well: the four warps meet at every item
             const Item it = item_at(P, starts, u, u1);
             const int len = it.r.len, total = len + it.r.nodes;
-            if (tid == 0) taint[item & 7] = 0;           // eight items back: nobody reads it any more
-            convert_sync();
+            if (values) {
+                if (tid == 0) taint[item & 7] = 0;       // eight items back: nobody reads it any more
+                convert_sync();
+            }
             int ref = 0;
             for (int j = 0; j < it.n; ++j, ++n) {
                 const int t0 = (it.first + j) * BLOCK, sV = n % NV;
@@ -463,64 +517,80 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                 } else {
                     const int sR = n % NR, sK = n % NK;
                     ok = wait(&raw_full[sR], n / NR);
-                    const uint8_t *ke = se + sR * 2 * BLOCK, *ve = ke + BLOCK;
-                    uint32_t kw = 0, vw = 0;
-                    if (ok) { kw = reinterpret_cast<const uint32_t*>(ke)[lane]; vw = reinterpret_cast<const uint32_t*>(ve)[lane]; }
+                    const uint8_t* exps = se + sR * 2 * BLOCK + (values ? BLOCK : 0);
+                    const uint32_t* words = reinterpret_cast<const uint32_t*>(se + sR * 2 * BLOCK);
+                    uint32_t kw = ok ? words[lane] : 0, vw = ok ? words[BLOCK / 4 + lane] : 0;       // exponents of four tokens
                     const int past = t0 + 4 * lane - total + 4;              // how many of these four lie behind the last token
                     if (past > 0) {
                         const uint32_t keep = past >= 4 ? 0u : 0xffffffffu >> (8 * past);
                         kw &= keep;
                         vw &= keep;
                     }
-                    const int top_k = (int)byte_max(kw), top_v = (int)byte_max(vw);
+                    const int top = (int)byte_max(kw), top_v = (int)byte_max(vw);
+                    // both sides follow the values' reference: the scores of a block, which its keys announce, may be there before its values are
                     if (j == 0 || top_v > ref + K_ROOM - V_ROOM) ref = top_v;
-                    // eight tokens and 64 of their elements at a time: lane (token, 16-byte piece).  Two tokens of a phase differ in the bits that part their pieces in the raw
-                    // lines and in the tile's, so that neither meets in a bank
-                    constexpr int HALVES = D / 64, TURNS = BLOCK / 8 * HALVES / 4;
+                    // A warp takes 32 tokens, eight of them and 64 of their elements at a time: lane (token, 16-byte piece).  Two tokens of a phase differ in the bits that part their
+                    // pieces in the raw lines and in the tile's, so that neither meets in a bank; all offsets but this lane's are constants
+                    constexpr int HALVES = D / 64;
                     const int pr = lane >> 3, sel = (lane >> 2) & 1, c4 = lane & 3, in8 = D == 128 ? (sel ? pr ^ 5 : pr) : 2 * pr + sel;
-                    auto convert = [&](const uint8_t* raw, const uint8_t* exps, uint8_t* tile, bool values, int top) {
-#pragma unroll 2
-                        for (int i = 0; i < TURNS; ++i) {
-                            const int turn = cw * TURNS + i, half = turn % HALVES, token = turn / HALVES * 8 + in8, x = token >> 6, t = token & 63;
-                            const uint32_t at = D == 128 ? t * 128 + (((half * 4 + c4) ^ (t & 7)) * 16) : (t >> 1) * 128 + ((((t & 1) * 4 + c4) ^ ((t >> 1) & 7)) * 16);
-                            const uint4 w = *reinterpret_cast<const uint4*>(raw + x * S::PAGE_RAW + at);
-                            uint32_t y[4] = {w.x, w.y, w.z, w.w};
-                            __half2 by = half2_pow2(min((int)exps[token] - top, 0) + (values ? min(top - ref + V_ROOM, K_ROOM) : K_ROOM));
-                            if (values && t0 + token >= len) {
-                                const bool gone = t0 + token >= total;
-                                uint32_t any = 0;
+                    const uint32_t from = D == 128 ? cw * 4096 + in8 * 128 + ((c4 ^ in8) * 16) : cw * 2048 + (in8 >> 1) * 128 + ((((in8 & 1) * 4 + c4) ^ (in8 >> 1)) * 16);
+                    const uint32_t to = (cw & 1) * 4096 + in8 * 128 + (((2 * c4) ^ in8) * 16);
+                    const int mine = cw * 32 + lane, pos = t0 + mine;        // this lane's token, whose factors the others ask for
+                    auto convert = [&](const uint8_t* raw, uint8_t* tile, auto values_, auto some_, int e) {
+                        constexpr bool VALUES = decltype(values_)::value, SOME = decltype(some_)::value;       // SOME: values of a block with drafted tokens
+                        const __half2 factor = half2_pow2(e);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const uint32_t no = gone ? ~0u : __vcmpeq4(y[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                                    any |= no;
-                                    y[k] &= ~no;
+                        for (int i = 0; i < 4; ++i) {                        // eight tokens each
+                            const uint32_t fw = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&factor), i * 8 + in8);
+                            const __half2 by = *reinterpret_cast<const __half2*>(&fw);
+#pragma unroll
+                            for (int half = 0; half < HALVES; ++half) {
+                                const uint32_t at = D == 128 ? (from + i * 1024) ^ (half * 64) : (from + i * 512) ^ ((i & 1) * 64);
+                                const uint4 w = *reinterpret_cast<const uint4*>(raw + at);
+                                uint32_t y[4] = {w.x, w.y, w.z, w.w};
+                                if constexpr (SOME) {                        // what lies behind the last token, and what is no number of a drafted one
+                                    const int token = t0 + cw * 32 + i * 8 + in8;
+                                    uint32_t any = 0;
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) {
+                                        const uint32_t no = token >= total ? ~0u : token >= len ? __vcmpeq4(y[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) : 0u;
+                                        any |= no;
+                                        y[k] &= ~no;
+                                    }
+                                    if (any && token < total) atomicOr(&taint[item & 7], 1ull << (token - len));
                                 }
-                                if (gone) by = half2_pow2(0);
-                                else if (any) atomicOr(&taint[item & 7], 1ull << (t0 + token - len));
-                            }
-                            uint32_t h[8];
+                                uint32_t h[8];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                const uint32_t two = e4m3x2(k & 1 ? y[k >> 1] >> 16 : y[k >> 1]);
-                                const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&two), by);
-                                h[k] = *reinterpret_cast<const uint32_t*>(&z);
+                                for (int k = 0; k < 8; ++k) {
+                                    const uint32_t two = e4m3x2(k & 1 ? y[k >> 1] >> 16 : y[k >> 1]);
+                                    const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&two), by);
+                                    h[k] = *reinterpret_cast<const uint32_t*>(&z);
+                                }
+                                // tile of keys: halves 16 KB apart, pages 8 KB; of values: pages 8 KB times the halves, halves 8 KB
+                                const uint32_t part = i * 1024 + (VALUES ? ((cw >> 1) * HALVES + half) * 8192 : half * (BLOCK * 128) + (cw >> 1) * 8192);
+                                *reinterpret_cast<uint4*>(tile + to + part) = make_uint4(h[0], h[1], h[2], h[3]);
+                                *reinterpret_cast<uint4*>(tile + (to ^ 16) + part) = make_uint4(h[4], h[5], h[6], h[7]);
                             }
-                            uint8_t* dst = tile + (values ? (x * HALVES + half) * 8192 : half * (BLOCK * 128) + x * 8192) + t * 128;
-                            *reinterpret_cast<uint4*>(dst + (((2 * c4) ^ (t & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
-                            *reinterpret_cast<uint4*>(dst + (((2 * c4 + 1) ^ (t & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
                         }
                     };
-                    if (ok && n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
-                    if (ok) convert(sr + sR * 2 * S::RAW, ke, sk + sK * S::TILE, false, top_k);
-                    if (tid == 0) { k_ref[n & 7] = top_k; v_ref[n & 7] = ref; }
+                    const int e = ok ? exps[mine] : 0;                       // behind the last token: anything, but no more than the largest
+                    const uint8_t* raw = sr + sR * 2 * S::RAW + (values ? S::RAW : 0);
+                    if (!values) {
+                        if (ok && n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
+                        if (ok) convert(raw, sk + sK * S::TILE, Flag<false>(), Flag<false>(), min(e - top, 0) + K_ROOM);
+                        if (tid == 0) { k_ref[n & 7] = top; v_ref[n & 7] = ref; }
+                    } else {
+                        if (ok && n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
+                        const int by = pos >= total ? 0 : min(e - ref + V_ROOM, K_ROOM);
+                        if (ok && t0 + BLOCK <= len) convert(raw, sv + sV * S::TILE, Flag<true>(), Flag<false>(), by);
+                        else if (ok) convert(raw, sv + sV * S::TILE, Flag<true>(), Flag<true>(), by);
+                    }
                     fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&k_full[sK]);
-                    if (ok && n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
-                    if (ok) convert(sr + sR * 2 * S::RAW + S::RAW, ve, sv + sV * S::TILE, true, top_v);
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) { mbar_arrive(&v_ready[sV]); mbar_arrive(&raw_empty[sR]); }
+                    if (lane == 0) {
+                        mbar_arrive(values ? &v_ready[sV] : &k_full[sK]);
+                        mbar_arrive(&raw_empty[sR]);
+                    }
                 }
                 ok = __all_sync(0xffffffffu, ok);
             }
@@ -555,7 +625,7 @@ int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cuda
         PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_tiles_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL + MAX_B * 4 + 4));
         if (dev < 64) attr[dev] = true;
     }
-    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D, Q8>, dim3(p.ctas), dim3(THREADS), (size_t)S::TOTAL + (p.B + 1) * 4, st, ptb_pdl_enabled(), mk, mv, p));
+    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D, Q8>, dim3(p.ctas), dim3(Split<Q8>::THREADS), (size_t)S::TOTAL + (p.B + 1) * 4, st, ptb_pdl_enabled(), mk, mv, p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }

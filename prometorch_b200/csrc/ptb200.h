@@ -300,7 +300,7 @@ int ptb_paged_attn_decode(const void* q, long long q_stride, void* out, int B, i
 
 // ---------------------------------------------------------------------------- paged_tree.cu
 // Floats of workspace that ptb_paged_attn_tree needs.
-long long ptb_paged_tree_work_floats(int T, int H, int Hk, int D);
+long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D);
 
 // T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with
 // pitches in elements, head h at column h * D; out [B, T, H D]; lens [B]: cached tokens before the drafted ones, node i stands in slot lens[b] + i; nodes [B]

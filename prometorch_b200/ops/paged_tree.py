@@ -38,7 +38,7 @@ def _decls(L):
         L.ptb_paged_keep.restype = ci
         L.ptb_paged_attn_tree.argtypes = [vp, ll, ll, vp, ci, ci, ci, ci, ci, vp, vp, vp, vp, ci, ci, vp, vp, vp, vp, cf, vp, vp, vp]
         L.ptb_paged_attn_tree.restype = ci
-        L.ptb_paged_tree_work_floats.argtypes = [ci, ci, ci, ci]
+        L.ptb_paged_tree_work_floats.argtypes = [ci, ci, ci, ci, ci]
         L.ptb_paged_tree_work_floats.restype = ll
 
 
@@ -206,7 +206,7 @@ def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.T
     if mask is not None and not (mask.dtype == torch.int64 and mask.shape == (B, T) and mask.is_contiguous() and mask.device == dev):
         raise ValueError(f"paged_attention_tree: a contiguous int64 mask [{B}, {T}] on {dev} is needed")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    if not 0.0 < scale < math.inf:
+    if not 1e-30 < scale < 1e30:
         raise ValueError(f"paged_attention_tree: a scale above zero is needed, not {scale}")
     if q.is_cuda:
         if q.dtype != torch.bfloat16 or D not in (64, 128):
@@ -218,7 +218,7 @@ def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.T
         out = torch.empty(B, T, H * D, dtype=torch.bfloat16, device=dev)
         L = N.lib()
         with _Device(dev):
-            work = torch.empty(L.ptb_paged_tree_work_floats(T, H, Hk, D), dtype=torch.float32, device=dev)
+            work = torch.empty(L.ptb_paged_tree_work_floats(B, T, H, Hk, D), dtype=torch.float32, device=dev)
             rc = L.ptb_paged_attn_tree(q.data_ptr(), s0, s1, out.data_ptr(), B, T, H, Hk, D, lens.data_ptr(), N.ptr(nodes), N.ptr(mask), page_table.data_ptr(), page_table.shape[1],
                                        k_pages.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp), N.ptr(v_exp), scale, work.data_ptr(), _status(dev).data_ptr(),
                                        _stream(dev.index))
