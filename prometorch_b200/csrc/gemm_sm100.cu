@@ -43,6 +43,19 @@ int ptb_make_tmap_bf16(CUtensorMap* map, const void* base, long long inner, long
     return 0;
 }
 
+// 2-D map of contiguous rows of 64 bytes, boxes of `box_rows` rows, 64-byte swizzle.
+int ptb_make_tmap_64b(CUtensorMap* map, const void* base, long long rows, int box_rows) {
+    EncodeTiledFn enc = get_encode();
+    if (!enc) { ptb_set_error("cuTensorMapEncodeTiled is not available (no CUDA driver?)"); return -1; }
+    if ((uintptr_t)base & 15) { ptb_set_error("TMA operand needs a 16-byte aligned base"); return -1; }
+    cuuint64_t dims[2] = {64, (cuuint64_t)rows}, strides[1] = {64};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { ptb_set_error("cuTensorMapEncodeTiled failed with code %d", (int)r); return -1; }
+    return 0;
+}
+
 // 3-D bf16 tensor map of a contiguous [n2][n1][n0] tensor (n0 fastest); box sizes per dimension.
 int ptb_make_tmap_bf16_3d(CUtensorMap* map, const void* base, long long n0, long long n1, long long n2, int b0, int b1, int b2) {
     EncodeTiledFn enc = get_encode();

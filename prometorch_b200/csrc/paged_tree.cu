@@ -30,8 +30,8 @@ struct Geo {
     static constexpr int PITCH = D + 8;                                // floats of a row of the joining buffer
     static constexpr int OFF_EXP = WARPS * STAGES * STAGE, OFF_JOIN = OFF_EXP + (Q8 ? WARPS * STAGES * 2 * PIECE : 0);
     static constexpr int OFF_ML = OFF_JOIN + WARPS * ROWS * PITCH * 4, OFF_BAR = OFF_ML + WARPS * ROWS * 8, OFF_PLAN = OFF_BAR + WARPS * STAGES * 8 + 64;
-    static constexpr int TOTAL = OFF_PLAN + 1024;                      // and (B + 1) ints
-    static_assert(TOTAL + MAX_B * 4 + 4 <= 227 * 1024, "shared memory of a CTA");
+    static constexpr int TOTAL = OFF_PLAN + 1024;                      // and the plan
+    static_assert(TOTAL + plan_bytes(MAX_B) <= 227 * 1024, "shared memory of a CTA");
 };
 
 // Which of eight neighbouring tokens lane r (0 .. 7) takes; see above.  Keys: lanes 2p and 2p + 1 of one phase differ in the bit that moves a token to the other
@@ -442,9 +442,11 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
     }
 }
 
-// The partial results of items: one block per sixteen rows of an item, a thread (row, eight columns); and the rows that no unit belongs to, which are zeros.  NATURAL: partial
-// columns are in the order of the head, and every item has partial results; else place i of a row is column i % 8 of tile i / 8, and an item of one CTA is written already.
-template <int D, bool Q8, bool NATURAL>
+// The partial results of items that were cut: one block per sixteen rows of an item, a thread (row, eight columns); and the rows that no unit belongs to, which are zeros.
+// How the accumulators of a partial result lie: TILES [D / 8][rows][8], place i of a row column i % 8 of product tile i / 8;
+// EIGHTS the same in the order of the head; ROWWISE [rows][D].
+enum Layout { TILES, EIGHTS, ROWWISE };
+template <int D, bool Q8, Layout LAYOUT>
 __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_constant__ Params P) {
     pdl_wait();
     pdl_launch_dependents();
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
     if (tile < r.tiles && (tile * P.tile_rows + row0) / P.G < r.nodes) {     // some of the sixteen rows are there
         const int per = units_per_cta(P.starts[P.B], P.ctas), a = P.starts[b] + i * r.units, e = a + r.units;
         const int c0 = a / per, c1 = (e - 1) / per, n = (c1 - c0 + 1) * P.parts;
-        if (!NATURAL && c0 == c1) return;                // written already
+        if (c0 == c1) return;                            // written already
         auto from = [&](int k) {                         // slot 0: the run begins in (or with) this item
             const int c = c0 + k / P.parts;
             return P.work + partial_at(P, c, c * per >= a ? 0 : 1, k % P.parts, D);
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
                 if (k0 + x < n) {
                     const float* p = from(k0 + x);
                     ml[x] = *reinterpret_cast<const float2*>(p + (size_t)P.tile_rows * D + 2 * row);
-                    const float4* q = reinterpret_cast<const float4*>(p + (size_t)(c8 * P.tile_rows + row) * 8);
+                    const float4* q = reinterpret_cast<const float4*>(p + (LAYOUT == ROWWISE ? (size_t)row * D + c8 * 8 : (size_t)(c8 * P.tile_rows + row) * 8));
                     v[x][0] = q[0];
                     v[x][1] = q[1];
                 } else {
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
     const bool on = node < r.nodes && L != 0.f;
     const float inv = on ? 1.f / L : 0.f;
     __nv_bfloat16* out = P.out + (((size_t)b * P.T + node) * P.H + kvh * P.G + g) * D;
-    if constexpr (NATURAL) {
+    if constexpr (LAYOUT != TILES) {
         uint4 w;
         __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
 #pragma unroll
@@ -513,10 +515,10 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
     }
 }
 
-template <int D, bool Q8, bool NATURAL>
+template <int D, bool Q8, Layout LAYOUT>
 int launch_merge(const Params& p, cudaStream_t st) {
     const int groups = (p.T * p.G + 15) / 16 < p.tile_rows / 16 ? (p.T * p.G + 15) / 16 : p.tile_rows / 16;
-    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, Q8, NATURAL>, dim3(p.tiles * p.Hk * groups, p.B), dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
+    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, Q8, LAYOUT>, dim3(p.tiles * p.Hk * groups, p.B), dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }
@@ -531,19 +533,18 @@ int launch(const Params& p, const void* k_pages, const void* v_pages, cudaStream
     int dev = 0;
     PTB_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ge::TOTAL + MAX_B * 4 + 4));
+        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ge::TOTAL + plan_bytes(MAX_B)));
         if (dev < 64) attr[dev] = true;
     }
-    PTB_CUDA_OK(ptb_launch(paged_tree_kernel<D, Q8>, dim3(p.ctas), dim3(THREADS), (size_t)Ge::TOTAL + (p.B + 1) * 4, st, ptb_pdl_enabled(), mk, mv, p));
-    return launch_merge<D, Q8, false>(p, st);
+    PTB_CUDA_OK(ptb_launch(paged_tree_kernel<D, Q8>, dim3(p.ctas), dim3(THREADS), (size_t)Ge::TOTAL + plan_bytes(p.B), st, ptb_pdl_enabled(), mk, mv, p));
+    return launch_merge<D, Q8, TILES>(p, st);
 }
 
-// Up to sixteen rows (nodes times heads of a group): mma.sync on tiles of sixteen; more: tcgen05 on tiles of 128.
 template <int D, bool Q8>
 int launch_any(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
-    if (p.tile_rows == ROWS) return launch<D, Q8>(p, k_pages, v_pages, st);
-    if (launch_tiles<D, Q8>(p, k_pages, v_pages, st)) return -1;
-    return launch_merge<D, Q8, true>(p, st);
+    if (p.parts == 1) return launch<D, Q8>(p, k_pages, v_pages, st);
+    if (p.tile_rows == 32) return launch_few<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, Q8, ROWWISE>(p, st);
+    return launch_tiles<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, Q8, EIGHTS>(p, st);
 }
 
 int sm_count() {
@@ -554,9 +555,12 @@ int sm_count() {
     }
     return n;
 }
-int tile_rows_of(int rows) { return rows <= ROWS ? ROWS : 128; }
-int parts_of(int tile_rows) { return tile_rows == ROWS ? 1 : 2; }
-
+// Which kernel, by the rows of a (request, kv head): its tile of rows, the tokens of a unit and the partial results that a CTA leaves of an item.
+struct Choice { int tile_rows, unit, parts; };
+Choice choose(int rows) {
+    if (rows <= ROWS) return {ROWS, PAGE, 1};
+    return {rows <= 32 ? 32 : 128, 128, 2};
+}
 }  // namespace
 }  // namespace tree
 }  // namespace ptb
@@ -566,14 +570,14 @@ using namespace ptb;
 // Floats of workspace that ptb_paged_attn_tree needs.
 PTB_API long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D) {
     if (Hk <= 0 || T <= 0) return 0;
-    const int rows = tree::tile_rows_of(T * (H / Hk));
-    return (long long)tree::sm_count() * 2 * tree::parts_of(rows) * (long long)tree::partial_floats(rows, D) + B + 1;
+    const tree::Choice c = tree::choose(T * (H / Hk));
+    return (long long)tree::sm_count() * 2 * c.parts * (long long)tree::partial_floats(c.tile_rows, D) + B + 1;
 }
 
 // T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with
 // pitches in elements, head h at column h * D; out [B, T, H D]; lens [B]: cached tokens before the drafted ones, node i stands in slot lens[b] + i; nodes [B]
 // (null: T), rows behind them come out as zeros, as do rows that see nothing; mask [B, T]: bit j, whether the node sees node j (null: a chain).  Pages
-// [n_pages, Hk, 64, D]: bf16, or e4m3 with exponents [n_pages, Hk, 64].  D is 64 or 128, T at most 64, B at most 4096.
+// [n_pages, Hk, 64, D]: bf16, or e4m3 with exponents [n_pages, Hk, 64].  D is 64 or 128, T at most 64, B at most 1024.
 PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_row, void* out, int B, int T, int H, int Hk, int D, const int* lens, const int* nodes, const void* mask,
                                 const int* page_table, int pt_stride, int n_pages, const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, float scale, float* work,
                                 int* status, cudaStream_t st) {
@@ -594,10 +598,11 @@ PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_ro
     p.q = (const __nv_bfloat16*)q; p.q_batch = q_batch; p.q_row = q_row; p.out = (__nv_bfloat16*)out; p.lens = lens; p.nodes = nodes; p.mask = (const unsigned long long*)mask;
     p.page_table = page_table; p.pt_stride = pt_stride; p.n_pages = n_pages; p.k_exp = (const uint8_t*)k_exp; p.v_exp = (const uint8_t*)v_exp; p.v_raw = (const uint8_t*)v_pages; p.work = work;
     p.B = B; p.T = T; p.H = H; p.Hk = Hk; p.G = H / Hk;
-    p.tile_rows = tree::tile_rows_of(T * p.G);
+    const tree::Choice c = tree::choose(T * p.G);
+    p.tile_rows = c.tile_rows;
+    p.unit = c.unit;
+    p.parts = c.parts;
     p.tiles = (T * p.G + p.tile_rows - 1) / p.tile_rows;
-    p.unit = p.tile_rows == tree::ROWS ? tree::PAGE : 128;
-    p.parts = tree::parts_of(p.tile_rows);
     p.ctas = tree::sm_count();
     p.starts = reinterpret_cast<int*>(work + (size_t)p.ctas * 2 * p.parts * tree::partial_floats(p.tile_rows, D));
     p.scale_log2 = scale * 1.4426950408889634f;

@@ -19,7 +19,7 @@ namespace tree {
 
 constexpr int PAGE = 64;
 constexpr int MAX_NODES = 64;
-constexpr int MAX_B = 4096;
+constexpr int MAX_B = 1024;
 
 struct Params {
     const __nv_bfloat16* q;              // [B, T, q_row] pitches in elements; head h at column h * D
@@ -51,24 +51,38 @@ __device__ __forceinline__ int cached_of(const Params& P, int b, int n) { return
 
 // What a request asks for: tiles with rows, units of an item.
 struct Req { int nodes, len, tiles, units; };
-__device__ __forceinline__ Req req_of(const Params& P, int b) {
+__device__ __forceinline__ Req req_with(const Params& P, int len, int nodes) {
     Req r;
-    r.nodes = nodes_of(P, b);
-    r.len = cached_of(P, b, r.nodes);
+    r.nodes = nodes;
+    r.len = len;
     r.tiles = (r.nodes * P.G + P.tile_rows - 1) / P.tile_rows;
     r.units = (r.len + r.nodes + P.unit - 1) / P.unit;
     return r;
 }
+__device__ __forceinline__ Req req_of(const Params& P, int b) {
+    const int nodes = nodes_of(P, b);
+    return req_with(P, cached_of(P, b, nodes), nodes);
+}
 __device__ __forceinline__ int units_of(const Params& P, const Req& r) { return r.tiles * P.Hk * r.units; }
 
-// starts[b]: units before request b (starts[B]: all).  The block's N threads, with `part` of N / 32 ints.
+// The plan, in shared memory: starts[b], units before request b (starts[B]: all), and behind them each request's cached tokens and nodes (bytes).
+__host__ __device__ constexpr int plan_bytes(int B) { return (2 * B + 1) * 4 + B; }
+__device__ __forceinline__ uint8_t* plan_nodes(const Params& P, int* starts) { return reinterpret_cast<uint8_t*>(starts + 2 * P.B + 1); }
+// The block's N threads make it, with `part` of N / 32 ints.
 template <int N>
 __device__ __forceinline__ void plan(const Params& P, int* starts, int* part) {
     int carry = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int b0 = 0; b0 < P.B; b0 += N) {
         const int b = b0 + (int)threadIdx.x;
-        int u = b < P.B ? units_of(P, req_of(P, b)) : 0, upto = u;
+        int u = 0;
+        if (b < P.B) {
+            const Req r = req_of(P, b);
+            u = units_of(P, r);
+            starts[P.B + 1 + b] = r.len;
+            plan_nodes(P, starts)[b] = (uint8_t)r.nodes;
+        }
+        int upto = u;
         if (b < P.B && P.status && (P.lens[b] < 0 || P.lens[b] > P.pt_stride * PAGE - nodes_of(P, b))) atomicExch(P.status, PTB_ERR_BOUNDS);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -92,13 +106,13 @@ __device__ __forceinline__ void plan(const Params& P, int* starts, int* part) {
 // The run of units of a CTA: `per` each.
 __device__ __forceinline__ int units_per_cta(int all, int ctas) { return max(1, (all + ctas - 1) / ctas); }
 
-// A CTA leaves partial results of at most two items: the one its run begins in (slot 0) and the one it ends in (slot 1; where both are the same, slot 0).
-// One is [D / 8][rows][8] accumulators (threads that own a row each then write whole lines), then [rows] (maximum, sum).
+// A CTA leaves partial results of at most two items that it shares with others: the one its run begins in (slot 0) and the one it ends in (slot 1; where both are the same,
+// slot 0).  An item that it has to itself it writes out.  One result is rows x D accumulators, then [rows] (maximum, sum).
 __device__ __forceinline__ size_t partial_at(const Params& P, int cta, int slot, int part, int D) { return (size_t)((cta * 2 + slot) * P.parts + part) * partial_floats(P.tile_rows, D); }
 
 // An item and the part of it in a CTA's run: n units from `first` on.
 struct Item { int b, tile, kvh, first, n; Req r; };
-__device__ __forceinline__ Item item_at(const Params& P, const int* starts, int u, int u1) {
+__device__ __forceinline__ Item item_at(const Params& P, int* starts, int u, int u1) {
     int lo = 0, hi = P.B;                                // the last request that starts at or before u (empty ones share a start with the next)
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -106,7 +120,7 @@ __device__ __forceinline__ Item item_at(const Params& P, const int* starts, int 
     }
     Item it;
     it.b = lo;
-    it.r = req_of(P, lo);
+    it.r = req_with(P, starts[P.B + 1 + lo], plan_nodes(P, starts)[lo]);
     const int in = u - starts[lo], i = in / it.r.units;
     it.first = in - i * it.r.units;
     it.n = min(it.r.units - it.first, u1 - u);
@@ -125,6 +139,12 @@ __device__ __forceinline__ uint32_t e4m3x2(uint32_t two) {
     asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(h) : "r"(two));
     return h;
 }
+// Two fp32 as e4m3 (the low 16 bits), rounded to nearest.
+__device__ __forceinline__ uint32_t e4m3_pack(float x, float y) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(x), "f"(y));
+    return r;
+}
 template <bool Q8>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     uint32_t r;
@@ -134,6 +154,7 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 }
 
 template <int D, bool Q8> int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);      // paged_tree_sm100.cu
+template <int D, bool Q8> int launch_few(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);        // paged_tree_few_sm100.cu
 
 }  // namespace tree
 }  // namespace ptb

@@ -18,86 +18,26 @@
 //
 // A drafted token that a row does not see must not reach it, whatever it holds: its weight is zero, and zero times a value that is no number is none.  So such values are
 // cleared in the tile and the rows that do see the token take them at the end.  What lies behind a request's last token is cleared as well.
-#include "paged_tree.cuh"
-#include "gemm_sm100.cuh"
+#include "paged_tree_sm100.cuh"
 
 namespace ptb {
 namespace tree {
 namespace {
 
-using namespace ptb::gemm;
-
-constexpr int BQ = 128, BLOCK = 128;
-constexpr int SOFTMAX_WARP = 4, CONVERT_WARP = 12;       // four warps of converters behind the latter, or (e4m3) eight
+constexpr int BQ = LANES;
 // Threads, and registers a thread of the softmax and of the other warps: the launch's shared out anew (512 x 128 = 256 x 184 + 256 x 72; 640 x 96 = 256 x 120 + 384 x 80).  A softmax
 // thread holds its 128 scores (64 of them): one wait for tensor memory a block, or three, in place of eight; 4900 clocks from the scores to the weights became 2000.
 template <bool Q8> struct Split { static constexpr int THREADS = Q8 ? 640 : 512, SOFTMAX = Q8 ? 120 : 184, OTHER = Q8 ? 80 : 72; };
-template <int R> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
-template <int R> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
-
 template <int D, bool Q8>
 struct Sm {
     static constexpr int Q_BYTES = BQ * D * 2, TILE = BLOCK * D * 2, RAW = BLOCK * D, PAGE_RAW = RAW / 2;
     static constexpr int NK = Q8 ? 1 : D == 128 ? 2 : 3, NV = Q8 ? 2 : D == 128 ? 3 : 4, NR = Q8 ? (D == 128 ? 2 : 4) : 0;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NK * TILE, OFF_R = OFF_V + NV * TILE, OFF_E = OFF_R + NR * 2 * RAW;
     static constexpr int OFF_BAR = OFF_E + NR * 2 * BLOCK, OFF_PLAN = OFF_BAR + 1024;
-    static constexpr int TOTAL = OFF_PLAN + 1024;                      // and (B + 1) ints
-    static_assert(TOTAL + MAX_B * 4 + 4 <= 227 * 1024, "shared memory of a CTA");
+    static constexpr int TOTAL = OFF_PLAN + 1024;                      // and the plan
+    static_assert(TOTAL + plan_bytes(MAX_B) <= 227 * 1024, "shared memory of a CTA");
 };
 
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc),
-                 "r"(accumulate)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) { tmem_st16(taddr, r); tmem_st16(taddr + 16, r + 16); }
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// Loads have arrived; the registers are not read before.
-__device__ __forceinline__ void tmem_ld_done(uint32_t* r) {
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 32; i += 8)
-        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])::"memory");
-}
-__device__ __forceinline__ void convert_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-
-// Pairs of fp32 in one instruction.
-__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y)); return r; }
-__device__ __forceinline__ uint64_t both(float x) { return pair(__float_as_uint(x), __float_as_uint(x)); }
-__device__ __forceinline__ void apart(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
-
-// fp16 or bf16 operands, fp32 accumulators.
-template <bool Q8>
-constexpr uint32_t idesc(int n, int b_mn) { return instr_desc(BQ, n, 0, b_mn) & (Q8 ? ~((1u << 7) | (1u << 10)) : ~0u); }
-
-// Which of 32 tokens from `d0` behind the cached ones on (negative: still cached) a row sees; seen: its mask, of nodes that are there.
-__device__ __forceinline__ uint32_t visible32(unsigned long long seen, int d0) {
-    if (d0 >= 0) return d0 < 64 ? (uint32_t)(seen >> d0) : 0u;
-    if (d0 <= -32) return ~0u;
-    return ((1u << -d0) - 1) | (uint32_t)(seen << -d0);
-}
-__device__ __forceinline__ uint32_t byte_max(uint32_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = __vmaxu4(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return max(max(v & 255, (v >> 8) & 255), max((v >> 16) & 255, v >> 24));
-}
-// 2^e as two fp16 (zero below what fp16 has).
-__device__ __forceinline__ __half2 half2_pow2(int e) {
-    const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
-    const uint32_t w = h | (h << 16);
-    return *reinterpret_cast<const __half2*>(&w);
-}
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
-
-template <bool X> struct Flag { static constexpr bool value = X; };
 constexpr int V_ROOM = 3;                // fp16 values stand for value * 2^(reference - V_ROOM): the reference may be passed by 2^4 before it has to grow
 constexpr int K_ROOM = 7;                // 448 * 2^7 fits fp16
 
@@ -218,7 +158,7 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
         } else if (warp == 1) {
             // ------------------------------------------------------------------------------------ products
             if (lane == 0) {
-                constexpr uint32_t id_s = idesc<Q8>(BLOCK, 0), id_o = idesc<Q8>(D, 1);
+                constexpr uint32_t id_s = idesc<Q8>(BLOCK, 0, 0), id_o = idesc<Q8>(D, 0, 1);
                 int base = 0, item = 0, p_turn[2] = {0, 0};  // base: block of the run that the item begins with
                 for (int u = u0; u < u1 && ok; ++item) {
                     const Item it = item_at(P, starts, u, u1);
@@ -426,48 +366,85 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
             float2* ml = reinterpret_cast<float2*>(wk + (size_t)BQ * D) + row;
             Row next = w;
             if (u + it.n < u1) next = enter(u + it.n, item + 1);
-            if (it.n > g) {
-                ok = wait(&o_full[g], o_turn++);
-                tc_fence_after();
-                if (live && ok) {
-                    const unsigned long long meets = taint[item & 7] & seen;
-                    const float down = Q8 ? pow2(ref - 127 - V_ROOM) : 1.f;
+            if (it.n > g) ok = wait(&o_full[g], o_turn++);
+            tc_fence_after();
+            const unsigned long long meets = taint[item & 7] & seen;
+            const float down = Q8 ? pow2(ref - 127 - V_ROOM) : 1.f;
+            uint32_t r[32];
+            auto columns = [&](int c) {                  // 32 of the accumulator's, from 32 c on
+                tmem_ld32(to + 32 * c, r);
+                tmem_ld_done(r);
+                if constexpr (Q8) {
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t r[32];
-                        tmem_ld32(to + 32 * c, r);
-                        tmem_ld_done(r);
+                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * down);
+                }
+                for (unsigned long long left = meets; left; left &= left - 1) {      // values that were cleared, of a token that this row sees
+                    const int t = len + __ffsll((long long)left) - 1;
+                    if (t / BLOCK < it.first || t / BLOCK >= it.first + it.n || ((t / BLOCK - it.first) & 1) != g) continue;
+                    const int page = P.page_table[(size_t)it.b * P.pt_stride + t / PAGE];
+                    if (page < 0 || page >= P.n_pages) continue;
+                    const size_t v = (((size_t)page * P.Hk + it.kvh) * PAGE + t % PAGE) * D + 32 * c;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
                         if constexpr (Q8) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * down);
-                        }
-                        for (unsigned long long left = meets; left; left &= left - 1) {          // values that were cleared, of a token that this row sees
-                            const int t = len + __ffsll((long long)left) - 1;
-                            if (t / BLOCK < it.first || t / BLOCK >= it.first + it.n || ((t / BLOCK - it.first) & 1) != g) continue;
-                            const int page = P.page_table[(size_t)it.b * P.pt_stride + t / PAGE];
-                            if (page < 0 || page >= P.n_pages) continue;
-                            const size_t v = (((size_t)page * P.Hk + it.kvh) * PAGE + t % PAGE) * D + 32 * c;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                if constexpr (Q8) {
-                                    if ((P.v_raw[v + i] & 0x7f) == 0x7f) r[i] = 0x7fffffffu;
-                                } else {
-                                    const uint32_t w = (uint32_t)reinterpret_cast<const uint16_t*>(P.v_raw)[v + i] << 16;
-                                    if ((w & 0x7f800000u) == 0x7f800000u) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(w));
-                                }
-                            }
-                        }
-                        if (on) {
-                            float* dst = wk + (4 * c * BQ + row) * 8;
-#pragma unroll
-                            for (int i = 0; i < 32; i += 8) st_global_32(dst + i * BQ, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]), make_uint4(r[i + 4], r[i + 5], r[i + 6], r[i + 7]));
+                            if ((P.v_raw[v + i] & 0x7f) == 0x7f) r[i] = 0x7fffffffu;
+                        } else {
+                            const uint32_t x = (uint32_t)reinterpret_cast<const uint16_t*>(P.v_raw)[v + i] << 16;
+                            if ((x & 0x7f800000u) == 0x7f800000u) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(x));
                         }
                     }
-                    *ml = on ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
                 }
-            } else if (live) {
-                *ml = make_float2(-INFINITY, 0.f);
+            };
+            // Of an item that no other CTA has a part of, the groups join their parts here, each for half of the columns.
+            const bool whole = it.n == it.r.units, shared = whole && it.n > 1;
+            if (live && it.n > g && (!whole || shared)) {
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    if (whole && (c < D / 64) == (g == 0)) continue;
+                    columns(c);
+                    if (on) {
+                        float* dst = wk + (4 * c * BQ + row) * 8;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) st_global_32(dst + i * BQ, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]), make_uint4(r[i + 4], r[i + 5], r[i + 6], r[i + 7]));
+                    }
+                }
             }
+            const float2 mine = on && it.n > g ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+            if (live) *ml = mine;
+            if (shared) both_sync();
+            if (whole && live && it.n > g) {
+                const float* theirs = wk + (g ? -1 : 1) * (long long)partial_floats(BQ, D);
+                const float2 other = shared ? *reinterpret_cast<const float2*>(theirs + (size_t)BQ * D + 2 * row) : make_float2(-INFINITY, 0.f);
+                const float top = fmaxf(mine.x, other.x), a = mine.x == -INFINITY ? 0.f : exp2f(mine.x - top), b = other.x == -INFINITY ? 0.f : exp2f(other.x - top);
+                const float sum = mine.y * a + other.y * b, inv = sum != 0.f ? 1.f / sum : 0.f;
+                const int at = it.tile * BQ + row, node = at / P.G, first = (at & ~15) / P.G;
+                const bool put = node < P.T && first < it.r.nodes;           // sixteen rows at a time, the ones behind the last are zeros
+                __nv_bfloat16* out = P.out + (((size_t)it.b * P.T + node) * P.H + it.kvh * P.G + (at - node * P.G)) * D;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    if (shared && (c < D / 64) == (g == 1)) continue;
+                    columns(c);
+                    if (!put) continue;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float y[8], z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                        if (b != 0.f) {
+                            const float4* q = reinterpret_cast<const float4*>(theirs + (size_t)((4 * c + i / 8) * BQ + row) * 8);
+                            const float4 q0 = q[0], q1 = q[1];
+                            z[0] = q0.x; z[1] = q0.y; z[2] = q0.z; z[3] = q0.w; z[4] = q1.x; z[5] = q1.y; z[6] = q1.z; z[7] = q1.w;
+                        }
+                        uint4 h;
+                        __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&h);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = (a != 0.f ? __uint_as_float(r[i + k]) * (a * inv) : 0.f) + (b != 0.f ? z[k] * (b * inv) : 0.f);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) h2[k] = __floats2bfloat162_rn(on ? y[2 * k] : 0.f, on ? y[2 * k + 1] : 0.f);
+                        *reinterpret_cast<uint4*>(out + 32 * c + i) = h;
+                    }
+                }
+            }
+            tc_fence_before();
+            both_sync();                                 // that part has been read; and neither group is more than an item ahead of the other
             base += it.n;
             u += it.n;
             w = next;
@@ -622,10 +599,10 @@ int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cuda
     int dev = 0;
     PTB_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_tiles_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL + MAX_B * 4 + 4));
+        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_tiles_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL + plan_bytes(MAX_B)));
         if (dev < 64) attr[dev] = true;
     }
-    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D, Q8>, dim3(p.ctas), dim3(Split<Q8>::THREADS), (size_t)S::TOTAL + (p.B + 1) * 4, st, ptb_pdl_enabled(), mk, mv, p));
+    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D, Q8>, dim3(p.ctas), dim3(Split<Q8>::THREADS), (size_t)S::TOTAL + plan_bytes(p.B), st, ptb_pdl_enabled(), mk, mv, p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }

@@ -305,7 +305,7 @@ long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D);
 // T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with
 // pitches in elements, head h at column h * D; out [B, T, H D]; lens [B]: cached tokens before the drafted ones, node i stands in slot lens[b] + i; nodes [B]
 // (null: T), rows behind them come out as zeros, as do rows that see nothing; mask [B, T]: bit j, whether the node sees node j (null: a chain).  Pages
-// [n_pages, Hk, 64, D]: bf16, or e4m3 with exponents [n_pages, Hk, 64].  D is 64 or 128, T at most 64, B at most 4096.
+// [n_pages, Hk, 64, D]: bf16, or e4m3 with exponents [n_pages, Hk, 64].  D is 64 or 128, T at most 64, B at most 1024.
 int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_row, void* out, int B, int T, int H, int Hk, int D, const int* lens, const int* nodes, const void* mask, const int* page_table, int pt_stride, int n_pages, const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, float scale, float* work, int* status, cudaStream_t st);
 
 // ---------------------------------------------------------------------------- paged_write.cu

@@ -147,6 +147,27 @@ def test_one_node_is_the_decode_step(kind, D):
         close(got[:, 0], old.double(), mag[:, 0] * 2, kind)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hk,T", [(4, 4, 3), (8, 4, 9), (6, 3, 20), (16, 4, 40)])
+def test_many_short_items(kind, D, H, Hk, T):
+    """Far more (request, tile, kv head) than there are SMs, of one block or a few each: most are one CTA's own, and it has several of them."""
+    B = 150
+    g = gen(D + T)
+    have = [(37 * b) % 300 for b in range(B)]
+    nodes = [1 + (5 * b) % T for b in range(B)]
+    table, n_pages = table_for([n + T for n in have], 3)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    mask = random_masks(B, B, T)
+    q = torch.randn(B, T, H * D, device=DEV, generator=g).bfloat16()
+    got = R.paged_attention_tree(q, H, Hk, D, torch.tensor(have, dtype=torch.int32, device=DEV), table, k, v, mask=mask.to(DEV), nodes=torch.tensor(nodes, dtype=torch.int32, device=DEV), k_exp=ke,
+                                 v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, have, nodes, mask, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
+    for b, n in enumerate(nodes):
+        assert not got[b, n:].any()
+
+
 @pytest.mark.parametrize("kind,D,H,Hk,T,lens", [("e4m3", 128, 8, 2, 3, [20011]), ("bf16", 64, 8, 2, 64, [9000, 40]), ("bf16", 128, 2, 1, 1, [5, 30000, 700]), ("e4m3", 64, 4, 1, 20, [64 * 150, 64 * 150 - 20])])
 def test_items_cut_between_ctas(kind, D, H, Hk, T, lens):
     g = gen(T)
