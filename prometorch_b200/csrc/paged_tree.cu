@@ -1,4 +1,4 @@
-// Up to sixteen rows of drafted tokens against a paged cache on mma.sync, and the merge of items that were cut; see paged_tree.cuh.
+// Up to sixteen rows of drafted tokens against a bf16 cache on mma.sync, and the merge of items that were cut; see paged_tree.cuh.
 //
 // One CTA of eight warps per SM.  A warp takes every eighth piece of sixteen tokens of the CTA's run, keeps an online softmax of its own over them, and joins the others when
 // an item ends.  It brings its pieces itself: keys and values of a piece are one TMA box each of 128-byte rows with the 128-byte swizzle, into a ring that only this warp
@@ -9,9 +9,7 @@
 // be any head element, so lane r holds one 16-byte piece of a value row for all tiles.  Which of eight tokens lane r takes (`token_of`) is chosen so
 // that the eight lanes of a quarter warp fall on the eight 16-byte columns of the swizzled rows, for keys and for values.
 //
-// e4m3 pages: values become fp16 exactly, queries are scaled by a power of two into fp16 (they come with eight bits), the exponent of a key's row scales its
-// scores, that of a value's row is added to them: p' = 2^(s + e_v) weighs the raw e4m3 values, and the sum takes p' 2^-e_v.  P is rounded to the operand's
-// type (by at most 2^-11 of a weight in fp16, 2^-8 in bf16, without a bias); scores, maxima, sums and accumulators are fp32.
+// P is rounded to bf16 (by at most 2^-9 of a weight's power of two, without a bias); scores, maxima, sums and accumulators are fp32.
 #include "paged_tree.cuh"
 
 namespace ptb {
@@ -20,15 +18,15 @@ namespace {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32, ROWS = 16, PIECE = 16, PIECES = PAGE / PIECE;
 
-template <int D, bool Q8>
+template <int D>
 struct Geo {
-    static constexpr int ROW = D * (Q8 ? 1 : 2);                       // bytes of a token
+    static constexpr int ROW = D * 2;                                  // bytes of a token
     static constexpr int BYTES = PIECE * ROW, LINES = BYTES / 128;     // of a piece
-    static constexpr int STAGE = 2 * BYTES;                            // keys, values (the exponents lie elsewhere)
+    static constexpr int STAGE = 2 * BYTES;                            // keys, values
     static constexpr int STAGES = 16384 / STAGE;                       // 16 KB a warp
     static constexpr int KSTEPS = D / 16, VTILES = D / 8;
     static constexpr int PITCH = D + 8;                                // floats of a row of the joining buffer
-    static constexpr int OFF_EXP = WARPS * STAGES * STAGE, OFF_JOIN = OFF_EXP + (Q8 ? WARPS * STAGES * 2 * PIECE : 0);
+    static constexpr int OFF_JOIN = WARPS * STAGES * STAGE;
     static constexpr int OFF_ML = OFF_JOIN + WARPS * ROWS * PITCH * 4, OFF_BAR = OFF_ML + WARPS * ROWS * 8, OFF_PLAN = OFF_BAR + WARPS * STAGES * 8 + 64;
     static constexpr int TOTAL = OFF_PLAN + 1024;                      // and the plan
     static_assert(TOTAL + plan_bytes(MAX_B) <= 227 * 1024, "shared memory of a CTA");
@@ -38,7 +36,7 @@ struct Geo {
 // half of a line.  Values: the tokens of lanes 0, 2, 4, 6 (and of 1, 3, 5, 7) fall on four different pairs of columns.
 template <int ROW>
 __device__ __forceinline__ int token_of(int r) {
-    constexpr uint32_t order = ROW == 128 ? 0x37156240u : ROW == 256 ? 0x57463120u : 0x65742130u;
+    constexpr uint32_t order = ROW == 128 ? 0x37156240u : 0x57463120u;
     return (order >> (4 * r)) & 7;
 }
 // Offset of byte `at` of token t in a swizzled piece.
@@ -48,14 +46,10 @@ __device__ __forceinline__ uint32_t place(int t, int at) {
     return x ^ (((x >> 7) & 7) << 4);
 }
 
-template <bool Q8>
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    if constexpr (Q8)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)),
@@ -64,14 +58,8 @@ __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int c0
 }
 
 // Head element of contraction step s, lane c (the first of four), and of output tile t, column n.
-template <int D, bool Q8>
-__device__ __forceinline__ constexpr int k_elem(int s, int c) {
-    return Q8 ? (D == 128 ? (s / 4) * 64 + c * 16 + (s % 4) * 4 : c * 16 + s * 4) : (s / 4) * 64 + (c + 4 * ((s / 2) & 1)) * 8 + (s & 1) * 4;
-}
-template <int D, bool Q8>
-__device__ __forceinline__ constexpr int v_elem(int t, int n) {
-    return Q8 ? n * (D / 8) + t : (t / 8) * 64 + n * 8 + t % 8;
-}
+__device__ __forceinline__ constexpr int k_elem(int s, int c) { return (s / 4) * 64 + (c + 4 * ((s / 2) & 1)) * 8 + (s & 1) * 4; }
+__device__ __forceinline__ constexpr int v_elem(int t, int n) { return (t / 8) * 64 + n * 8 + t % 8; }
 
 // Pieces of an item's part that have tokens.
 __device__ __forceinline__ int pieces_of(const Item& it) { return min(it.n * PIECES, (it.r.len + it.r.nodes - it.first * PAGE + PIECE - 1) / PIECE); }
@@ -81,9 +69,9 @@ struct Fetch {
     int u, piece, ids_from, kvh, n, pieces, row, ids;    // ids: this lane's page id, of the warp's pages from ids_from on; row: first entry of the item's pages in the table
 };
 
-template <int D, bool Q8>
+template <int D>
 __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params P) {
-    using Ge = Geo<D, Q8>;
+    using Ge = Geo<D>;
     constexpr int ROW = Ge::ROW;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -93,7 +81,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
     int* starts = reinterpret_cast<int*>(smem + Ge::OFF_PLAN);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     uint8_t* ring = smem + warp * Ge::STAGES * Ge::STAGE;
-    uint8_t* exps = smem + Ge::OFF_EXP + warp * Ge::STAGES * 2 * PIECE;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + Ge::OFF_BAR) + warp * Ge::STAGES;
     if (lane == 0) {
         for (int s = 0; s < Ge::STAGES; ++s) mbar_init(&full[s], 1);
@@ -141,14 +128,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
         if (lane == 0) {
             const int head = max(page, 0) * P.Hk + f.kvh, line = head * (PIECES * Ge::LINES) + f.piece % PIECES * Ge::LINES;
             uint8_t* st = ring + s * Ge::STAGE;
-            mbar_expect_tx(&full[s], Ge::STAGE + (Q8 ? 2 * PIECE : 0));
+            mbar_expect_tx(&full[s], Ge::STAGE);
             tma_2d(st, &tmK, 0, line, &full[s]);
             tma_2d(st + Ge::BYTES, &tmV, 0, line, &full[s]);
-            if (Q8) {
-                const size_t at = (size_t)head * PAGE + f.piece % PIECES * PIECE;
-                bulk_g2s(exps + s * 2 * PIECE, P.k_exp + at, PIECE, &full[s]);
-                bulk_g2s(exps + s * 2 * PIECE + PIECE, P.v_exp + at, PIECE, &full[s]);
-            }
         }
         bad = page < 0 ? bad | 1u << s : bad & ~(1u << s);
         f.piece += WARPS;
@@ -160,24 +142,14 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
     for (int s = 0; s < Ge::STAGES; ++s) fetch(s);
 
     // ---- this lane's offsets in a piece: its piece of a key (the first of eight tokens; the second lies eight tokens on), of two values
-    constexpr int HALVES = D * (Q8 ? 1 : 2) / 64;        // 64-byte halves of lines of a key row that a row's four lanes cover 16 bytes of each at a time
-    constexpr bool NARROW = ROW == 64;                   // two tokens share a line: eight tokens on, the swizzle differs
-    uint32_t ko[NARROW ? 2 : HALVES], vo[2][NARROW ? 2 : (ROW + 127) / 128];
-    if constexpr (NARROW) {
+    constexpr int HALVES = ROW / 64;                     // 64-byte halves of lines of a key row that a row's four lanes cover 16 bytes of each at a time
+    uint32_t ko[HALVES], vo[2][ROW / 128];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            ko[j] = place<ROW>(8 * j + token_of<ROW>(r), c * 16);
-            vo[0][j] = place<ROW>(8 * j + token_of<ROW>(2 * c), r * 8);
-            vo[1][j] = place<ROW>(8 * j + token_of<ROW>(2 * c + 1), r * 8);
-        }
-    } else {
+    for (int h = 0; h < HALVES; ++h) ko[h] = place<ROW>(token_of<ROW>(r), h * 64 + c * 16);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) ko[h] = place<ROW>(token_of<ROW>(r), h * 64 + c * 16);
-#pragma unroll
-        for (int h = 0; h < ROW / 128; ++h) {
-            vo[0][h] = place<ROW>(token_of<ROW>(2 * c), h * 128 + r * 16);
-            vo[1][h] = place<ROW>(token_of<ROW>(2 * c + 1), h * 128 + r * 16);
-        }
+    for (int h = 0; h < ROW / 128; ++h) {
+        vo[0][h] = place<ROW>(token_of<ROW>(2 * c), h * 128 + r * 16);
+        vo[1][h] = place<ROW>(token_of<ROW>(2 * c + 1), h * 128 + r * 16);
     }
 
     int count = 0;
@@ -187,7 +159,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
         const int len = it.r.len, nodes = it.r.nodes, pieces = pieces_of(it);
         // this lane's two rows
         uint32_t qa[Ge::KSTEPS][4];
-        float fac[2];
         unsigned long long seen[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -197,28 +168,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
             const __nv_bfloat16* q = P.q + (size_t)it.b * P.q_batch + (size_t)(on ? node : 0) * P.q_row + (size_t)(it.kvh * P.G + g) * D;
             uint2 raw[Ge::KSTEPS];
 #pragma unroll
-            for (int s = 0; s < Ge::KSTEPS; ++s) raw[s] = on ? *reinterpret_cast<const uint2*>(q + k_elem<D, Q8>(s, c)) : make_uint2(0, 0);
-            fac[x] = P.scale_log2;
-            if constexpr (Q8) {                          // the row's largest magnitude to [1, 2)
-                uint32_t a = 0;
+            for (int s = 0; s < Ge::KSTEPS; ++s) raw[s] = on ? *reinterpret_cast<const uint2*>(q + k_elem(s, c)) : make_uint2(0, 0);
 #pragma unroll
-                for (int s = 0; s < Ge::KSTEPS; ++s)
-                    a = max(a, max(max(raw[s].x & 0x7fffu, (raw[s].x >> 16) & 0x7fffu), max(raw[s].y & 0x7fffu, (raw[s].y >> 16) & 0x7fffu)));
-                a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-                a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-                const int k = min(253, max(40, (int)(a >> 7)));              // biased exponent
-                const float down = __uint_as_float((uint32_t)(254 - k) << 23);
-                fac[x] *= __uint_as_float((uint32_t)k << 23);
-#pragma unroll
-                for (int s = 0; s < Ge::KSTEPS; ++s) {
-                    const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[s].x)), hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[s].y));
-                    qa[s][x] = pack2<true>(lo.x * down, lo.y * down);
-                    qa[s][2 + x] = pack2<true>(hi.x * down, hi.y * down);
-                }
-            } else {
-#pragma unroll
-                for (int s = 0; s < Ge::KSTEPS; ++s) { qa[s][x] = raw[s].x; qa[s][2 + x] = raw[s].y; }
-            }
+            for (int s = 0; s < Ge::KSTEPS; ++s) { qa[s][x] = raw[s].x; qa[s][2 + x] = raw[s].y; }
         }
         float acc[Ge::VTILES][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -231,10 +183,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
             const int s = count % Ge::STAGES, first = it.first * PAGE + piece * PIECE;       // first: the piece's first token
             if (ok) ok = mbar_wait(&full[s], (uint32_t)((count / Ge::STAGES) & 1), P.status);
             if (ok && !((bad >> s) & 1)) {
-                const uint8_t *sk = ring + s * Ge::STAGE, *sv = sk + Ge::BYTES, *se = exps + s * 2 * PIECE;
+                const uint8_t *sk = ring + s * Ge::STAGE, *sv = sk + Ge::BYTES;
                 const bool tail = first + PIECE > len;   // some of its tokens are drafted, or lie behind the last
                 float sc[2][4];
-                float ev[2][2], un[2][2];                // exponent of a token's values, 2^-exponent
                 {
                     float part4[2][2][4];                // two chains of products a tile
 #pragma unroll
@@ -245,16 +196,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                     for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(sk + (NARROW ? ko[j] : ko[h] + j * 8 * ROW));
-                            if constexpr (Q8) {
-                                mma<true>(part4[j][0], qa[4 * h], e4m3x2(w.x), e4m3x2(w.x >> 16));
-                                mma<true>(part4[j][1], qa[4 * h + 1], e4m3x2(w.y), e4m3x2(w.y >> 16));
-                                mma<true>(part4[j][0], qa[4 * h + 2], e4m3x2(w.z), e4m3x2(w.z >> 16));
-                                mma<true>(part4[j][1], qa[4 * h + 3], e4m3x2(w.w), e4m3x2(w.w >> 16));
-                            } else {
-                                mma<false>(part4[j][0], qa[2 * h], w.x, w.y);
-                                mma<false>(part4[j][1], qa[2 * h + 1], w.z, w.w);
-                            }
+                            const uint4 w = *reinterpret_cast<const uint4*>(sk + ko[h] + j * 8 * ROW);
+                            mma(part4[j][0], qa[2 * h], w.x, w.y);
+                            mma(part4[j][1], qa[2 * h + 1], w.z, w.w);
                         }
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
@@ -266,22 +210,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         const int t = 8 * j + token_of<ROW>(2 * c + y);
-                        float ks = 1.f;
-                        if constexpr (Q8) {
-                            uint32_t ke = se[t], ve = se[PIECE + t];
-                            if (tail) {                  // a byte of a slot that nobody wrote may hold anything: within what is ever stored
-                                ke = min(191u, max(63u, ke));
-                                ve = min(191u, max(63u, ve));
-                            }
-                            ks = __uint_as_float(ke << 23);
-                            ev[j][y] = __uint_as_float(0x4b000000u | ve) - (8388608.f + 127.f);
-                            un[j][y] = __uint_as_float(0x7f000000u - (ve << 23));
-                        }
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             float& v = sc[j][2 * x + y];
-                            if constexpr (Q8) v = fmaf(v * ks, fac[x], ev[j][y]);
-                            else v *= fac[x];
+                            v *= P.scale_log2;
                             if (tail) {
                                 const int d = first + t - len;
                                 if (d >= 0 && (d >= nodes || !((seen[x] >> d) & 1))) v = -INFINITY;
@@ -294,15 +226,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                 bool odd = false;                        // a value that is no number, which a row that does not see its token must not meet
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    if constexpr (NARROW) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(sv + vo[k & 1][k >> 1]);
-                        vw[k][0] = w.x; vw[k][1] = w.y;
-                    } else {
 #pragma unroll
-                        for (int h = 0; h < VW / 4; ++h) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(sv + vo[k & 1][h] + (k >> 1) * 8 * ROW);
-                            vw[k][4 * h] = w.x; vw[k][4 * h + 1] = w.y; vw[k][4 * h + 2] = w.z; vw[k][4 * h + 3] = w.w;
-                        }
+                    for (int h = 0; h < VW / 4; ++h) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(sv + vo[k & 1][h] + (k >> 1) * 8 * ROW);
+                        vw[k][4 * h] = w.x; vw[k][4 * h + 1] = w.y; vw[k][4 * h + 2] = w.z; vw[k][4 * h + 3] = w.w;
                     }
                     if (tail) {
                         const int d = first + 8 * (k >> 1) + token_of<ROW>(2 * c + (k & 1)) - len;
@@ -311,10 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                             for (int i = 0; i < VW; ++i) vw[k][i] = 0;
                         } else if (d >= 0) {
 #pragma unroll
-                            for (int i = 0; i < VW; ++i) {
-                                if constexpr (Q8) odd |= __vcmpeq4(vw[k][i] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
-                                else odd |= __vcmpeq2(vw[k][i] & 0x7f807f80u, 0x7f807f80u) != 0;
-                            }
+                            for (int i = 0; i < VW; ++i) odd |= __vcmpeq2(vw[k][i] & 0x7f807f80u, 0x7f807f80u) != 0;
                         }
                     }
                 }
@@ -340,34 +264,22 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const float mu = m[x] == -INFINITY ? 0.f : m[x] - weight_up<Q8>();
+                    const float mu = m[x] == -INFINITY ? 0.f : m[x];
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             float& v = sc[j][2 * x + y];
                             v = exp2f(v - mu);
-                            l[x] = Q8 ? fmaf(v, un[j][y], l[x]) : l[x] + v;
+                            l[x] += v;
                         }
                 }
-                const uint32_t pa[4] = {pack2<Q8>(sc[0][0], sc[0][1]), pack2<Q8>(sc[0][2], sc[0][3]), pack2<Q8>(sc[1][0], sc[1][1]), pack2<Q8>(sc[1][2], sc[1][3])};
+                const uint32_t pa[4] = {pack2<false>(sc[0][0], sc[0][1]), pack2<false>(sc[0][2], sc[0][3]), pack2<false>(sc[1][0], sc[1][1]), pack2<false>(sc[1][2], sc[1][3])};
                 if (!tail || !__any_sync(0xffffffffu, odd)) {
-                    if constexpr (Q8) {
 #pragma unroll
-                        for (int i = 0; i < VW; ++i) {
-                            const uint32_t a0 = __byte_perm(vw[0][i], vw[1][i], 0x5140), a1 = __byte_perm(vw[0][i], vw[1][i], 0x7362);
-                            const uint32_t b0 = __byte_perm(vw[2][i], vw[3][i], 0x5140), b1 = __byte_perm(vw[2][i], vw[3][i], 0x7362);
-                            mma<true>(acc[4 * i], pa, e4m3x2(a0), e4m3x2(b0));
-                            mma<true>(acc[4 * i + 1], pa, e4m3x2(a0 >> 16), e4m3x2(b0 >> 16));
-                            mma<true>(acc[4 * i + 2], pa, e4m3x2(a1), e4m3x2(b1));
-                            mma<true>(acc[4 * i + 3], pa, e4m3x2(a1 >> 16), e4m3x2(b1 >> 16));
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < VW; ++i) {
-                            mma<false>(acc[2 * i], pa, __byte_perm(vw[0][i], vw[1][i], 0x5410), __byte_perm(vw[2][i], vw[3][i], 0x5410));
-                            mma<false>(acc[2 * i + 1], pa, __byte_perm(vw[0][i], vw[1][i], 0x7632), __byte_perm(vw[2][i], vw[3][i], 0x7632));
-                        }
+                    for (int i = 0; i < VW; ++i) {
+                        mma(acc[2 * i], pa, __byte_perm(vw[0][i], vw[1][i], 0x5410), __byte_perm(vw[2][i], vw[3][i], 0x5410));
+                        mma(acc[2 * i + 1], pa, __byte_perm(vw[0][i], vw[1][i], 0x7632), __byte_perm(vw[2][i], vw[3][i], 0x7632));
                     }
                 } else {                                 // token by token, each for the rows that see it
 #pragma unroll
@@ -381,10 +293,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                         for (int tt = 0; tt < Ge::VTILES; ++tt)
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
-                                const int e = v_elem<D, Q8>(tt, 2 * c + y);
-                                float v;
-                                if constexpr (Q8) v = __half2float(__ushort_as_half((unsigned short)(e4m3x2(sv[place<ROW>(t, e)]) & 0xffff)));
-                                else v = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(sv + place<ROW>(t, 2 * e)) << 16);
+                                const int e = v_elem(tt, 2 * c + y);
+                                const float v = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(sv + place<ROW>(t, 2 * e)) << 16);
                                 if (s0) acc[tt][y] += w0 * v;
                                 if (s1) acc[tt][2 + y] += w1 * v;
                             }
@@ -400,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
             const int row = warp * ROWS + r + 8 * x;
-            if (c == 0) ml[row] = make_float2(m[x], l[x]);
+            if (c == 0) ml[row] = make_float2(m[x] == -INFINITY && l[x] != 0.f ? 0.f : m[x], l[x]);          // a sum without a maximum is of no numbers
             float* dst = joined + (size_t)row * Ge::PITCH + 2 * c;
 #pragma unroll
             for (int t = 0; t < Ge::VTILES; ++t) *reinterpret_cast<float2*>(dst + 8 * t) = make_float2(acc[t][2 * x], acc[t][2 * x + 1]);
@@ -429,8 +339,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                 if (node < P.T) {
                     const bool on = node < nodes && L != 0.f;
                     __nv_bfloat16* o = P.out + (((size_t)it.b * P.T + node) * P.H + it.kvh * P.G + g) * D;
-                    o[v_elem<D, Q8>(i / 8, i % 8)] = __float2bfloat16_rn(on ? o0 / L : 0.f);
-                    o[v_elem<D, Q8>(i / 8, i % 8 + 1)] = __float2bfloat16_rn(on ? o1 / L : 0.f);
+                    o[v_elem(i / 8, i % 8)] = __float2bfloat16_rn(on ? o0 / L : 0.f);
+                    o[v_elem(i / 8, i % 8 + 1)] = __float2bfloat16_rn(on ? o1 / L : 0.f);
                 }
             } else {
                 *reinterpret_cast<float2*>(wk + ((i / 8) * ROWS + row) * 8 + i % 8) = make_float2(o0, o1);
@@ -446,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
 // How the accumulators of a partial result lie: TILES [D / 8][rows][8], place i of a row column i % 8 of product tile i / 8;
 // EIGHTS the same in the order of the head; ROWWISE [rows][D].
 enum Layout { TILES, EIGHTS, ROWWISE };
-template <int D, bool Q8, Layout LAYOUT>
+template <int D, Layout LAYOUT>
 __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_constant__ Params P) {
     pdl_wait();
     pdl_launch_dependents();
@@ -511,21 +421,21 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
         *reinterpret_cast<uint4*>(out + 8 * c8) = w;
     } else {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) out[v_elem<D, Q8>(c8, x)] = __float2bfloat16_rn(on ? o[x] * inv : 0.f);
+        for (int x = 0; x < 8; ++x) out[v_elem(c8, x)] = __float2bfloat16_rn(on ? o[x] * inv : 0.f);
     }
 }
 
-template <int D, bool Q8, Layout LAYOUT>
+template <int D, Layout LAYOUT>
 int launch_merge(const Params& p, cudaStream_t st) {
     const int groups = (p.T * p.G + 15) / 16 < p.tile_rows / 16 ? (p.T * p.G + 15) / 16 : p.tile_rows / 16;
-    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, Q8, LAYOUT>, dim3(p.tiles * p.Hk * groups, p.B), dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
+    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, LAYOUT>, dim3(p.tiles * p.Hk * groups, p.B), dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }
 
-template <int D, bool Q8>
-int launch(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
-    using Ge = Geo<D, Q8>;
+template <int D>
+int launch_pieces(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
+    using Ge = Geo<D>;
     CUtensorMap mk, mv;
     const long long lines = (long long)p.n_pages * p.Hk * PIECES * Ge::LINES;
     if (ptb_make_tmap_bf16(&mk, k_pages, 64, lines, 64, 64, Ge::LINES) || ptb_make_tmap_bf16(&mv, v_pages, 64, lines, 64, 64, Ge::LINES)) return -1;
@@ -533,18 +443,12 @@ int launch(const Params& p, const void* k_pages, const void* v_pages, cudaStream
     int dev = 0;
     PTB_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ge::TOTAL + plan_bytes(MAX_B)));
+        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ge::TOTAL + plan_bytes(MAX_B)));
         if (dev < 64) attr[dev] = true;
     }
-    PTB_CUDA_OK(ptb_launch(paged_tree_kernel<D, Q8>, dim3(p.ctas), dim3(THREADS), (size_t)Ge::TOTAL + plan_bytes(p.B), st, ptb_pdl_enabled(), mk, mv, p));
-    return launch_merge<D, Q8, TILES>(p, st);
-}
-
-template <int D, bool Q8>
-int launch_any(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
-    if (p.parts == 1) return launch<D, Q8>(p, k_pages, v_pages, st);
-    if (p.tile_rows == 32) return launch_few<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, Q8, ROWWISE>(p, st);
-    return launch_tiles<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, Q8, EIGHTS>(p, st);
+    PTB_CUDA_OK(ptb_launch(paged_tree_kernel<D>, dim3(p.ctas), dim3(THREADS), (size_t)Ge::TOTAL + plan_bytes(p.B), st, ptb_pdl_enabled(), mk, mv, p));
+    PTB_CUDA_OK(cudaGetLastError());
+    return 0;
 }
 
 int sm_count() {
@@ -555,22 +459,38 @@ int sm_count() {
     }
     return n;
 }
-// Which kernel, by the rows of a (request, kv head): its tile of rows, the tokens of a unit and the partial results that a CTA leaves of an item.
+// Which kernel, by the rows of a (request, kv head), the type of the pages and what the page table has room for: its tile of rows, the tokens of a unit and the partial
+// results that a CTA leaves of an item.
+//   up to 16 rows, bf16: mma.sync.  16 requests of 8192 tokens, 8 rows of 128: 78.6 us, tokens along the lanes of tensor memory 81; one of 540 tokens, 4 rows: 12.2 and 17.7.
+//   up to 32 rows, bf16, and two pages a CTA at most: mma.sync, in one or two tiles.  One request of 540 tokens, 20 rows of 128: 14.9 us, tokens along the lanes 20.
+//   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 87 and 90 us, in tiles of 128 rows 104 and 108; e4m3, 64 rows over 4100
+//   tokens: 73 and 117.  e4m3, 4 rows over 8192 tokens, 32 requests: 84, where mma.sync, for which every warp converts what it reads, took 148.
+//   more: tiles of 128 rows.
 struct Choice { int tile_rows, unit, parts; };
-Choice choose(int rows) {
-    if (rows <= ROWS) return {ROWS, PAGE, 1};
-    return {rows <= 32 ? 32 : 128, 128, 2};
+Choice choose(int rows, bool q8, long long pages) {
+    if (!q8 && (rows <= ROWS || (rows <= 2 * ROWS && pages * ((rows + ROWS - 1) / ROWS) <= 2 * sm_count()))) return {ROWS, PAGE, 1};
+    if (rows > 64) return {128, 128, 2};
+    if (rows <= 16) return {16, 128, 2};
+    return {rows <= 32 ? 32 : 64, 128, rows <= 32 ? 2 : 1};
 }
+template <int D, bool Q8>
+int launch(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
+    if (p.tile_rows == 128) return launch_tiles<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, EIGHTS>(p, st);
+    if constexpr (!Q8)
+        if (p.unit == PAGE) return launch_pieces<D>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, TILES>(p, st);
+    return launch_few<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, ROWWISE>(p, st);
+}
+
 }  // namespace
 }  // namespace tree
 }  // namespace ptb
 
 using namespace ptb;
 
-// Floats of workspace that ptb_paged_attn_tree needs.
+// Floats of workspace that ptb_paged_attn_tree needs, for either type of pages.
 PTB_API long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D) {
     if (Hk <= 0 || T <= 0) return 0;
-    const tree::Choice c = tree::choose(T * (H / Hk));
+    const tree::Choice c = tree::choose(T * (H / Hk), true, 0);    // the larger need
     return (long long)tree::sm_count() * 2 * c.parts * (long long)tree::partial_floats(c.tile_rows, D) + B + 1;
 }
 
@@ -598,7 +518,7 @@ PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_ro
     p.q = (const __nv_bfloat16*)q; p.q_batch = q_batch; p.q_row = q_row; p.out = (__nv_bfloat16*)out; p.lens = lens; p.nodes = nodes; p.mask = (const unsigned long long*)mask;
     p.page_table = page_table; p.pt_stride = pt_stride; p.n_pages = n_pages; p.k_exp = (const uint8_t*)k_exp; p.v_exp = (const uint8_t*)v_exp; p.v_raw = (const uint8_t*)v_pages; p.work = work;
     p.B = B; p.T = T; p.H = H; p.Hk = Hk; p.G = H / Hk;
-    const tree::Choice c = tree::choose(T * p.G);
+    const tree::Choice c = tree::choose(T * p.G, k_exp != nullptr, (long long)B * Hk * pt_stride);
     p.tile_rows = c.tile_rows;
     p.unit = c.unit;
     p.parts = c.parts;
@@ -611,6 +531,6 @@ PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_ro
     int dev = 0;
     PTB_CUDA_OK(cudaGetDevice(&dev));
     PTB_CUDA_OK(cudaSetDevice(dev));     // the tensor-map encoder is a driver call: bind the primary context to this thread
-    if (D == 128) return k_exp ? tree::launch_any<128, true>(p, k_pages, v_pages, st) : tree::launch_any<128, false>(p, k_pages, v_pages, st);
-    return k_exp ? tree::launch_any<64, true>(p, k_pages, v_pages, st) : tree::launch_any<64, false>(p, k_pages, v_pages, st);
+    if (D == 128) return k_exp ? tree::launch<128, true>(p, k_pages, v_pages, st) : tree::launch<128, false>(p, k_pages, v_pages, st);
+    return k_exp ? tree::launch<64, true>(p, k_pages, v_pages, st) : tree::launch<64, false>(p, k_pages, v_pages, st);
 }

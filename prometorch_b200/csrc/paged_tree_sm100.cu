@@ -30,7 +30,7 @@ constexpr int BQ = LANES;
 template <bool Q8> struct Split { static constexpr int THREADS = Q8 ? 640 : 512, SOFTMAX = Q8 ? 120 : 184, OTHER = Q8 ? 80 : 72; };
 template <int D, bool Q8>
 struct Sm {
-    static constexpr int Q_BYTES = BQ * D * 2, TILE = BLOCK * D * 2, RAW = BLOCK * D, PAGE_RAW = RAW / 2;
+    static constexpr int Q_BYTES = BQ * D * 2, TILE = BLOCK * D * 2, RAW = BLOCK * D;
     static constexpr int NK = Q8 ? 1 : D == 128 ? 2 : 3, NV = Q8 ? 2 : D == 128 ? 3 : 4, NR = Q8 ? (D == 128 ? 2 : 4) : 0;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NK * TILE, OFF_R = OFF_V + NV * TILE, OFF_E = OFF_R + NR * 2 * RAW;
     static constexpr int OFF_BAR = OFF_E + NR * 2 * BLOCK, OFF_PLAN = OFF_BAR + 1024;
@@ -122,11 +122,11 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                             if (n >= NR) ok = wait(&raw_empty[s], n / NR - 1);
                             if (ok) {
                                 bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
-                                mbar_expect_tx(&raw_full[s], there * (2 * S::PAGE_RAW + 2 * PAGE));
+                                mbar_expect_tx(&raw_full[s], there * (S::RAW + 2 * PAGE));
                                 for (int x = 0; x < there; ++x) {
                                     const int head = max(page[x], 0) * P.Hk + it.kvh;        // a page that is none of the pool's: any other in its place, which no row sees
-                                    tma_load_2d(sr + s * 2 * S::RAW + x * S::PAGE_RAW, &tmK, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
-                                    tma_load_2d(sr + s * 2 * S::RAW + S::RAW + x * S::PAGE_RAW, &tmV, 0, head * (S::PAGE_RAW / 128), &raw_full[s]);
+                                    tma_load_2d(sr + s * 2 * S::RAW + x * S::RAW / 2, &tmK, 0, head * (S::RAW / 256), &raw_full[s]);
+                                    tma_load_2d(sr + s * 2 * S::RAW + S::RAW + x * S::RAW / 2, &tmV, 0, head * (S::RAW / 256), &raw_full[s]);
                                     bulk_g2s(se + s * 2 * BLOCK + x * PAGE, P.k_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
                                     bulk_g2s(se + s * 2 * BLOCK + BLOCK + x * PAGE, P.v_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
                                 }
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                     }
                 }
             }
-            const float2 mine = on && it.n > g ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+            const float2 mine = on && it.n > g ? make_float2(m == -INFINITY && l != 0.f ? 0.f : m, l) : make_float2(-INFINITY, 0.f);      // a sum without a maximum is of no numbers
             if (live) *ml = mine;
             if (shared) both_sync();
             if (whole && live && it.n > g) {

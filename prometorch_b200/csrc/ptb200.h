@@ -299,7 +299,7 @@ long long ptb_paged_attn_work_floats(int B, int H, int D, int nsplit);
 int ptb_paged_attn_decode(const void* q, long long q_stride, void* out, int B, int H, int Hk, int D, const int* lens, const int* page_table, int pt_stride, int n_pages, const void* k_pages, const void* v_pages, float scale, float* work, int nsplit, int* status, cudaStream_t st);
 
 // ---------------------------------------------------------------------------- paged_tree.cu
-// Floats of workspace that ptb_paged_attn_tree needs.
+// Floats of workspace that ptb_paged_attn_tree needs, for either type of pages.
 long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D);
 
 // T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with

@@ -130,6 +130,27 @@ def test_trees(kind, D, H, Hk, T):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("T", [4, 8, 16, 40])
+@pytest.mark.parametrize("have", [30, 3000])
+@pytest.mark.parametrize("value", [math.nan, math.inf, 2.0 ** 40])
+def test_a_query_that_is_no_number_or_a_large_one(kind, T, have, value):
+    """It spoils its own row, whole or cut between CTAs, and no other."""
+    H, Hk, D, B = 8, 2, 128, 2
+    g = gen(T)
+    table, n_pages = table_for([have + T] * B, 3)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    q = torch.randn(B, T, H * D, device=DEV, generator=g).bfloat16()
+    lens = torch.full((B,), have, dtype=torch.int32, device=DEV)
+    want, mag = oracle(q, H, Hk, D, [have] * B, [T] * B, None, table, k, v, ke, ve, D ** -0.5)
+    spoilt = q.clone()
+    spoilt[1, 2, 3 * D + 5] = value
+    got = R.paged_attention_tree(spoilt, H, Hk, D, lens, table, k, v, k_exp=ke, v_exp=ve)
+    assert got[1, 2, 3 * D:4 * D].isnan().all() or math.isfinite(value)
+    got[1, 2, 3 * D:4 * D] = want[1, 2, 3 * D:4 * D].bfloat16()
+    close(got, want, mag, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("D", [64, 128])
 def test_one_node_is_the_decode_step(kind, D):
     """A whole batch of single tokens, lengths one after another: every place of the last token in a page."""
