@@ -352,19 +352,24 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
     }
 }
 
-// The partial results of items that were cut: one block per sixteen rows of an item, a thread (row, eight columns); and the rows that no unit belongs to, which are zeros.
+// The partial results of items that were cut: one block per sixteen rows of an item, a thread (row, eight columns, every SLICES-th result); and the rows that no unit belongs
+// to, which are zeros.  With few blocks a chain of loads is what it costs, and four shorter ones cost less (a chain of 5 behind 540 tokens, both kernels: 14.9 us with one,
+// 12.3 with four); with more blocks than the SMs hold, more threads only wait (64 nodes, 8 requests: 9 and 18 us).
 // How the accumulators of a partial result lie: TILES [D / 8][rows][8], place i of a row column i % 8 of product tile i / 8;
 // EIGHTS the same in the order of the head; ROWWISE [rows][D].
 enum Layout { TILES, EIGHTS, ROWWISE };
-template <int D, Layout LAYOUT>
-__global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_constant__ Params P) {
+template <int D, Layout LAYOUT, int SLICES>
+__global__ void __launch_bounds__(2 * D * SLICES) paged_tree_merge_kernel(const __grid_constant__ Params P) {
+    constexpr int OTHERS = SLICES > 1 ? SLICES - 1 : 1;
+    __shared__ float4 share[OTHERS][2][2 * D];
+    __shared__ float2 share_ml[OTHERS][2 * D];
     pdl_wait();
     pdl_launch_dependents();
     const int b = blockIdx.y, groups = min(P.tile_rows, (P.T * P.G + 15) / 16 * 16) / 16;
     const int i = blockIdx.x / groups, row0 = (blockIdx.x - i * groups) * 16;
     const int tile = i / P.Hk, kvh = i - tile * P.Hk;
     const Req r = req_of(P, b);
-    const int row = row0 + threadIdx.x % 16, c8 = threadIdx.x / 16, at = tile * P.tile_rows + row, node = at / P.G, g = at - node * P.G;
+    const int slice = threadIdx.x / (2 * D), tid = threadIdx.x % (2 * D), row = row0 + tid % 16, c8 = tid / 16, at = tile * P.tile_rows + row, node = at / P.G, g = at - node * P.G;
     float o[8], L = 0.f, M = -INFINITY;
 #pragma unroll
     for (int x = 0; x < 8; ++x) o[x] = 0.f;
@@ -377,13 +382,13 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
             return P.work + partial_at(P, c, c * per >= a ? 0 : 1, k % P.parts, D);
         };
         constexpr int AT_ONCE = 4;                       // fetched together, before any of them is needed
-        for (int k0 = 0; k0 < n; k0 += AT_ONCE) {
+        for (int k0 = slice; k0 < n; k0 += AT_ONCE * SLICES) {
             float2 ml[AT_ONCE];
             float4 v[AT_ONCE][2];
 #pragma unroll
             for (int x = 0; x < AT_ONCE; ++x)
-                if (k0 + x < n) {
-                    const float* p = from(k0 + x);
+                if (k0 + x * SLICES < n) {
+                    const float* p = from(k0 + x * SLICES);
                     ml[x] = *reinterpret_cast<const float2*>(p + (size_t)P.tile_rows * D + 2 * row);
                     const float4* q = reinterpret_cast<const float4*>(p + (LAYOUT == ROWWISE ? (size_t)row * D + c8 * 8 : (size_t)(c8 * P.tile_rows + row) * 8));
                     v[x][0] = q[0];
@@ -408,8 +413,34 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
                 o[4] += v[x][1].x * w; o[5] += v[x][1].y * w; o[6] += v[x][1].z * w; o[7] += v[x][1].w * w;
             }
         }
+        if constexpr (SLICES > 1) {                      // the slices', in their order
+            if (slice > 0) {
+                share_ml[slice - 1][tid] = make_float2(M, L);
+                share[slice - 1][0][tid] = make_float4(o[0], o[1], o[2], o[3]);
+                share[slice - 1][1][tid] = make_float4(o[4], o[5], o[6], o[7]);
+            }
+            __syncthreads();
+            if (slice > 0) return;
+            float mn = M;
+#pragma unroll
+            for (int x = 0; x < SLICES - 1; ++x) mn = fmaxf(mn, share_ml[x][tid].x);
+            const float old = M == -INFINITY ? 0.f : exp2f(M - mn);
+            L *= old;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) o[x] *= old;
+#pragma unroll
+            for (int x = 0; x < SLICES - 1; ++x) {
+                const float2 ml = share_ml[x][tid];
+                if (ml.x == -INFINITY) continue;
+                const float w = exp2f(ml.x - mn);
+                const float4 a = share[x][0][tid], b = share[x][1][tid];
+                L += ml.y * w;
+                o[0] += a.x * w; o[1] += a.y * w; o[2] += a.z * w; o[3] += a.w * w;
+                o[4] += b.x * w; o[5] += b.y * w; o[6] += b.z * w; o[7] += b.w * w;
+            }
+        }
     }
-    if (node >= P.T) return;
+    if (slice > 0 || node >= P.T) return;
     const bool on = node < r.nodes && L != 0.f;
     const float inv = on ? 1.f / L : 0.f;
     __nv_bfloat16* out = P.out + (((size_t)b * P.T + node) * P.H + kvh * P.G + g) * D;
@@ -428,7 +459,9 @@ __global__ void __launch_bounds__(2 * D) paged_tree_merge_kernel(const __grid_co
 template <int D, Layout LAYOUT>
 int launch_merge(const Params& p, cudaStream_t st) {
     const int groups = (p.T * p.G + 15) / 16 < p.tile_rows / 16 ? (p.T * p.G + 15) / 16 : p.tile_rows / 16;
-    PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, LAYOUT>, dim3(p.tiles * p.Hk * groups, p.B), dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
+    const dim3 grid(p.tiles * p.Hk * groups, p.B);
+    if ((int)(grid.x * grid.y) <= p.ctas) PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, LAYOUT, 4>, grid, dim3(8 * D), 0, st, ptb_pdl_enabled(), p));
+    else PTB_CUDA_OK(ptb_launch(paged_tree_merge_kernel<D, LAYOUT, 1>, grid, dim3(2 * D), 0, st, ptb_pdl_enabled(), p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }
@@ -464,7 +497,7 @@ int sm_count() {
 //   up to 16 rows, bf16: mma.sync.  16 requests of 8192 tokens, 8 rows of 128: 78.6 us, tokens along the lanes of tensor memory 81; one of 540 tokens, 4 rows: 12.2 and 17.7.
 //   up to 32 rows, bf16, and two pages a CTA at most: mma.sync, in one or two tiles.  One request of 540 tokens, 20 rows of 128: 14.9 us, tokens along the lanes 20.
 //   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 87 and 90 us, in tiles of 128 rows 104 and 108; e4m3, 64 rows over 4100
-//   tokens: 73 and 117.  e4m3, 4 rows over 8192 tokens, 32 requests: 84, where mma.sync, for which every warp converts what it reads, took 148.
+//   tokens: 73 and 117.  e4m3, 4 rows over 8192 tokens, 32 requests: 85, where mma.sync, for which every warp converts what it reads, took 148.
 //   more: tiles of 128 rows.
 struct Choice { int tile_rows, unit, parts; };
 Choice choose(int rows, bool q8, long long pages) {

@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                     if (lane == 0) {
                         const int there = page[1] == -2 ? 1 : 2, sK = n % NK, sV = n % NV;
                         if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
+                        else if (n >= 2) ok = wait(&k_full[n - 2], 0);               // two blocks under way at a time: what others fetch does not wait behind a whole ring
                         if (ok) {
                             bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
                             mbar_expect_tx(&k_full[sK], there * (S::TILE / 2 + (Q8 ? 2 * PAGE : 0)));
