@@ -9,7 +9,9 @@
 //
 // Two launches.  verify_stats_kernel reads every logit once: a chunk's maximum, its place, and the sum of exponentials; the bytes of the logits bound it.
 // verify_walk_kernel, a cluster per request, joins the chunks, walks, and draws from one row.  A draw has to fall on the same token for everybody, so that row's weights and
-// sums are held in fp64 (an fp32 cumulative sum over 150000 tokens is off by more than a token's share); the weights stay in shared memory between its steps.
+// sums are held in fp64 (an fp32 cumulative sum over 150000 tokens is off by more than a token's share).  Shared memory keeps the logits, half of the weights' size, and
+// two CTAs share an SM: a batch of 32 rows of 151936 is one wave (with the weights there, one CTA an SM, it was two: both launches 80 us, now 69, of which
+// the logits' bytes take 41).  Bound by the fp64 exponentials, 4.9 million of them.
 #include "common.cuh"
 #include <math.h>
 
@@ -17,10 +19,10 @@ namespace ptb {
 namespace {
 
 constexpr int VF_THREADS = 256, VF_EACH = 32, VF_CHUNK = VF_THREADS * VF_EACH;
-constexpr int VF_WALKERS = 1024;            // threads of the walk: fp64 exponentials and sums are long chains, so many run side by side
 constexpr int VF_NODES = 64;                 // nodes of a request
 constexpr int VF_CLUSTER = 16, VF_TOGETHER = 4;
-constexpr int VF_SLICE = 27 * 1024;          // weights a CTA can hold
+constexpr int VF_WIDE = 128;                 // CTAs of clusters of eight that surely find SMs of their own
+constexpr int VF_SLICE = 27 * 1024;          // logits, and the draft's probabilities, that a CTA can hold
 
 struct VerifyParams {
     const void* logits;              // [B, T, V] fp32 or bf16
@@ -36,7 +38,7 @@ struct VerifyParams {
     int* path;                       // [B, T]
     int* count;                      // [B]
     int* out;                        // [B, T]
-    int B, T, V, chunks, slice;      // slice: weights per CTA of the cluster
+    int B, T, V, chunks, slice;      // slice: tokens per CTA of the cluster
 };
 
 __device__ __forceinline__ float clean(float l) { return fmaxf(l, -INFINITY); }         // NaN is no token's logit
@@ -126,23 +128,25 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr, uint32_t rank) {
     return v;
 }
 // Sum over the block, the same for every thread (and in every order of arrival).
+template <int W>
 __device__ __forceinline__ double block_sum(double v, double* part) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = part[threadIdx.x & 31];
+    v = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int i = 0; i < W / 32; ++i) v += part[i];
     return v;
 }
 
-// One cluster a request; each CTA of it walks by itself (the tree is small) and holds the weights of `slice` tokens of the row that the last token is drawn from.
-template <bool BF16>
-__global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid_constant__ VerifyParams P) {
-    extern __shared__ double w[];
-    __shared__ double node_z[VF_NODES], node_w[VF_NODES], part[32], total_s[2];
+// One cluster a request; each CTA of it walks by itself (the tree is small) and holds `slice` logits of the row that the last token is drawn from.
+template <bool BF16, int W>
+__global__ void __launch_bounds__(W, 1024 / W) verify_walk_kernel(const __grid_constant__ VerifyParams P) {
+    extern __shared__ float kept[];                      // logits, then the draft's probabilities
+    constexpr int RUN = ((VF_SLICE + W - 1) / W) | 1;
+    __shared__ double node_z[VF_NODES], node_w[VF_NODES], part[W / 32], total_s[2], run_w[RUN];
     __shared__ float node_m[VF_NODES];
     __shared__ int node_at[VF_NODES], parent[VF_NODES], token[VF_NODES], next[VF_NODES], path[VF_NODES], gone[VF_NODES];
     __shared__ int length, n_gone, finder;
@@ -152,7 +156,7 @@ __global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid
     const int rank = (int)cluster_rank(), ranks = (int)cluster_size();
     if (n == 0) {                                        // the whole cluster agrees
         if (rank == 0) {
-            for (int i = tid; i < T; i += VF_WALKERS) { P.path[(size_t)b * T + i] = -1; P.out[(size_t)b * T + i] = -1; }
+            for (int i = tid; i < T; i += W) { P.path[(size_t)b * T + i] = -1; P.out[(size_t)b * T + i] = -1; }
             if (tid == 0) P.count[b] = -1;
         }
         return;
@@ -166,8 +170,8 @@ __global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid
         token[tid] = P.tokens[(size_t)b * T + tid];
         next[tid] = VF_NODES;
     }
-    if (tid == 0) { n_gone = 0; finder = VF_WALKERS; }
-    for (int i = warp; i < n; i += VF_WALKERS / 32) {    // the chunks of a node's row
+    if (tid == 0) { n_gone = 0; finder = W; }
+    for (int i = warp; i < n; i += W / 32) {    // the chunks of a node's row
         const float4* st = P.stats + ((size_t)b * T + i) * P.chunks;
         float m = -INFINITY;
         int at = 0x7fffffff;
@@ -225,7 +229,7 @@ __global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid
     __syncthreads();
     const int last = length, end = path[last];
     if (rank == 0) {
-        for (int i = tid; i < T; i += VF_WALKERS) {
+        for (int i = tid; i < T; i += W) {
             P.path[(size_t)b * T + i] = i <= last ? path[i] : -1;
             if (i != last) P.out[(size_t)b * T + i] = i < last ? token[path[i + 1]] : -1;
             else if (greedy) P.out[(size_t)b * T + i] = node_at[end];
@@ -234,40 +238,48 @@ __global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid
     }
     if (greedy) return;
     if (child && parent[tid] == end) gone[atomicAdd(&n_gone, 1)] = token[tid];
+    __syncthreads();
     const int v0 = rank * P.slice, len = max(0, min(P.slice, P.V - v0));
     const float m = node_m[end];
-    for (int k0 = tid; k0 < len; k0 += VF_TOGETHER * VF_WALKERS) {          // several at a time: loads and exponentials overlap
-        float l[VF_TOGETHER];
-        double x[VF_TOGETHER];
-#pragma unroll
-        for (int i = 0; i < VF_TOGETHER; ++i) l[i] = k0 + i * VF_WALKERS < len ? logit_at<BF16>(P, b, end, v0 + k0 + i * VF_WALKERS) : -INFINITY;
-#pragma unroll
-        for (int i = 0; i < VF_TOGETHER; ++i) x[i] = exp(((double)l[i] - (double)m) * inv);
-#pragma unroll
-        for (int i = 0; i < VF_TOGETHER; ++i)
-            if (k0 + i * VF_WALKERS < len) w[k0 + i * VF_WALKERS] = l[i] == -INFINITY ? 0.0 : l[i] == m ? 1.0 : x[i];
-    }
+    for (int k = tid; k < len; k += W) kept[k] = logit_at<BF16>(P, b, end, v0 + k);
+    const bool rest = P.probs && n_gone > 0;         // a child was rejected: what the draft's distribution leaves of the target's
+    float* q = kept + P.slice;
+    if (rest)
+        for (int k = tid; k < len; k += W) q[k] = P.probs[(size_t)b * P.p_batch + (size_t)end * P.p_row + v0 + k];
     __syncthreads();
-    if (P.probs && n_gone > 0) {                         // what the draft's distribution leaves of the target's
-        double s = 0;
-        for (int k = tid; k < len; k += VF_WALKERS) s += w[k];
-        s = block_sum(s, part);
-        if (tid == 0) total_s[0] = s;
-        cluster_sync();
-        double z = 0;
-        for (int r = 0; r < ranks; ++r) z += ld_cluster_f64(smem_u32(&total_s[0]), r);
-        const float* q = P.probs + (size_t)b * P.p_batch + (size_t)end * P.p_row + v0;
-        for (int k = tid; k < len; k += VF_WALKERS) w[k] = fmax(w[k] / z - (double)q[k], 0.0);
-    } else if (tid < n_gone) {
+    if (!rest && tid < n_gone) {
         const int g = gone[tid] - v0;
-        if (g >= 0 && g < len) w[g] = 0;
+        if (g >= 0 && g < len) kept[g] = -INFINITY;
     }
     __syncthreads();
     // each thread sums a run of neighbours (an odd number: no two lanes of a warp meet in a bank), the block scans the sums
-    const int run = ((P.slice + VF_WALKERS - 1) / VF_WALKERS) | 1, k0 = min(len, tid * run), k1 = min(len, k0 + run);
-    double mine = 0;
-#pragma unroll 4
-    for (int k = k0; k < k1; ++k) mine += w[k];
+    const int run = ((P.slice + W - 1) / W) | 1, k0 = min(len, tid * run), k1 = min(len, k0 + run);
+    double z = 1.0;
+    auto left = [&](int k) {                             // the weight of a token
+        const double x = weight(kept[k], m, inv);
+        return rest ? fmax(x / z - (double)q[k], 0.0) : x;
+    };
+    auto sum_run = [&] {
+        double s = 0;
+        for (int k = k0; k < k1; k += VF_TOGETHER) {     // several at a time: exponentials overlap
+            double x[VF_TOGETHER];
+#pragma unroll
+            for (int i = 0; i < VF_TOGETHER; ++i) x[i] = k + i < k1 ? left(k + i) : 0.0;
+#pragma unroll
+            for (int i = 0; i < VF_TOGETHER; ++i) s += x[i];
+        }
+        return s;
+    };
+    if (rest) {                                          // first against nothing: the target's sum
+        double s = 0;
+        for (int k = k0; k < k1; ++k) s += weight(kept[k], m, inv);
+        s = block_sum<W>(s, part);
+        if (tid == 0) total_s[0] = s;
+        cluster_sync();
+        z = 0;
+        for (int r = 0; r < ranks; ++r) z += ld_cluster_f64(smem_u32(&total_s[0]), r);
+    }
+    const double mine = sum_run();
     double upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -277,13 +289,14 @@ __global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid
     if (lane == 31) part[warp] = upto;
     __syncthreads();
     if (warp == 0) {                                     // the warps' sums, scanned by one of them
-        double x = part[lane], up = x;
+        const double x = lane < W / 32 ? part[lane] : 0.0;
+        double up = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double y = __shfl_up_sync(0xffffffffu, up, o);
             if (lane >= o) up += y;
         }
-        part[lane] = up - x;
+        if (lane < W / 32) part[lane] = up - x;
         if (lane == 31) total_s[1] = up;
     }
     __syncthreads();
@@ -311,41 +324,44 @@ __global__ void __launch_bounds__(VF_WALKERS, 1) verify_walk_kernel(const __grid
     const double aim = target - base;
     if (mine > 0 && before + upto > aim) atomicMin(&finder, tid);
     __syncthreads();
-    if (finder == VF_WALKERS) {                          // rounding put the target behind the last sum: the last run with weight
+    if (finder == W) {                          // rounding put the target behind the last sum: the last run with weight
         __syncthreads();
         if (tid == 0) finder = -1;
         __syncthreads();
         if (mine > 0) atomicMax(&finder, tid);
         __syncthreads();
     }
-    if (tid == finder) {
+    const int found = finder, first = found * run, count = min(len, first + run) - first;      // the run that it falls into
+    if (tid < count) run_w[tid] = left(first + tid);
+    __syncthreads();
+    if (tid == found) {
         double c = before + (upto - mine);
         int pick = -1;
-        for (int k = k0; k < k1; ++k) {
-            if (w[k] <= 0) continue;
-            pick = k;
-            c += w[k];
+        for (int k = 0; k < count; ++k) {
+            if (run_w[k] <= 0) continue;
+            pick = first + k;
+            c += run_w[k];
             if (c > aim) break;
         }
         P.out[(size_t)b * T + last] = v0 + pick;
     }
 }
 
-template <bool BF16>
+template <bool BF16, int W>
 int launch_walk(const VerifyParams& p, int cluster, cudaStream_t st) {
     static bool attr[64];
     int dev = 0;
     PTB_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        PTB_CUDA_OK(cudaFuncSetAttribute(verify_walk_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, VF_SLICE * 8));
-        PTB_CUDA_OK(cudaFuncSetAttribute(verify_walk_kernel<BF16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        PTB_CUDA_OK(cudaFuncSetAttribute(verify_walk_kernel<BF16, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, VF_SLICE * 8));
+        PTB_CUDA_OK(cudaFuncSetAttribute(verify_walk_kernel<BF16, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         if (dev < 64) attr[dev] = true;
     }
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(cluster, p.B);
-    cfg.blockDim = dim3(VF_WALKERS);
-    cfg.dynamicSmemBytes = (size_t)p.slice * 8;
+    cfg.blockDim = dim3(W);
+    cfg.dynamicSmemBytes = (size_t)p.slice * (p.probs ? 8 : 4);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -354,7 +370,7 @@ int launch_walk(const VerifyParams& p, int cluster, cudaStream_t st) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = ptb_pdl_enabled() ? 2 : 1;
-    PTB_CUDA_OK(cudaLaunchKernelEx(&cfg, verify_walk_kernel<BF16>, p));
+    PTB_CUDA_OK(cudaLaunchKernelEx(&cfg, verify_walk_kernel<BF16, W>, p));
     return 0;
 }
 
@@ -390,7 +406,10 @@ PTB_API int ptb_verify_drafts(const void* logits, int bf16, long long l_batch, l
     const bool vec = !((uintptr_t)logits & 15) && l_batch % unit == 0 && l_row % unit == 0;
     void (*k)(VerifyParams) = bf16 ? (vec ? verify_stats_kernel<true, true> : verify_stats_kernel<true, false>) : (vec ? verify_stats_kernel<false, true> : verify_stats_kernel<false, false>);
     PTB_CUDA_OK(ptb_launch(k, dim3(p.chunks, B * T), dim3(VF_THREADS), 0, st, ptb_pdl_enabled(), p));
-    if (bf16 ? launch_walk<true>(p, cluster, st) : launch_walk<false>(p, cluster, st)) return -1;
+    // threads of a CTA of the walk: 1024 where each finds an SM of its own, else two of 512 share one
+    const bool wide = (long long)B * cluster <= VF_WIDE;
+    if (bf16 ? (wide ? launch_walk<true, 1024>(p, cluster, st) : launch_walk<true, 512>(p, cluster, st)) : (wide ? launch_walk<false, 1024>(p, cluster, st) : launch_walk<false, 512>(p, cluster, st)))
+        return -1;
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }

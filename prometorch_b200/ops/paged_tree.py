@@ -24,7 +24,7 @@ from .. import _native as N
 from .paged import PAGE, _status
 
 E4M3 = torch.float8_e4m3fn
-MAX_NODES = 64
+MAX_NODES, MAX_REQUESTS = 64, 1024
 _LARGEST, _E_MIN, _E_MAX = 448.0, -64, 64
 
 
@@ -82,7 +82,16 @@ class _Device:
             torch.cuda.set_device(self.old)
 
 
-_looks = operator.attrgetter("shape", "dtype", "device")
+_shape, _dtype = operator.attrgetter("shape"), operator.attrgetter("dtype")
+
+
+def _alike(tensors: Sequence[torch.Tensor], shape: tuple, dtype: torch.dtype, index: int) -> bool:
+    """Contiguous, of one shape, type and device (its index, -1 for the host).  A pass over all of them for each: models have hundreds of pools, and a check in turn costs more."""
+    n = len(tensors)
+    return (list(map(_shape, tensors)).count(shape) == n and list(map(_dtype, tensors)).count(dtype) == n and list(map(torch.Tensor.get_device, tensors)).count(index) == n
+            and all(map(torch.Tensor.is_contiguous, tensors)))
+
+
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
@@ -187,7 +196,7 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
 def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.Tensor, page_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                          mask: Optional[torch.Tensor] = None, nodes: Optional[torch.Tensor] = None, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None,
                          scale: Optional[float] = None) -> torch.Tensor:
-    """``q [B, T, >= H D]``: up to 64 drafted tokens of each request (heads packed along the row), node i of request b in slot ``lens[b] + i`` of the pages
+    """``q [B, T, >= H D]``: up to 64 drafted tokens of each of up to 1024 requests (heads packed along the row), node i of request b in slot ``lens[b] + i`` of the pages
     ``page_table[b]``.  It sees the ``lens[b]`` cached tokens and the nodes j of its request whose bit j is set in ``mask[b, i]`` (int64; None: a chain, nodes 0 to i).  ``nodes [B]``: how
     many of the T are there (None: all).  Returns ``[B, T, H D]``; rows behind ``nodes[b]`` and rows that see nothing are zeros.  e4m3 pages come with ``k_exp`` and ``v_exp``."""
     if q.dim() != 3 or Hk <= 0 or H <= 0 or H % Hk or q.shape[2] < H * D:
@@ -196,6 +205,8 @@ def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.T
     dev = q.device
     if not 1 <= T <= MAX_NODES:
         raise ValueError(f"paged_attention_tree: 1 to {MAX_NODES} nodes a request, not {T}")
+    if B > MAX_REQUESTS:
+        raise ValueError(f"paged_attention_tree: up to {MAX_REQUESTS} requests, not {B}")
     _pools(q, Hk, D, k_pages, v_pages, k_exp, v_exp)
     _index(lens, dev, (B,), "paged_attention_tree: lens")
     if nodes is not None:
@@ -271,12 +282,12 @@ def paged_keep(layers: Sequence[Sequence[Optional[torch.Tensor]]], lens: torch.T
     if k0.dim() != 4 or k0.shape[2] != PAGE:
         raise ValueError(f"paged_keep: pages [page, kv head, {PAGE}, D], not {list(k0.shape)}")
     pools, exps = ks + vs, kes + ves
-    if list(map(_looks, pools)).count(_looks(k0)) != 2 * n or not all(map(torch.Tensor.is_contiguous, pools)):
+    if not _alike(pools, k0.shape, k0.dtype, k0.get_device()):
         raise ValueError("paged_keep: layers need contiguous pools of one shape, type and device")
-    none = sum(e is None for e in exps)
-    if not quant and none != 2 * n:
+    there = sum(map(torch.is_tensor, exps))
+    if not quant and there:
         raise ValueError("paged_keep: only e4m3 pools have exponents")
-    if quant and (none or list(map(_looks, exps)).count((k0.shape[:3], torch.uint8, dev)) != 2 * n or not all(map(torch.Tensor.is_contiguous, exps))):
+    if quant and (there != 2 * n or not _alike(exps, k0.shape[:3], torch.uint8, k0.get_device())):
         raise ValueError(f"paged_keep: exponents are contiguous uint8 [page, kv head, {PAGE}] on {dev}, for e4m3 pools all of them")
     if path.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] != path.shape[0]:
         raise ValueError(f"paged_keep: a path [B, T] and a row of pages for each request, not {list(path.shape)} and {list(page_table.shape)}")

@@ -132,6 +132,12 @@ def test_attention_refuses(kw):
         call_attend(**kw)
 
 
+def test_attention_refuses_more_requests_than_a_launch_can_plan():
+    n = R.MAX_REQUESTS + 1
+    with pytest.raises(ValueError, match="requests"):
+        call_attend(q=torch.zeros(n, 1, 256), lens=torch.zeros(n, dtype=torch.int32), page_table=torch.zeros(n, 1, dtype=torch.int32))
+
+
 @pytest.mark.parametrize("kw", [dict(page_table=i32(0, 2)[None], lens=i32(70)), dict(page_table=i32(-1, 0)[None]), dict(lens=i32(126)), dict(lens=i32(-1))])
 def test_attention_outside_the_pool(kw):
     with pytest.raises(IndexError):

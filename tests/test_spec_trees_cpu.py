@@ -104,3 +104,13 @@ def test_refusals():
         eng = LLMEngine(device="cpu", **kw)
         with pytest.raises(ValueError):
             eng.set_weights(type("W", (), {"cfg": KifusunConfig(vocab_size=64, hidden_size=32, embed_scale=1.0, eps=1e-6)})())
+
+
+@pytest.mark.parametrize("kw", [dict(kv_dtype="e4m3"), dict(spec_tokens=2, spec_branches=1), dict()])
+def test_more_requests_than_the_attention_of_trees_takes(kw):
+    eng = LLMEngine(device="cpu", max_active=1025, max_pages=4, **kw)
+    if kw:
+        with pytest.raises(ValueError, match="max_active"):
+            eng.set_weights(LlamaWeights.random(tiny(), seed=1))
+    else:
+        eng.set_weights(LlamaWeights.random(tiny(), seed=1))
