@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import array
 import ctypes as C
+import functools
 import math
 import operator
 from typing import Optional, Sequence, Tuple
@@ -21,7 +22,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from .. import _native as N
-from .paged import PAGE, _status
+from .paged import PAGE, _STATUS, _status
 
 E4M3 = torch.float8_e4m3fn
 MAX_NODES, MAX_REQUESTS = 64, 1024
@@ -42,44 +43,42 @@ def _decls(L):
         L.ptb_paged_tree_work_floats.restype = ll
 
 
-def _index(t: torch.Tensor, dev: torch.device, shape: tuple, name: str) -> None:
-    """int32, contiguous, on the device."""
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+def _index(t: torch.Tensor, dev: torch.device, at: int, shape: tuple, name: str) -> None:
+    """int32, contiguous, on the device (`at`: its index, -1 for the host)."""
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != at:
         raise ValueError(f"{name}: a contiguous int32 tensor {list(shape)} on {dev} is needed, not {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _pools(like, Hk: int, D: int, k_pages, v_pages, k_exp, v_exp) -> bool:
+def _pools(like, at: int, Hk: int, D: int, k_pages, v_pages, k_exp, v_exp) -> bool:
     """Checks a layer's pools; whether they are quantised."""
-    quant, shape, dev = k_pages.dtype == E4M3, k_pages.shape, like.device
-    if k_pages.dtype != v_pages.dtype or not (quant or k_pages.dtype == like.dtype):
+    kind, shape = k_pages.dtype, k_pages.shape
+    quant = kind is E4M3
+    if kind is not v_pages.dtype or not (quant or kind is like.dtype):
         raise ValueError(f"pages: {k_pages.dtype} and {v_pages.dtype} for {like.dtype} tokens")
-    if len(shape) != 4 or shape[1] != Hk or shape[2] != PAGE or shape[3] != D or v_pages.shape != shape:
+    if len(shape) != 4 or shape[1:] != (Hk, PAGE, D) or v_pages.shape != shape:
         raise ValueError(f"pages: [page, {Hk}, {PAGE}, {D}] is needed, not {list(shape)} and {list(v_pages.shape)}")
     if (k_exp is not None) != quant or (v_exp is not None) != quant:
         raise ValueError("pages: e4m3 pages come with exponents of keys and of values, others without")
-    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.device == dev and v_pages.device == dev):
-        raise ValueError(f"pages: contiguous pools on {dev} are needed")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.get_device() == at and v_pages.get_device() == at):
+        raise ValueError(f"pages: contiguous pools on {like.device} are needed")
     if quant:
         for t in (k_exp, v_exp):
-            if t.dtype != torch.uint8 or t.shape != shape[:3] or not t.is_contiguous() or t.device != dev:
-                raise ValueError(f"pages: exponents are contiguous uint8 [page, kv head, 64] on {dev}")
+            if t.dtype is not torch.uint8 or t.shape != shape[:3] or not t.is_contiguous() or t.get_device() != at:
+                raise ValueError(f"pages: exponents are contiguous uint8 [page, kv head, 64] on {like.device}")
     return quant
 
 
-class _Device:
-    """Makes a device the current one for the length of a launch, if it is not."""
+def _launch(at: int, entry, *args) -> int:
+    """Calls an entry that launches, with the device current for its length and the current stream behind the arguments."""
+    if torch.cuda.current_device() == at:
+        return entry(*args, _stream(at))
+    with torch.cuda.device(at):
+        return entry(*args, _stream(at))
 
-    def __init__(self, dev: torch.device):
-        self.index = dev.index
 
-    def __enter__(self):
-        self.old = torch.cuda.current_device()
-        if self.old != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *_):
-        if self.old != self.index:
-            torch.cuda.set_device(self.old)
+def _status_ptr(dev: torch.device, at: int) -> int:
+    t = _STATUS.get(at)
+    return (t if t is not None else _status(dev)).data_ptr()
 
 
 _shape, _dtype = operator.attrgetter("shape"), operator.attrgetter("dtype")
@@ -130,20 +129,20 @@ def paged_write(qkv: torch.Tensor, H: int, Hk: int, D: int, pos: torch.Tensor, r
     """Rotates q and k of the ``n`` tokens of ``qkv [n, >= (H + 2 Hk) D]`` (pairs (j, j + D/2)) to the positions ``pos`` and stores k and v at
     ``page_table[req[i], slot[i] // 64]``, place ``slot[i] % 64``.  ``slot`` None: the position; a negative one is not stored (padding).  No two tokens have one slot.  e4m3 pages
     come with ``k_exp`` and ``v_exp``.  Returns the rotated ``q [n, H D]`` and, if asked for, the rotated keys ``[n, Hk, D]`` as they were before quantising."""
-    width, dev = (H + 2 * Hk) * D, qkv.device
+    width, dev, home = (H + 2 * Hk) * D, qkv.device, qkv.get_device()
     if qkv.dim() != 2 or qkv.shape[1] < width or H < 0 or Hk <= 0 or D <= 0 or D % 2:
         raise ValueError(f"paged_write: rows of {width} values for {H} + 2 x {Hk} heads of {D} are needed, not {list(qkv.shape)}")
     n = qkv.shape[0]
-    quant = _pools(qkv, Hk, D, k_pages, v_pages, k_exp, v_exp)
-    _index(pos, dev, (n,), "paged_write: pos")
-    _index(req, dev, (n,), "paged_write: req")
+    quant = _pools(qkv, home, Hk, D, k_pages, v_pages, k_exp, v_exp)
+    _index(pos, dev, home, (n,), "paged_write: pos")
+    _index(req, dev, home, (n,), "paged_write: req")
     if slot is not None:
-        _index(slot, dev, (n,), "paged_write: slot")
+        _index(slot, dev, home, (n,), "paged_write: slot")
     if page_table.dim() != 2:
         raise ValueError("paged_write: page_table [requests, pages]")
-    _index(page_table, dev, page_table.shape, "paged_write: page_table")
+    _index(page_table, dev, home, page_table.shape, "paged_write: page_table")
     if not (cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == D // 2 and cos.is_contiguous() and sin.is_contiguous()
-            and cos.device == dev and sin.device == dev):
+            and cos.get_device() == home and sin.get_device() == home):
         raise ValueError(f"paged_write: contiguous fp32 tables [positions, {D // 2}] on {dev} are needed")
     if qkv.is_cuda:
         if qkv.dtype != torch.bfloat16 or D not in (64, 128):
@@ -153,10 +152,9 @@ def paged_write(qkv: torch.Tensor, H: int, Hk: int, D: int, pos: torch.Tensor, r
             qkv, ld = torch.empty(n, width, dtype=qkv.dtype, device=dev).copy_(qkv[:, :width]), width
         q = torch.empty(n, H * D, dtype=torch.bfloat16, device=dev)
         k = torch.empty(n, Hk, D, dtype=torch.bfloat16, device=dev) if want_k else None
-        with _Device(dev):
-            rc = N.lib().ptb_paged_write(qkv.data_ptr(), ld, n, H, Hk, D, pos.data_ptr(), N.ptr(slot), req.data_ptr(), page_table.data_ptr(), page_table.shape[1], page_table.shape[0],
-                                         k_pages.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), N.ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp),
-                                         N.ptr(v_exp), _status(dev).data_ptr(), _stream(dev.index))
+        rc = _launch(home, N.lib().ptb_paged_write, qkv.data_ptr(), ld, n, H, Hk, D, pos.data_ptr(), N.ptr(slot), req.data_ptr(), page_table.data_ptr(), page_table.shape[1],
+                     page_table.shape[0], k_pages.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), N.ptr(k), k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp),
+                     N.ptr(v_exp), _status_ptr(dev, home))
         if rc:
             N.check(rc, "paged_write")
         return q, k
@@ -193,6 +191,11 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
     return mask
 
 
+@functools.lru_cache(maxsize=1024)
+def _work_floats(B: int, T: int, H: int, Hk: int, D: int) -> int:
+    return N.lib().ptb_paged_tree_work_floats(B, T, H, Hk, D)
+
+
 def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.Tensor, page_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                          mask: Optional[torch.Tensor] = None, nodes: Optional[torch.Tensor] = None, k_exp: Optional[torch.Tensor] = None, v_exp: Optional[torch.Tensor] = None,
                          scale: Optional[float] = None) -> torch.Tensor:
@@ -202,19 +205,19 @@ def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.T
     if q.dim() != 3 or Hk <= 0 or H <= 0 or H % Hk or q.shape[2] < H * D:
         raise ValueError(f"paged_attention_tree: [B, T, {H} x {D}] over {Hk} kv heads, not {list(q.shape)}")
     B, T, _ = q.shape
-    dev = q.device
+    dev, home = q.device, q.get_device()
     if not 1 <= T <= MAX_NODES:
         raise ValueError(f"paged_attention_tree: 1 to {MAX_NODES} nodes a request, not {T}")
     if B > MAX_REQUESTS:
         raise ValueError(f"paged_attention_tree: up to {MAX_REQUESTS} requests, not {B}")
-    _pools(q, Hk, D, k_pages, v_pages, k_exp, v_exp)
-    _index(lens, dev, (B,), "paged_attention_tree: lens")
+    _pools(q, home, Hk, D, k_pages, v_pages, k_exp, v_exp)
+    _index(lens, dev, home, (B,), "paged_attention_tree: lens")
     if nodes is not None:
-        _index(nodes, dev, (B,), "paged_attention_tree: nodes")
+        _index(nodes, dev, home, (B,), "paged_attention_tree: nodes")
     if page_table.dim() != 2 or page_table.shape[0] != B:
         raise ValueError(f"paged_attention_tree: a row of pages for each of {B} requests, not {list(page_table.shape)}")
-    _index(page_table, dev, page_table.shape, "paged_attention_tree: page_table")
-    if mask is not None and not (mask.dtype == torch.int64 and mask.shape == (B, T) and mask.is_contiguous() and mask.device == dev):
+    _index(page_table, dev, home, page_table.shape, "paged_attention_tree: page_table")
+    if mask is not None and not (mask.dtype is torch.int64 and mask.shape == (B, T) and mask.is_contiguous() and mask.get_device() == home):
         raise ValueError(f"paged_attention_tree: a contiguous int64 mask [{B}, {T}] on {dev} is needed")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     if not 1e-30 < scale < 1e30:
@@ -227,12 +230,9 @@ def paged_attention_tree(q: torch.Tensor, H: int, Hk: int, D: int, lens: torch.T
             q = torch.empty(B, T, H * D, dtype=q.dtype, device=dev).copy_(q[:, :, :H * D])
             s0, s1, s2 = q.stride()
         out = torch.empty(B, T, H * D, dtype=torch.bfloat16, device=dev)
-        L = N.lib()
-        with _Device(dev):
-            work = torch.empty(L.ptb_paged_tree_work_floats(B, T, H, Hk, D), dtype=torch.float32, device=dev)
-            rc = L.ptb_paged_attn_tree(q.data_ptr(), s0, s1, out.data_ptr(), B, T, H, Hk, D, lens.data_ptr(), N.ptr(nodes), N.ptr(mask), page_table.data_ptr(), page_table.shape[1],
-                                       k_pages.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp), N.ptr(v_exp), scale, work.data_ptr(), _status(dev).data_ptr(),
-                                       _stream(dev.index))
+        work = torch.empty(_work_floats(B, T, H, Hk, D), dtype=torch.float32, device=dev)
+        rc = _launch(home, N.lib().ptb_paged_attn_tree, q.data_ptr(), s0, s1, out.data_ptr(), B, T, H, Hk, D, lens.data_ptr(), N.ptr(nodes), N.ptr(mask), page_table.data_ptr(),
+                     page_table.shape[1], k_pages.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), N.ptr(k_exp), N.ptr(v_exp), scale, work.data_ptr(), _status_ptr(dev, home))
         if rc:
             N.check(rc, "paged_attention_tree")
         return out
@@ -278,35 +278,34 @@ def paged_keep(layers: Sequence[Sequence[Optional[torch.Tensor]]], lens: torch.T
         return
     ks, vs, kes, ves = zip(*[l if len(l) == 4 else (*l, None, None) for l in layers])
     k0 = ks[0]
-    dev, quant = k0.device, k0.dtype == E4M3
+    dev, home, quant = k0.device, k0.get_device(), k0.dtype is E4M3
     if k0.dim() != 4 or k0.shape[2] != PAGE:
         raise ValueError(f"paged_keep: pages [page, kv head, {PAGE}, D], not {list(k0.shape)}")
     pools, exps = ks + vs, kes + ves
-    if not _alike(pools, k0.shape, k0.dtype, k0.get_device()):
+    if not _alike(pools, k0.shape, k0.dtype, home):
         raise ValueError("paged_keep: layers need contiguous pools of one shape, type and device")
     there = sum(map(torch.is_tensor, exps))
     if not quant and there:
         raise ValueError("paged_keep: only e4m3 pools have exponents")
-    if quant and (there != 2 * n or not _alike(exps, k0.shape[:3], torch.uint8, k0.get_device())):
+    if quant and (there != 2 * n or not _alike(exps, k0.shape[:3], torch.uint8, home)):
         raise ValueError(f"paged_keep: exponents are contiguous uint8 [page, kv head, {PAGE}] on {dev}, for e4m3 pools all of them")
     if path.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] != path.shape[0]:
         raise ValueError(f"paged_keep: a path [B, T] and a row of pages for each request, not {list(path.shape)} and {list(page_table.shape)}")
     B, T = path.shape
     if T > MAX_NODES:
         raise ValueError(f"paged_keep: up to {MAX_NODES} nodes a request, not {T}")
-    _index(path, dev, (B, T), "paged_keep: path")
-    _index(lens, dev, (B,), "paged_keep: lens")
-    _index(count, dev, (B,), "paged_keep: count")
-    _index(page_table, dev, page_table.shape, "paged_keep: page_table")
+    _index(path, dev, home, (B, T), "paged_keep: path")
+    _index(lens, dev, home, (B,), "paged_keep: lens")
+    _index(count, dev, home, (B,), "paged_keep: count")
+    _index(page_table, dev, home, page_table.shape, "paged_keep: page_table")
     if k0.is_cuda:
         row = k0.shape[3] * k0.element_size()
         if row % 16:
             raise ValueError(f"paged_keep: rows of 16-byte pieces are needed, not {row} bytes")
         at = list(map(torch.Tensor.data_ptr, pools + exps)) if quant else list(map(torch.Tensor.data_ptr, pools)) + [0] * (2 * n)
         ptrs = array.array("Q", at)                  # all keys, all values, all exponents of keys, all of values
-        with _Device(dev):
-            rc = N.lib().ptb_paged_keep(ptrs.buffer_info()[0], n, B, T, k0.shape[1], row, k0.shape[0], lens.data_ptr(), path.data_ptr(), count.data_ptr(), page_table.data_ptr(),
-                                        page_table.shape[1], _status(dev).data_ptr(), _stream(dev.index))
+        rc = _launch(home, N.lib().ptb_paged_keep, ptrs.buffer_info()[0], n, B, T, k0.shape[1], row, k0.shape[0], lens.data_ptr(), path.data_ptr(), count.data_ptr(), page_table.data_ptr(),
+                     page_table.shape[1], _status_ptr(dev, home))
         if rc:
             N.check(rc, "paged_keep")
         return

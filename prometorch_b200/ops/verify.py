@@ -8,12 +8,13 @@ CUDA tensors go through csrc/verify.cu (logits read once, the draw's row in fp64
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _native as N
-from .paged_tree import _Device, _index, _stream
+from .paged_tree import _index, _launch
 
 MAX_NODES = 64
 
@@ -28,9 +29,14 @@ def _decls(L):
         L.ptb_verify_work_bytes.restype = ll
 
 
-def _floats(t: torch.Tensor, dev: torch.device, shape: tuple, name: str) -> None:
-    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+def _floats(t: torch.Tensor, dev: torch.device, at: int, shape: tuple, name: str) -> None:
+    if t.dtype is not torch.float32 or t.shape != shape or not t.is_contiguous() or t.get_device() != at:
         raise ValueError(f"verify_drafts: {name} is a contiguous fp32 tensor {list(shape)} on {dev}, not {t.dtype} {list(t.shape)} on {t.device}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _work_bytes(B: int, T: int, V: int) -> int:
+    return N.lib().ptb_verify_work_bytes(B, T, V)
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor, parents: Optional[torch.Tensor] = None,
@@ -48,19 +54,19 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, t
     if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"verify_drafts: fp32 or bf16 logits [B, T, V] are needed, not {logits.dtype} {list(logits.shape)}")
     B, T, V = logits.shape
-    dev = logits.device
+    dev, home = logits.device, logits.get_device()
     if not 1 <= T <= MAX_NODES or V < 1:
         raise ValueError(f"verify_drafts: 1 to {MAX_NODES} nodes a request and a vocabulary, not {T} and {V}")
-    _index(tokens, dev, (B, T), "verify_drafts: tokens")
+    _index(tokens, dev, home, (B, T), "verify_drafts: tokens")
     if parents is not None:
-        _index(parents, dev, (B, T), "verify_drafts: parents")
+        _index(parents, dev, home, (B, T), "verify_drafts: parents")
         if draft_probs is not None:
             raise ValueError("verify_drafts: draft probabilities go with chains")
     if nodes is not None:
-        _index(nodes, dev, (B,), "verify_drafts: nodes")
-    _floats(u, dev, (B, T), "u")
-    _floats(temperature, dev, (B,), "temperature")
-    if draft_probs is not None and (draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape or draft_probs.device != dev):
+        _index(nodes, dev, home, (B,), "verify_drafts: nodes")
+    _floats(u, dev, home, (B, T), "u")
+    _floats(temperature, dev, home, (B,), "temperature")
+    if draft_probs is not None and (draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape or draft_probs.get_device() != home):
         raise ValueError(f"verify_drafts: draft_probs are fp32 {[B, T, V]} on {dev}, not {draft_probs.dtype} {list(draft_probs.shape)} on {draft_probs.device}")
     if logits.is_cuda:
         if logits.stride(2) != 1:
@@ -71,13 +77,12 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, t
                 draft_probs = draft_probs.contiguous()
             p_batch, p_row, _ = draft_probs.stride()
         l_batch, l_row, _ = logits.stride()
+        path, out = torch.empty(2, B, T, dtype=torch.int32, device=dev).unbind(0)
+        count = torch.empty(B, dtype=torch.int32, device=dev)
         L = N.lib()
-        ints = torch.empty((2 * T + 1) * B, dtype=torch.int32, device=dev)
-        path, out, count = ints[:B * T].view(B, T), ints[B * T:2 * B * T].view(B, T), ints[2 * B * T:]
-        with _Device(dev):
-            work = torch.empty(L.ptb_verify_work_bytes(B, T, V), dtype=torch.uint8, device=dev)
-            rc = L.ptb_verify_drafts(logits.data_ptr(), int(logits.dtype == torch.bfloat16), l_batch, l_row, N.ptr(draft_probs), p_batch, p_row, tokens.data_ptr(), N.ptr(parents),
-                                     N.ptr(nodes), u.data_ptr(), temperature.data_ptr(), work.data_ptr(), path.data_ptr(), count.data_ptr(), out.data_ptr(), B, T, V, _stream(dev.index))
+        work = torch.empty(_work_bytes(B, T, V), dtype=torch.uint8, device=dev)
+        rc = _launch(home, L.ptb_verify_drafts, logits.data_ptr(), int(logits.dtype is torch.bfloat16), l_batch, l_row, N.ptr(draft_probs), p_batch, p_row, tokens.data_ptr(),
+                     N.ptr(parents), N.ptr(nodes), u.data_ptr(), temperature.data_ptr(), work.data_ptr(), path.data_ptr(), count.data_ptr(), out.data_ptr(), B, T, V)
         if rc:
             N.check(rc, "verify_drafts")
         return path, count, out
