@@ -523,8 +523,14 @@ using namespace ptb;
 // Floats of workspace that ptb_paged_attn_tree needs, for either type of pages.
 PTB_API long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D) {
     if (Hk <= 0 || T <= 0) return 0;
-    const tree::Choice c = tree::choose(T * (H / Hk), true, 0);    // the larger need
-    return (long long)tree::sm_count() * 2 * c.parts * (long long)tree::partial_floats(c.tile_rows, D) + B + 1;
+    long long most = 0;
+    for (const bool q8 : {false, true})                  // page tables with little room take the smallest tiles
+        for (const long long pages : {0ll, 1ll << 40}) {
+            const tree::Choice c = tree::choose(T * (H / Hk), q8, pages);
+            const long long n = (long long)tree::sm_count() * 2 * c.parts * (long long)tree::partial_floats(c.tile_rows, D);
+            most = n > most ? n : most;
+        }
+    return most + B + 1;
 }
 
 // T drafted tokens of each of B requests (the latest token among them) attend to their request's cached tokens and to one another.  q: [B, T, heads] bf16 with

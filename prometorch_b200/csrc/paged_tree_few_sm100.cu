@@ -706,11 +706,9 @@ int launch_few(const Params& p, const void* k_pages, const void* v_pages, cudaSt
         return Q8 && D == 64 ? ptb_make_tmap_64b(m, pages, rows, PAGE) : ptb_make_tmap_bf16(m, pages, Q8 ? 64 : D, rows, Q8 ? 64 : D, 64, PAGE);
     };
     if (map(&mk, k_pages) || map(&mv, v_pages)) return -1;
-    switch (p.tile_rows) {
-        case 16: return launch_n<D, Q8, 16>(p, mk, mv, st);
-        case 32: return launch_n<D, Q8, 32>(p, mk, mv, st);
-        default: return launch_n<D, Q8, 64>(p, mk, mv, st);
-    }
+    if constexpr (Q8)                                    // bf16 pages: mma.sync
+        if (p.tile_rows == 16) return launch_n<D, Q8, 16>(p, mk, mv, st);
+    return p.tile_rows == 32 ? launch_n<D, Q8, 32>(p, mk, mv, st) : launch_n<D, Q8, 64>(p, mk, mv, st);
 }
 template int launch_few<64, false>(const Params&, const void*, const void*, cudaStream_t);
 template int launch_few<64, true>(const Params&, const void*, const void*, cudaStream_t);

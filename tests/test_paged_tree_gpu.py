@@ -130,6 +130,59 @@ def test_trees(kind, D, H, Hk, T):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 5, 8, 16, 40])
+@pytest.mark.parametrize("up", [True, False])
+def test_scores_that_rise_or_fall_along_the_cache(kind, D, T, up):
+    """By several powers of two from block to block: references are outgrown again and again, or the first tokens outweigh all others.
+
+    One rounding of the result and of each weight, as everywhere; a score is off by at most D fp32 roundings of its terms' magnitudes, and (e4m3) by queries rounded to 2^-18 of the row's
+    largest, which both moves the weights, in numerator and sum."""
+    H, Hk, have = 8, 2, 2500
+    g = gen(D + T)
+    table, n_pages = table_for([have + T], 3)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    place = torch.zeros(n_pages, 1, PAGE, 1, device=DEV)
+    at = torch.arange(have + T, device=DEV)
+    place[table[0, at // PAGE].long(), 0, at % PAGE, 0] = (at.float() / (have + T) * 6 - 3) * (1 if up else -1)
+    new = place * (1 + 0.1 * torch.randn(n_pages, Hk, PAGE, D, device=DEV, generator=g))
+    if kind == "e4m3":
+        values, exps = R.quantise_rows(new)
+        k.view(torch.uint8).copy_(values.view(torch.uint8))
+        ke.copy_(exps)
+    else:
+        k.copy_(new.bfloat16())
+    q = (1 + 0.1 * torch.randn(1, T, H * D, device=DEV, generator=g)).bfloat16()
+    got = R.paged_attention_tree(q, H, Hk, D, torch.tensor([have], dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, [have], [T], None, table, k, v, ke, ve, D ** -0.5)
+    terms = float(q.abs().max()) * float(new.abs().max()) * 1.0625 * D * D ** -0.5         # magnitudes of a score's terms; an e4m3 key is off by 2^-4 at most
+    score = D * terms * 2 ** -24 + (2 ** -18 * terms if kind == "e4m3" else 0)
+    bound = 2 ** -8 * want.abs() + (2 ** -8 if kind == "bf16" else 2 ** -11) * mag + (2 ** -11 + 2 * score) * mag + 1e-30
+    assert torch.isfinite(got).all()
+    assert float(((got.double() - want).abs() / bound).max()) <= 1.0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hk,T", [(8, 2, 5), (8, 2, 8), (3, 1, 7), (4, 1, 6)])
+@pytest.mark.parametrize("lens", [[540], [0], [63, 64], [1, 130]])
+def test_page_tables_with_room_for_little(kind, D, H, Hk, T, lens):
+    """Few pages in all: 17 to 32 rows over bf16 pages are tiles of 16."""
+    g = gen(T + len(lens))
+    nodes = [T, T - 2][:len(lens)]
+    table, n_pages = table_for([n + T for n in lens], 3)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    mask = random_masks(T, len(lens), T)
+    q = torch.randn(len(lens), T, H * D, device=DEV, generator=g).bfloat16()
+    got = R.paged_attention_tree(q, H, Hk, D, torch.tensor(lens, dtype=torch.int32, device=DEV), table, k, v, mask=mask.to(DEV), nodes=torch.tensor(nodes, dtype=torch.int32, device=DEV), k_exp=ke,
+                                 v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, lens, nodes, mask, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
+    for b, n in enumerate(nodes):
+        assert not got[b, n:].any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("T", [4, 8, 16, 40])
 @pytest.mark.parametrize("have", [30, 3000])
 @pytest.mark.parametrize("value", [math.nan, math.inf, 2.0 ** 40])
