@@ -22,7 +22,8 @@
 //
 // What bounds it.  Shared memory takes 128 bytes a cycle, and a product of few columns costs what its 4 KB of keys or values take (measured 42 cycles alone).  bf16: pages 64 KB written and
 // 64 KB read, weights and queries 24 KB: 1250 cycles a block of 128 elements, of the 2100 that the SM's share of the memory takes.  e4m3: 32 + 32 KB, and 32 KB for the parts,
-// 750 cycles of 1050.  (Values converted to fp16, the fp16 product and the two parts of queries one after the other took 1400 and more.)
+// 750 cycles of 1050.  Measured are 1300 with 16 rows (the chain of waits of the warp that issues the products), 1500 with 32 and 2400 with 64 (the softmax's): 32 requests of 8192 tokens,
+// 4 rows, 85 us, 74 % of the copy rate.  Values converted to fp16, the fp16 product and the two parts of queries one after the other took 148.
 #include "paged_tree_sm100.cuh"
 
 int ptb_make_tmap_64b(CUtensorMap* map, const void* base, long long rows, int box_rows);
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    constexpr uint32_t TM_S = 0, TM_O = S::TM_O;         // two buffers of scores, two accumulators (SPLIT: one)
+    constexpr uint32_t TM_S = 0, TM_O = S::TM_O;         // two buffers of scores, two accumulators (64 rows: one)
     pdl_wait();
     pdl_launch_dependents();
     plan<THREADS>(P, starts, part);
