@@ -5,7 +5,7 @@
 //   without draft probabilities (tokens proposed outright, several to a parent):  child c is accepted iff u_c (1 - R) < p_s(x_c), R the mass of the children rejected before it;
 //   with them (a chain; q_s is what the child was drawn from):                   iff u_c q_s(x_c) < p_s(x_c).
 // It goes on at the accepted child.  Where none is left, the last token is drawn with u_0 by the inverse of the cumulative distribution: of p_s without the rejected tokens, or of
-// max(p_s - q_s, 0) where a child was rejected; both leave the target's distribution as it is.  Temperature 0 or below takes the arg-max (the lowest of equals) throughout.
+// max(p_s - q_s, 0) where a child was rejected; both leave the target's distribution as it is.  Temperature 0 or below (or no number) takes the arg-max (the lowest of equals) throughout.
 //
 // Two launches.  verify_stats_kernel reads every logit once: a chunk's maximum, its place, and the sum of exponentials; the bytes of the logits bound it.
 // verify_walk_kernel, a cluster per request, joins the chunks, walks, and draws from one row.  A draw has to fall on the same token for everybody, so that row's weights and
@@ -50,6 +50,12 @@ __device__ __forceinline__ float logit_at(const VerifyParams& P, int b, int i, i
 }
 __device__ __forceinline__ int nodes_of(const VerifyParams& P, int b) { return P.nodes ? max(0, min(P.nodes[b], P.T)) : P.T; }
 
+// Hotter ones count as 2^126, the last whose reciprocal is a normal number in fp32: what a difference of logits is multiplied by stays above zero, and one of -infinity weighs nothing.
+__device__ __forceinline__ float temperature_of(const VerifyParams& P, int b) {
+    const float t = P.temperature[b];
+    return t > 0x1p126f ? 0x1p126f : t;                        // no number stays none
+}
+
 // One chunk of one row: maximum, its first place, sum of exp((l - maximum) / temperature).  VEC: rows start on 16 bytes.  Bound by the logits' bytes as long as an element
 // costs few instructions: the place is looked for only in the warps that hold the chunk's maximum.
 template <bool BF16, bool VEC>
@@ -61,7 +67,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(const __grid_c
     const int row = blockIdx.y, b = row / P.T, i = row - b * P.T, chunk = blockIdx.x, tid = threadIdx.x;
     if (i >= nodes_of(P, b)) return;
     if (tid == 0) place = 0x7fffffff;
-    const float t = P.temperature[b], scale = (t > 0.f ? __frcp_rn(t) : 1.f) * 1.4426950408889634f;
+    const float t = temperature_of(P, b), scale = (t > 0.f ? __frcp_rn(t) : 1.f) * 1.4426950408889634f;
     const size_t base = (size_t)b * P.l_batch + (size_t)i * P.l_row;
     const int v0 = chunk * VF_CHUNK;
     constexpr int W = !VEC ? 1 : BF16 ? 8 : 4;                 // neighbours that a thread has at once: element k stands at v0 + ((k / W) * VF_THREADS + tid) * W + k % W
@@ -161,7 +167,7 @@ __global__ void __launch_bounds__(W, 1024 / W) verify_walk_kernel(const __grid_c
         }
         return;
     }
-    const float t = P.temperature[b];
+    const float t = temperature_of(P, b);
     const bool greedy = !(t > 0.f);
     const double inv = greedy ? 1.0 : 1.0 / (double)t;
     if (tid < n) {

@@ -17,6 +17,7 @@ from .. import _native as N
 from .paged_tree import _index, _launch
 
 MAX_NODES = 64
+MAX_TEMPERATURE = 2.0 ** 126
 
 
 @N.register_decls
@@ -43,7 +44,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, t
                   nodes: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``logits [B, T, V]`` (fp32 or bf16): what the target says behind each of a request's T nodes; node 0 is the latest token, the others are drafted.  ``tokens [B, T]`` (int32):
     their ids; ``parents [B, T]`` (int32): a node before the node, -1 for the first (None: a chain); ``nodes [B]`` (int32): how many are there (None: all).  ``u [B, T]`` (fp32 in
-    [0, 1)): node i's number decides on it, the first one's draws the last token.  ``temperature [B]`` (fp32): 0 or below takes the arg-max, of equals the lowest id.
+    [0, 1)): node i's number decides on it, the first one's draws the last token.  ``temperature [B]`` (fp32): 0 or below takes the arg-max, of equals the lowest id; above 2^126
+    (infinity too) counts as 2^126, a uniform row for logits of any ordinary size.
     ``draft_probs [B, T, V]`` (fp32, chains only): row i is what the node behind node i was drawn from.
 
     Returns ``(path, count, out)``, int32: ``path [B, T]`` the accepted nodes, the first one among them, -1 behind; ``count [B]`` how many drafted tokens were accepted (-1 for a
@@ -98,7 +100,7 @@ def verify_drafts_reference(logits, tokens, u, temperature, parents=None, nodes=
         n = T if nodes is None else max(0, min(int(nodes[b]), T))
         if n == 0:
             continue
-        temp = float(temperature[b])
+        temp = min(float(temperature[b]), MAX_TEMPERATURE)
         up = [-1] + [(i - 1 if parents is None else int(parents[b, i])) for i in range(1, n)]
         tok = tokens[b].tolist()
 

@@ -87,3 +87,12 @@ def test_native_entry_refuses():
         return rc == -1 and L.ptb_last_error().decode() or ""
     assert "nodes" in call(T=65) and "nodes" in call(T=0) and "tokens" in call(V=1 << 20) and "in all" in call(B=20000, T=8)
     assert "chains" in call(probs=BASE, parents=BASE) and "aligned" in call(work=BASE + 8)
+
+
+def test_an_infinite_temperature():
+    """Every token that has a probability has the same; of infinite logits only they have one."""
+    V, inf = 6, math.inf
+    logits = torch.tensor([[0.0, -inf, 3.0, 1.0, -inf, -2.0], [inf, 1.0, -inf, inf, 0.0, 0.0]])[:, None]
+    for u, want in ((0.0, [0, 0]), (0.26, [2, 0]), (0.51, [3, 3]), (0.99, [5, 3])):
+        out = verify_drafts(logits, torch.zeros(2, 1, dtype=torch.int32), torch.full((2, 1), u), torch.full((2,), inf))[2]
+        assert out.flatten().tolist() == want

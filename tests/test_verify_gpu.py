@@ -147,3 +147,26 @@ def test_streams_graphs_and_repeats():
     want = call()
     for o in outs:
         assert all(torch.equal(a, b) for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [math.inf, 3e38, 1e38, 2e30, 0.9e30, 1e4, 1e-3, 1.2e-38, math.nan])
+def test_temperatures_of_any_size(dtype, t):
+    """A row is as good as uniform, or as good as its arg-max; masked logits (-inf, the type's lowest value) and the end of the last chunk behind the vocabulary are what they are at any other."""
+    g = torch.Generator().manual_seed(6)
+    B, T, V = 6, 8, 9001
+    logits = peaked(g, B, T, V)
+    logits[1, :, ::3] = -math.inf
+    logits[2, :, 5:] = -math.inf
+    logits[3, :, 1::2] = torch.finfo(dtype).min
+    logits[4, :, ::2] = 3e38
+    logits[5, 0, 7] = math.inf
+    parents = torch.tensor([[-1, 0, 0, 0, 1, 1, 2, 4]] * B, dtype=torch.int32)
+    logits, tokens = logits.to(dtype), torch.randint(0, V, (B, T), generator=g).int()
+    tokens[2] %= 5
+    tokens[:, 1] = logits[:, 0].float().argmax(-1).int()
+    for seed in range(3):
+        u = torch.rand(B, T, generator=torch.Generator().manual_seed(seed))
+        u[:, 1:] *= (1.0, 1.0, 1e-4)[seed]                # small numbers accept tokens of a uniform row
+        check(logits, tokens, u, torch.full((B,), t), parents=parents)
+        check(logits, tokens, u, torch.full((B,), t))
