@@ -498,19 +498,21 @@ int sm_count() {
 //   up to 32 rows, bf16, and two pages a CTA at most: mma.sync, in one or two tiles.  One request of 540 tokens, 20 rows of 128: 14.9 us, tokens along the lanes 20.
 //   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 87 and 90 us, in tiles of 128 rows 104 and 108; e4m3, 64 rows over 4100
 //   tokens: 73 and 117.  e4m3, 4 rows over 8192 tokens, 32 requests: 85, where mma.sync, for which every warp converts what it reads, took 148.
-//   more: tiles of 128 rows.
+//   more, bf16: tiles of 128 rows.
+//   more, e4m3: tokens along the lanes, in tiles of 64 rows (see paged_tree_sm100.cu).
 struct Choice { int tile_rows, unit, parts; };
 Choice choose(int rows, bool q8, long long pages) {
     if (!q8 && (rows <= ROWS || (rows <= 2 * ROWS && pages * ((rows + ROWS - 1) / ROWS) <= 2 * sm_count()))) return {ROWS, PAGE, 1};
-    if (rows > 64) return {128, 128, 2};
+    if (rows > 64) return q8 ? Choice{64, 128, 1} : Choice{128, 128, 2};
     if (rows <= 16) return {16, 128, 2};
     return {rows <= 32 ? 32 : 64, 128, rows <= 32 ? 2 : 1};
 }
 template <int D, bool Q8>
 int launch(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
-    if (p.tile_rows == 128) return launch_tiles<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, EIGHTS>(p, st);
-    if constexpr (!Q8)
+    if constexpr (!Q8) {
+        if (p.tile_rows == 128) return launch_tiles<D>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, EIGHTS>(p, st);
         if (p.unit == PAGE) return launch_pieces<D>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, TILES>(p, st);
+    }
     return launch_few<D, Q8>(p, k_pages, v_pages, st) ? -1 : launch_merge<D, ROWWISE>(p, st);
 }
 

@@ -129,10 +129,6 @@ __device__ __forceinline__ Item item_at(const Params& P, int* starts, int u, int
     return it;
 }
 
-// Weights are 2^(s - m + up): fp16, whose smallest step is 2^-24, holds what a long context's many small weights add up to.  m is the reference, a maximum that
-// was passed by less than 2^8; the largest weight is 2^15.
-template <bool Q8> __device__ __forceinline__ constexpr float weight_up() { return Q8 ? 7.f : 0.f; }
-
 // Two e4m3 values (the low 16 bits) as fp16, exactly.
 __device__ __forceinline__ uint32_t e4m3x2(uint32_t two) {
     uint32_t h;
@@ -153,7 +149,7 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return r;
 }
 
-template <int D, bool Q8> int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);      // paged_tree_sm100.cu
+template <int D> int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);               // paged_tree_sm100.cu: bf16
 template <int D, bool Q8> int launch_few(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);        // paged_tree_few_sm100.cu
 
 }  // namespace tree

@@ -1,5 +1,4 @@
-// Up to 64 rows of drafted tokens (nodes times the heads of a group) against a paged cache, on the 5th-generation tensor cores with the tokens along the lanes; see
-// paged_tree.cuh.
+// Drafted tokens against a paged cache on the 5th-generation tensor cores with the tokens along the lanes, up to 64 rows (nodes times the heads of a group) at a time; see paged_tree.cuh.
 //
 // The scores of a block of 128 tokens are S^T = K Q^T: a lane of tensor memory is a token, a column a row of queries.  Of a handful of rows that leaves each of a group's
 // 128 softmax threads as many scores as there are rows, where rows along the lanes would leave 128 to each of a few; and a product costs by its columns.  The second product is
@@ -128,6 +127,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
     constexpr int NK = S::NK, NV = S::NV;
     constexpr bool SPLIT = N == 64;                      // the groups part the rows, not the blocks
     constexpr int R = SPLIT ? 32 : N;                    // rows of a softmax thread
+    auto tile_row = [](const Item& it) { return N == 64 ? it.tile * N : 0; };        // an item's first row: of fewer than 64 there is one tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sq = smem, *sk = smem + S::OFF_K, *sv = smem + S::OFF_V, *sp = smem + S::OFF_P, *se = smem + S::OFF_E;
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
             const bool whole = it.n == it.r.units, shared = !SPLIT && whole && it.n > 1;
             float* wk = P.work + partial_at(P, blockIdx.x, u == u0 ? 0 : 1, SPLIT ? 0 : g, D);
             const float* theirs = wk + (g ? -1 : 1) * (long long)partial_floats(N, D);
-            const int rows = max(0, min(N, it.r.nodes * P.G) - r0);          // of this group's R
+            const int rows = max(0, min(N, it.r.nodes * P.G - tile_row(it)) - r0);        // of this group's R
             wk += (size_t)r0 * D;
             float2* ml = reinterpret_cast<float2*>(wk - (size_t)r0 * D + (size_t)N * D) + r0;
             {
@@ -544,7 +544,8 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                 }
                 group_sync(g);
                 if (some && (D == 128 || wg < 2)) {
-                    int node = r0 / P.G, head = r0 - node * P.G;
+                    const int at = tile_row(it) + r0;
+                    int node = at / P.G, head = at - node * P.G;
                     __nv_bfloat16* out = P.out + (((size_t)it.b * P.T + node) * P.H + it.kvh * P.G) * D + tid;           // head 0 of the node
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
@@ -573,18 +574,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
         constexpr int EACH = N * D / 8 / 128;            // 16-byte pieces of queries a thread
         uint4 raw[EACH];
         unsigned long long seen = 0, there = 0;
-        const uint32_t per_head = 65536 / P.G + 1;       // row / G = row * per_head >> 16 for rows up to 64
+        const uint32_t per_head = 65536 / P.G + 1;
         auto fetch = [&](const Item& it) {
-            const int rows = it.r.nodes * P.G;
+            const int rows = it.r.nodes * P.G - tile_row(it), node0 = tile_row(it) / P.G, head0 = tile_row(it) - node0 * P.G;
+            auto node_of = [&](int r) {                  // (head0 + r) / G: below 128 a product and a shift where G is below 64, else 0 or 1
+                return node0 + (P.G < 64 ? (int)((head0 + r) * per_head >> 16) : head0 + r >= P.G ? 1 : 0);
+            };
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const int x = i * 128 + tid, r = x / (D / 8), c = x % (D / 8), node = (int)(r * per_head >> 16), head = r - node * P.G;
+                const int x = i * 128 + tid, r = x / (D / 8), c = x % (D / 8), node = node_of(r), head = tile_row(it) + r - node * P.G;
                 raw[i] = make_uint4(0, 0, 0, 0);
                 if (r < rows) raw[i] = *reinterpret_cast<const uint4*>(P.q + (size_t)it.b * P.q_batch + (size_t)node * P.q_row + (size_t)(it.kvh * P.G + head) * D + c * 8);
             }
             seen = there = 0;
             if (tid < min(N, rows)) {                    // joined later: nothing waits for a load here
-                const int node = (int)(tid * per_head >> 16);
+                const int node = node_of(tid);
                 seen = P.mask ? P.mask[(size_t)it.b * P.T + node] : (2ull << node) - 1;
                 there = it.r.nodes < 64 ? (1ull << it.r.nodes) - 1 : ~0ull;
             }

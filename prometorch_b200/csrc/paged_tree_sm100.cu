@@ -1,20 +1,19 @@
-// More than sixteen rows of drafted tokens against a paged cache, both products on the 5th-generation tensor cores; see paged_tree.cuh.
+// More than 64 rows of drafted tokens against a cache in bf16, both products on the 5th-generation tensor cores; see paged_tree.cuh.
 //
-// One CTA per SM walks its run of units, blocks of 128 tokens (two pages).  Rows lie along the 128 lanes of tensor memory.  Sixteen warps, or (e4m3) twenty:
-//   warp 0      brings pages: bf16 keys and values straight to the tiles the products read; e4m3 ones, and their exponents, to a ring of raw pages;
+// One CTA per SM walks its run of units, blocks of 128 tokens (two pages).  Rows lie along the 128 lanes of tensor memory.  Sixteen warps:
+//   warp 0      brings keys and values straight to the tiles the products read;
 //   warp 1      owns tensor memory and issues S(j) = Q K_j^T and O += P(j) V_j;
 //   warps 4-11  softmax, two groups of four warps that take every other block, each with a score buffer, a running maximum and sum and an output accumulator of its
 //               own: while one group works on its scores the tensor cores work for the other.  A thread owns a row, so nothing is exchanged.  Weights go back to
 //               tensor memory, over the scores they came from, as the first operand of the second product.  The accumulator is scaled, by its own threads, only
 //               when a row's maximum has grown by 2^8;
-//   warps 12-19 e4m3: raw pages to fp16 tiles, four warps the keys and four the values.  12-15, bf16: of a block with drafted tokens they clear the values that must not meet a weight.
+//   warps 12-15 of a block with drafted tokens they clear the values that must not meet a weight.
 //
-// e4m3 values times a power of two are exact in fp16, which has five more exponents than they need: a block's keys are brought to the largest exponent among them (which
-// then scales the block's scores), the values to a reference that only grows and that the accumulator follows.  A key or a value more than 2^30 below those loses bits that
-// the scores and the sums do not hold either.
-//
-// What bounds it: the cache's bytes up to 128 rows (a block of 128 keys of 128 elements is 64 KB in bf16 and takes an SM's share of the memory 1.5 us; exponentials, products and
+// What bounds it: the cache's bytes up to 128 rows (a block of 128 keys of 128 elements is 64 KB and takes an SM's share of the memory 1.5 us; exponentials, products and
 // softmax instructions take about 0.6 us each, side by side); with more tiles of rows, which fetch the pages again, the products and exponentials.
+//
+// e4m3 pages do not come here.  As fp16 tiles, their tokens brought to a common exponent, they were faster with many rows (512 rows of 64 over 8191 tokens: 106 us, with the tokens
+// along the lanes 145; 80 over 700: 31 and 27), but one token 2^30 times the others took the others' bits with it, for rows that do not see it as well.
 //
 // A drafted token that a row does not see must not reach it, whatever it holds: its weight is zero, and zero times a value that is no number is none.  So such values are
 // cleared in the tile and the rows that do see the token take them at the end.  What lies behind a request's last token is cleared as well.
@@ -25,40 +24,33 @@ namespace tree {
 namespace {
 
 constexpr int BQ = LANES;
-// Threads, and registers a thread of the softmax and of the other warps: the launch's shared out anew (512 x 128 = 256 x 184 + 256 x 72; 640 x 96 = 256 x 120 + 384 x 80).  A softmax
-// thread holds its 128 scores (64 of them): one wait for tensor memory a block, or three, in place of eight; 4900 clocks from the scores to the weights became 2000.
-template <bool Q8> struct Split { static constexpr int THREADS = Q8 ? 640 : 512, SOFTMAX = Q8 ? 120 : 184, OTHER = Q8 ? 80 : 72; };
-template <int D, bool Q8>
+// Registers a thread of the softmax and of the other warps: the launch's shared out anew (512 x 128 = 256 x 184 + 256 x 72).  A softmax thread holds its 128 scores: one wait for tensor
+// memory a block in place of eight; 4900 clocks from the scores to the weights became 2000.
+constexpr int THREADS = 512, REGS_SOFTMAX = 184, REGS_OTHER = 72;
+template <int D>
 struct Sm {
-    static constexpr int Q_BYTES = BQ * D * 2, TILE = BLOCK * D * 2, RAW = BLOCK * D;
-    static constexpr int NK = Q8 ? 1 : D == 128 ? 2 : 3, NV = Q8 ? 2 : D == 128 ? 3 : 4, NR = Q8 ? (D == 128 ? 2 : 4) : 0;
-    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NK * TILE, OFF_R = OFF_V + NV * TILE, OFF_E = OFF_R + NR * 2 * RAW;
-    static constexpr int OFF_BAR = OFF_E + NR * 2 * BLOCK, OFF_PLAN = OFF_BAR + 1024;
+    static constexpr int Q_BYTES = BQ * D * 2, TILE = BLOCK * D * 2;
+    static constexpr int NK = D == 128 ? 2 : 3, NV = D == 128 ? 3 : 4;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE, OFF_PLAN = OFF_BAR + 1024;
     static constexpr int TOTAL = OFF_PLAN + 1024;                      // and the plan
     static_assert(TOTAL + plan_bytes(MAX_B) <= 227 * 1024, "shared memory of a CTA");
 };
 
-constexpr int V_ROOM = 3;                // fp16 values stand for value * 2^(reference - V_ROOM): the reference may be passed by 2^4 before it has to grow
-constexpr int K_ROOM = 7;                // 448 * 2^7 fits fp16
-
-template <int D, bool Q8>
-__global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params P) {
-    using S = Sm<D, Q8>;
-    constexpr int NK = S::NK, NV = S::NV, NR = Q8 ? S::NR : 1;
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params P) {
+    using S = Sm<D>;
+    constexpr int NK = S::NK, NV = S::NV;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *sq = smem, *sk = smem + S::OFF_K, *sv = smem + S::OFF_V, *sr = smem + S::OFF_R, *se = smem + S::OFF_E;
+    uint8_t *sq = smem, *sk = smem + S::OFF_K, *sv = smem + S::OFF_V;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
     uint64_t *q_full = bars, *q_free = bars + 1, *s_full = bars + 2, *p_ready = bars + 4, *o_full = bars + 6;            // [1], [1], [2], [2], [2]
     uint64_t *k_full = bars + 8, *k_empty = bars + 12, *v_full = bars + 16, *v_empty = bars + 20, *v_ready = bars + 24;  // [NK], [NK], [NV], [NV], [NV]
-    uint64_t *raw_full = bars + 28, *raw_empty = bars + 32;                                                              // [NR], [NR]
-    unsigned long long* taint = reinterpret_cast<unsigned long long*>(bars + 36);          // [8] by item: drafted tokens whose values were cleared
-    int* bad_pages = reinterpret_cast<int*>(bars + 44);                // [8] by block: bits of pages that are none of the pool's
-    int* k_ref = bad_pages + 8;                                        // [8] by block: biased exponent that its keys were brought to
-    int* v_ref = k_ref + 8;                                            // [8] by block: that of its values' reference
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ref + 8);
-    int* part = reinterpret_cast<int*>(tmem_slot + 1);                 // [20]
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(part + 20);
+    unsigned long long* taint = reinterpret_cast<unsigned long long*>(bars + 28);          // [8] by item: drafted tokens whose values were cleared
+    int* bad_pages = reinterpret_cast<int*>(bars + 36);                // [8] by block: bits of pages that are none of the pool's
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bad_pages + 8);
+    int* part = reinterpret_cast<int*>(tmem_slot + 1);                 // [16]
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(part + 16);
     int* starts = reinterpret_cast<int*>(smem + S::OFF_PLAN);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -66,9 +58,8 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
         mbar_init(q_full, 4);
         mbar_init(q_free, 1);
         for (int g = 0; g < 2; ++g) { mbar_init(&s_full[g], 1); mbar_init(&p_ready[g], 4); mbar_init(&o_full[g], 1); }
-        for (int s = 0; s < NK; ++s) { mbar_init(&k_full[s], Q8 ? 4 : 1); mbar_init(&k_empty[s], 1); }
+        for (int s = 0; s < NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
         for (int s = 0; s < NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); mbar_init(&v_ready[s], 4); }
-        for (int s = 0; s < NR; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 8); }
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tmK);
@@ -83,20 +74,19 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     constexpr uint32_t TM_S = 0, TM_O = 256;             // two buffers of 128 columns, two of D
-    constexpr uint32_t TM_P = Q8 ? 64 : 0;               // weights lie in the half of the scores that is in registers when they are written
     pdl_wait();
     pdl_launch_dependents();
-    plan<Split<Q8>::THREADS>(P, starts, part);
+    plan<THREADS>(P, starts, part);
     __syncthreads();
     const int all = starts[P.B], per = units_per_cta(all, P.ctas);
     const int u0 = (int)min((long long)all, (long long)blockIdx.x * per), u1 = min(all, u0 + per);
     if (blockIdx.x == 0)
-        for (int b = threadIdx.x; b <= P.B; b += Split<Q8>::THREADS) P.starts[b] = starts[b];
+        for (int b = threadIdx.x; b <= P.B; b += THREADS) P.starts[b] = starts[b];
     bool ok = true;
     auto wait = [&](uint64_t* bar, int turn) { return ok && (mbar_try_wait(bar, (uint32_t)(turn & 1)) || (!*abort_flag && mbar_wait(bar, (uint32_t)(turn & 1), P.status))); };
 
     if (warp < SOFTMAX_WARP) {
-        regs_dec<Split<Q8>::OTHER>();                          // one instruction for the warp group
+        regs_dec<REGS_OTHER>();                          // one instruction for the warp group
         if (warp == 0) {
             // ------------------------------------------------------------------------------------ pages
             int n = 0;                                       // block of the run
@@ -117,37 +107,21 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                     const int page[2] = {__shfl_sync(0xffffffffu, id, 0), __shfl_sync(0xffffffffu, id, 1)};
                     if (lane == 0) {
                         const int there = page[1] == -2 ? 1 : 2;
-                        if constexpr (Q8) {
-                            const int s = n % NR;
-                            if (n >= NR) ok = wait(&raw_empty[s], n / NR - 1);
-                            if (ok) {
-                                bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
-                                mbar_expect_tx(&raw_full[s], there * (S::RAW + 2 * PAGE));
-                                for (int x = 0; x < there; ++x) {
-                                    const int head = max(page[x], 0) * P.Hk + it.kvh;        // a page that is none of the pool's: any other in its place, which no row sees
-                                    tma_load_2d(sr + s * 2 * S::RAW + x * S::RAW / 2, &tmK, 0, head * (S::RAW / 256), &raw_full[s]);
-                                    tma_load_2d(sr + s * 2 * S::RAW + S::RAW + x * S::RAW / 2, &tmV, 0, head * (S::RAW / 256), &raw_full[s]);
-                                    bulk_g2s(se + s * 2 * BLOCK + x * PAGE, P.k_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
-                                    bulk_g2s(se + s * 2 * BLOCK + BLOCK + x * PAGE, P.v_exp + (size_t)head * PAGE, PAGE, &raw_full[s]);
-                                }
-                            }
-                        } else {
-                            const int sK = n % NK, sV = n % NV;
-                            if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
-                            if (ok) {
-                                bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
-                                mbar_expect_tx(&k_full[sK], there * (S::TILE / 2));
-                                for (int x = 0; x < there; ++x)
-                                    for (int c = 0; c < D / 64; ++c)
-                                        tma_load_2d(sk + sK * S::TILE + c * (BLOCK * 128) + x * 8192, &tmK, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &k_full[sK]);
-                                if (n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
-                            }
-                            if (ok) {
-                                mbar_expect_tx(&v_full[sV], there * (S::TILE / 2));
-                                for (int x = 0; x < there; ++x)
-                                    for (int c = 0; c < D / 64; ++c)
-                                        tma_load_2d(sv + sV * S::TILE + (x * (D / 64) + c) * 8192, &tmV, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &v_full[sV]);
-                            }
+                        const int sK = n % NK, sV = n % NV;
+                        if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
+                        if (ok) {
+                            bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
+                            mbar_expect_tx(&k_full[sK], there * (S::TILE / 2));
+                            for (int x = 0; x < there; ++x)
+                                for (int c = 0; c < D / 64; ++c)
+                                    tma_load_2d(sk + sK * S::TILE + c * (BLOCK * 128) + x * 8192, &tmK, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &k_full[sK]);
+                            if (n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
+                        }
+                        if (ok) {
+                            mbar_expect_tx(&v_full[sV], there * (S::TILE / 2));
+                            for (int x = 0; x < there; ++x)
+                                for (int c = 0; c < D / 64; ++c)
+                                    tma_load_2d(sv + sV * S::TILE + (x * (D / 64) + c) * 8192, &tmV, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &v_full[sV]);
                         }
                     }
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0);
@@ -158,7 +132,7 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
         } else if (warp == 1) {
             // ------------------------------------------------------------------------------------ products
             if (lane == 0) {
-                constexpr uint32_t id_s = idesc<Q8>(BLOCK, 0, 0), id_o = idesc<Q8>(D, 0, 1);
+                constexpr uint32_t id_s = idesc<false>(BLOCK, 0, 0), id_o = idesc<false>(D, 0, 1);
                 int base = 0, item = 0, p_turn[2] = {0, 0};  // base: block of the run that the item begins with
                 for (int u = u0; u < u1 && ok; ++item) {
                     const Item it = item_at(P, starts, u, u1);
@@ -188,7 +162,7 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t b0 = smem_desc(smem_u32(sv + s * S::TILE), 8192, 1024);
-                        const uint32_t d = tmem + TM_O + (uint32_t)(g * D), p = tmem + TM_S + (uint32_t)(g * BLOCK) + TM_P;
+                        const uint32_t d = tmem + TM_O + (uint32_t)(g * D), p = tmem + TM_S + (uint32_t)(g * BLOCK);
 #pragma unroll
                         for (int x = 0; x < 2; ++x)
                             if (x == 0 || t0 + PAGE < total)               // the second page is there
@@ -206,12 +180,12 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
         }
     } else if (warp < CONVERT_WARP) {
         // ------------------------------------------------------------------------------------ softmax
-        regs_inc<Split<Q8>::SOFTMAX>();
+        regs_inc<REGS_SOFTMAX>();
         const int g = (warp - SOFTMAX_WARP) >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + TM_S + (uint32_t)(g * BLOCK), to = lanes + TM_O + (uint32_t)(g * D);
         int base = 0, s_turn = 0, o_turn = 0;
         // what a thread knows of its row in an item
-        struct Row { Item it; bool live, on; unsigned long long seen; float fac; };
+        struct Row { Item it; bool live, on; unsigned long long seen; };
         auto enter = [&](int u, int item) {
             Row w;
             w.it = item_at(P, starts, u, u1);
@@ -221,41 +195,17 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
             const int node = w.on ? at / P.G : 0, head = w.on ? at - node * P.G : 0;
             w.seen = 0;
             if (w.on) w.seen = (P.mask ? P.mask[(size_t)w.it.b * P.T + node] : (2ull << node) - 1) & (w.it.r.nodes < 64 ? (1ull << w.it.r.nodes) - 1 : ~0ull);
-            w.fac = P.scale_log2;
-            if (Q8 || g == 0) {                          // the row of q: both groups want its scale, the first puts it into the tile
+            if (g == 0) {                                // the first group puts the row of q into the tile
                 const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)w.it.b * P.q_batch + (size_t)node * P.q_row + (size_t)(w.it.kvh * P.G + head) * D);
                 uint4 raw[D / 8];
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) raw[i] = w.on ? q[i] : make_uint4(0, 0, 0, 0);
-                if constexpr (Q8) {                      // to fp16, its largest magnitude in [1, 2)
-                    uint32_t a = 0;
+                if (item > 0) ok = wait(q_free, item - 1);                   // the products of the last item have read theirs
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) a = max(a, max(x[k] & 0x7fffu, (x[k] >> 16) & 0x7fffu));
-                    }
-                    const int k = min(253, max(40, (int)(a >> 7)));          // biased exponent
-                    const float down = __uint_as_float((uint32_t)(254 - k) << 23);
-                    w.fac *= __uint_as_float((uint32_t)k << 23);
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        uint32_t* x = reinterpret_cast<uint32_t*>(&raw[i]);
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[y]));
-                            x[y] = pack2<true>(f.x * down, f.y * down);
-                        }
-                    }
-                }
-                if (g == 0) {
-                    if (item > 0) ok = wait(q_free, item - 1);               // the products of the last item have read theirs
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(sq + (i / 8) * (BQ * 128) + row * 128 + (((i & 7) ^ (row & 7)) * 16)) = raw[i];
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(q_full);
-                }
+                for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(sq + (i / 8) * (BQ * 128) + row * 128 + (((i & 7) ^ (row & 7)) * 16)) = raw[i];
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
             }
             return w;
         };
@@ -266,9 +216,7 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
             const int len = it.r.len;
             const bool live = w.live, on = w.on;
             const unsigned long long seen = w.seen;
-            const float fac = w.fac;
             float m = -INFINITY, l = 0.f;
-            int ref = 0;                                 // of the values that the accumulator holds
             for (int j = g; j < it.n; j += 2) {
                 const int n = base + j, t0 = (it.first + j) * BLOCK;
                 ok = wait(&s_full[g], s_turn++);
@@ -276,36 +224,24 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                 if (live && ok) {
                     const int bad = bad_pages[n & 7];
                     const bool some = t0 + BLOCK > len || bad;               // not every row sees every token
-                    const float f = Q8 ? fmaxf(fac * pow2(k_ref[n & 7] - 127 - K_ROOM), 1e-30f) : fac;      // above zero: it meets -infinity
-                    // HOLD scores at a time in registers: all of a block, or (e4m3) halves, the first fetched a second time
-                    constexpr int HOLD = Q8 ? BLOCK / 2 : BLOCK;
-                    uint32_t r[HOLD];
-                    auto fetch = [&](int from) {
+                    const float f = P.scale_log2;
+                    uint32_t r[BLOCK];                                       // all scores of the block
 #pragma unroll
-                        for (int c = 0; c < HOLD / 32; ++c) tmem_ld32(ts + from + 32 * c, r + 32 * c);
+                    for (int c = 0; c < BLOCK / 32; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
 #pragma unroll
-                        for (int c = 0; c < HOLD / 32; ++c) tmem_ld_done(r + 32 * c);
-                        if (some) {
+                    for (int c = 0; c < BLOCK / 32; ++c) tmem_ld_done(r + 32 * c);
+                    if (some) {
 #pragma unroll
-                            for (int c = 0; c < HOLD / 32; ++c) {
-                                const uint32_t vis = (bad >> ((from + 32 * c) / PAGE)) & 1 ? 0u : visible32(seen, t0 + from + 32 * c - len);
+                        for (int c = 0; c < BLOCK / 32; ++c) {
+                            const uint32_t vis = (bad >> (32 * c / PAGE)) & 1 ? 0u : visible32(seen, t0 + 32 * c - len);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (!((vis >> i) & 1)) r[32 * c + i] = 0xff800000u;      // -infinity
-                            }
+                            for (int i = 0; i < 32; ++i)
+                                if (!((vis >> i) & 1)) r[32 * c + i] = 0xff800000u;          // -infinity
                         }
-                    };
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto top = [&] {
-#pragma unroll
-                        for (int i = 0; i < HOLD; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                    };
-                    fetch(0);
-                    top();
-                    if constexpr (Q8) {
-                        fetch(HOLD);
-                        top();
                     }
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < BLOCK; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
                     const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
                     float alpha = 1.f;
                     if (mx > m + 8.f) {
@@ -313,34 +249,23 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                         m = mx;
                         l *= alpha;
                     }
-                    if constexpr (Q8) {
-                        const int to_ref = v_ref[n & 7];
-                        alpha *= pow2(j > 1 ? ref - to_ref : 0);
-                        ref = to_ref;
-                    }
-                    const float mu = m == -INFINITY ? 0.f : m - weight_up<Q8>();
+                    const float mu = m == -INFINITY ? 0.f : m;
                     const uint64_t f2 = both(f), mu2 = both(-mu);
                     uint64_t l2[2] = {0, 0};
-                    auto weigh = [&](int from) {                             // the packed weights take the place of the scores, in registers and in tensor memory
+                    // the packed weights take the place of the scores, in registers and in tensor memory
 #pragma unroll
-                        for (int c = 0; c < HOLD / 32; ++c) {
+                    for (int c = 0; c < BLOCK / 32; ++c) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                float x, y;
-                                apart(fma2(pair(r[32 * c + 2 * i], r[32 * c + 2 * i + 1]), f2, mu2), x, y);
-                                x = exp2f(x);
-                                y = exp2f(y);
-                                l2[i & 1] = add2(l2[i & 1], pair(__float_as_uint(x), __float_as_uint(y)));
-                                r[16 * c + i] = pack2<Q8>(x, y);
-                            }
-                            tmem_st16(ts + TM_P + from / 2 + 16 * c, r + 16 * c);
+                        for (int i = 0; i < 16; ++i) {
+                            float x, y;
+                            apart(fma2(pair(r[32 * c + 2 * i], r[32 * c + 2 * i + 1]), f2, mu2), x, y);
+                            x = exp2f(x);
+                            y = exp2f(y);
+                            l2[i & 1] = add2(l2[i & 1], pair(__float_as_uint(x), __float_as_uint(y)));
+                            r[16 * c + i] = pack2<false>(x, y);
                         }
-                    };
-                    if constexpr (Q8) {
-                        weigh(HOLD);
-                        fetch(0);
+                        tmem_st16(ts + 16 * c, r + 16 * c);
                     }
-                    weigh(0);
                     float lx[4];
                     apart(l2[0], lx[0], lx[1]);
                     apart(l2[1], lx[2], lx[3]);
@@ -369,15 +294,10 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
             if (it.n > g) ok = wait(&o_full[g], o_turn++);
             tc_fence_after();
             const unsigned long long meets = taint[item & 7] & seen;
-            const float down = Q8 ? pow2(ref - 127 - V_ROOM) : 1.f;
             uint32_t r[32];
             auto columns = [&](int c) {                  // 32 of the accumulator's, from 32 c on
                 tmem_ld32(to + 32 * c, r);
                 tmem_ld_done(r);
-                if constexpr (Q8) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * down);
-                }
                 for (unsigned long long left = meets; left; left &= left - 1) {      // values that were cleared, of a token that this row sees
                     const int t = len + __ffsll((long long)left) - 1;
                     if (t / BLOCK < it.first || t / BLOCK >= it.first + it.n || ((t / BLOCK - it.first) & 1) != g) continue;
@@ -386,12 +306,8 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
                     const size_t v = (((size_t)page * P.Hk + it.kvh) * PAGE + t % PAGE) * D + 32 * c;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        if constexpr (Q8) {
-                            if ((P.v_raw[v + i] & 0x7f) == 0x7f) r[i] = 0x7fffffffu;
-                        } else {
-                            const uint32_t x = (uint32_t)reinterpret_cast<const uint16_t*>(P.v_raw)[v + i] << 16;
-                            if ((x & 0x7f800000u) == 0x7f800000u) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(x));
-                        }
+                        const uint32_t x = (uint32_t)reinterpret_cast<const uint16_t*>(P.v_raw)[v + i] << 16;
+                        if ((x & 0x7f800000u) == 0x7f800000u) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(x));
                     }
                 }
             };
@@ -452,123 +368,39 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
         if (!ok) *abort_flag = 1;
     } else {
         // ------------------------------------------------------------------------------------ tiles
-        regs_dec<Split<Q8>::OTHER>();
-        const int cw = (warp - CONVERT_WARP) & 3, tid = (threadIdx.x - CONVERT_WARP * 32) & 127;
-        const bool values = !Q8 || warp >= CONVERT_WARP + 4;                 // e4m3: keys are the first four warps' matter, values the others'
+        regs_dec<REGS_OTHER>();
+        const int tid = threadIdx.x - CONVERT_WARP * 32;
         int n = 0, item = 0;
         for (int u = u0; u < u1; ++item) {               // after a wait that ran out as well: the four warps meet at every item
             const Item it = item_at(P, starts, u, u1);
             const int len = it.r.len, total = len + it.r.nodes;
-            if (values) {
-                if (tid == 0) taint[item & 7] = 0;       // eight items back: nobody reads it any more
-                convert_sync();
-            }
-            int ref = 0;
+            if (tid == 0) taint[item & 7] = 0;           // eight items back: nobody reads it any more
+            convert_sync();
             for (int j = 0; j < it.n; ++j, ++n) {
-                const int t0 = (it.first + j) * BLOCK, sV = n % NV;
-                if constexpr (!Q8) {
-                    ok = wait(&v_full[sV], n / NV);
-                    const int t = t0 + tid;
-                    if (ok && t0 + BLOCK > len && t >= len) {
-                        uint8_t* v = sv + sV * S::TILE + (tid >> 6) * (D / 64) * 8192 + (tid & 63) * 128;
-                        bool odd = false;
-                        for (int i = 0; i < D / 8; ++i) {
-                            uint4* w = reinterpret_cast<uint4*>(v + (i / 8) * 8192 + (i & 7) * 16);
-                            if (t >= total) { *w = make_uint4(0, 0, 0, 0); continue; }
-                            uint4 x = *w;
-                            uint32_t* y = reinterpret_cast<uint32_t*>(&x);
-                            uint32_t any = 0;
+                const int t0 = (it.first + j) * BLOCK, sV = n % NV, t = t0 + tid;
+                ok = wait(&v_full[sV], n / NV);
+                if (ok && t >= len) {                    // a drafted token, or none
+                    uint8_t* v = sv + sV * S::TILE + (tid >> 6) * (D / 64) * 8192 + (tid & 63) * 128;
+                    bool odd = false;
+                    for (int i = 0; i < D / 8; ++i) {
+                        uint4* w = reinterpret_cast<uint4*>(v + (i / 8) * 8192 + (i & 7) * 16);
+                        if (t >= total) { *w = make_uint4(0, 0, 0, 0); continue; }
+                        uint4 x = *w;
+                        uint32_t* y = reinterpret_cast<uint32_t*>(&x);
+                        uint32_t any = 0;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t no = __vcmpeq2(y[k] & 0x7f807f80u, 0x7f807f80u);
-                                any |= no;
-                                y[k] &= ~no;
-                            }
-                            if (any) { *w = x; odd = true; }
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t no = __vcmpeq2(y[k] & 0x7f807f80u, 0x7f807f80u);
+                            any |= no;
+                            y[k] &= ~no;
                         }
-                        if (odd) atomicOr(&taint[item & 7], 1ull << (t - len));
+                        if (any) { *w = x; odd = true; }
                     }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&v_ready[sV]);
-                } else {
-                    const int sR = n % NR, sK = n % NK;
-                    ok = wait(&raw_full[sR], n / NR);
-                    const uint8_t* exps = se + sR * 2 * BLOCK + (values ? BLOCK : 0);
-                    const uint32_t* words = reinterpret_cast<const uint32_t*>(se + sR * 2 * BLOCK);
-                    uint32_t kw = ok ? words[lane] : 0, vw = ok ? words[BLOCK / 4 + lane] : 0;       // exponents of four tokens
-                    const int past = t0 + 4 * lane - total + 4;              // how many of these four lie behind the last token
-                    if (past > 0) {
-                        const uint32_t keep = past >= 4 ? 0u : 0xffffffffu >> (8 * past);
-                        kw &= keep;
-                        vw &= keep;
-                    }
-                    const int top = (int)byte_max(kw), top_v = (int)byte_max(vw);
-                    // both sides follow the values' reference: the scores of a block, which its keys announce, may be there before its values are
-                    if (j == 0 || top_v > ref + K_ROOM - V_ROOM) ref = top_v;
-                    // A warp takes 32 tokens, eight of them and 64 of their elements at a time: lane (token, 16-byte piece).  Two tokens of a phase differ in the bits that part their
-                    // pieces in the raw lines and in the tile's, so that neither meets in a bank; all offsets but this lane's are constants
-                    constexpr int HALVES = D / 64;
-                    const int pr = lane >> 3, sel = (lane >> 2) & 1, c4 = lane & 3, in8 = D == 128 ? (sel ? pr ^ 5 : pr) : 2 * pr + sel;
-                    const uint32_t from = D == 128 ? cw * 4096 + in8 * 128 + ((c4 ^ in8) * 16) : cw * 2048 + (in8 >> 1) * 128 + ((((in8 & 1) * 4 + c4) ^ (in8 >> 1)) * 16);
-                    const uint32_t to = (cw & 1) * 4096 + in8 * 128 + (((2 * c4) ^ in8) * 16);
-                    const int mine = cw * 32 + lane, pos = t0 + mine;        // this lane's token, whose factors the others ask for
-                    auto convert = [&](const uint8_t* raw, uint8_t* tile, auto values_, auto some_, int e) {
-                        constexpr bool VALUES = decltype(values_)::value, SOME = decltype(some_)::value;       // SOME: values of a block with drafted tokens
-                        const __half2 factor = half2_pow2(e);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {                        // eight tokens each
-                            const uint32_t fw = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&factor), i * 8 + in8);
-                            const __half2 by = *reinterpret_cast<const __half2*>(&fw);
-#pragma unroll
-                            for (int half = 0; half < HALVES; ++half) {
-                                const uint32_t at = D == 128 ? (from + i * 1024) ^ (half * 64) : (from + i * 512) ^ ((i & 1) * 64);
-                                const uint4 w = *reinterpret_cast<const uint4*>(raw + at);
-                                uint32_t y[4] = {w.x, w.y, w.z, w.w};
-                                if constexpr (SOME) {                        // what lies behind the last token, and what is no number of a drafted one
-                                    const int token = t0 + cw * 32 + i * 8 + in8;
-                                    uint32_t any = 0;
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        const uint32_t no = token >= total ? ~0u : token >= len ? __vcmpeq4(y[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) : 0u;
-                                        any |= no;
-                                        y[k] &= ~no;
-                                    }
-                                    if (any && token < total) atomicOr(&taint[item & 7], 1ull << (token - len));
-                                }
-                                uint32_t h[8];
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    const uint32_t two = e4m3x2(k & 1 ? y[k >> 1] >> 16 : y[k >> 1]);
-                                    const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&two), by);
-                                    h[k] = *reinterpret_cast<const uint32_t*>(&z);
-                                }
-                                // tile of keys: halves 16 KB apart, pages 8 KB; of values: pages 8 KB times the halves, halves 8 KB
-                                const uint32_t part = i * 1024 + (VALUES ? ((cw >> 1) * HALVES + half) * 8192 : half * (BLOCK * 128) + (cw >> 1) * 8192);
-                                *reinterpret_cast<uint4*>(tile + to + part) = make_uint4(h[0], h[1], h[2], h[3]);
-                                *reinterpret_cast<uint4*>(tile + (to ^ 16) + part) = make_uint4(h[4], h[5], h[6], h[7]);
-                            }
-                        }
-                    };
-                    const int e = ok ? exps[mine] : 0;                       // behind the last token: anything, but no more than the largest
-                    const uint8_t* raw = sr + sR * 2 * S::RAW + (values ? S::RAW : 0);
-                    if (!values) {
-                        if (ok && n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
-                        if (ok) convert(raw, sk + sK * S::TILE, Flag<false>(), Flag<false>(), min(e - top, 0) + K_ROOM);
-                        if (tid == 0) { k_ref[n & 7] = top; v_ref[n & 7] = ref; }
-                    } else {
-                        if (ok && n >= NV) ok = wait(&v_empty[sV], n / NV - 1);
-                        const int by = pos >= total ? 0 : min(e - ref + V_ROOM, K_ROOM);
-                        if (ok && t0 + BLOCK <= len) convert(raw, sv + sV * S::TILE, Flag<true>(), Flag<false>(), by);
-                        else if (ok) convert(raw, sv + sV * S::TILE, Flag<true>(), Flag<true>(), by);
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(values ? &v_ready[sV] : &k_full[sK]);
-                        mbar_arrive(&raw_empty[sR]);
-                    }
+                    if (odd) atomicOr(&taint[item & 7], 1ull << (t - len));
                 }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_ready[sV]);
                 ok = __all_sync(0xffffffffu, ok);
             }
             u += it.n;
@@ -583,33 +415,25 @@ __global__ void __launch_bounds__(Split<Q8>::THREADS, 1) paged_tree_tiles_kernel
 }  // namespace
 
 // All items' partial results, two for each CTA and item.
-template <int D, bool Q8>
+template <int D>
 int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
-    using S = Sm<D, Q8>;
+    using S = Sm<D>;
     CUtensorMap mk, mv;
-    if constexpr (Q8) {                                  // raw pages as 128-byte lines
-        constexpr int LINES = PAGE * D / 128;
-        const long long lines = (long long)p.n_pages * p.Hk * LINES;
-        if (ptb_make_tmap_bf16(&mk, k_pages, 64, lines, 64, 64, LINES) || ptb_make_tmap_bf16(&mv, v_pages, 64, lines, 64, 64, LINES)) return -1;
-    } else {
-        const long long rows = (long long)p.n_pages * p.Hk * PAGE;
-        if (ptb_make_tmap_bf16(&mk, k_pages, D, rows, D, 64, PAGE) || ptb_make_tmap_bf16(&mv, v_pages, D, rows, D, 64, PAGE)) return -1;
-    }
+    const long long rows = (long long)p.n_pages * p.Hk * PAGE;
+    if (ptb_make_tmap_bf16(&mk, k_pages, D, rows, D, 64, PAGE) || ptb_make_tmap_bf16(&mv, v_pages, D, rows, D, 64, PAGE)) return -1;
     static bool attr[64];
     int dev = 0;
     PTB_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_tiles_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL + plan_bytes(MAX_B)));
+        PTB_CUDA_OK(cudaFuncSetAttribute(paged_tree_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL + plan_bytes(MAX_B)));
         if (dev < 64) attr[dev] = true;
     }
-    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D, Q8>, dim3(p.ctas), dim3(Split<Q8>::THREADS), (size_t)S::TOTAL + plan_bytes(p.B), st, ptb_pdl_enabled(), mk, mv, p));
+    PTB_CUDA_OK(ptb_launch(paged_tree_tiles_kernel<D>, dim3(p.ctas), dim3(THREADS), (size_t)S::TOTAL + plan_bytes(p.B), st, ptb_pdl_enabled(), mk, mv, p));
     PTB_CUDA_OK(cudaGetLastError());
     return 0;
 }
-template int launch_tiles<64, false>(const Params&, const void*, const void*, cudaStream_t);
-template int launch_tiles<64, true>(const Params&, const void*, const void*, cudaStream_t);
-template int launch_tiles<128, false>(const Params&, const void*, const void*, cudaStream_t);
-template int launch_tiles<128, true>(const Params&, const void*, const void*, cudaStream_t);
+template int launch_tiles<64>(const Params&, const void*, const void*, cudaStream_t);
+template int launch_tiles<128>(const Params&, const void*, const void*, cudaStream_t);
 
 }  // namespace tree
 }  // namespace ptb

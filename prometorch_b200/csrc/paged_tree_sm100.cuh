@@ -57,19 +57,8 @@ __device__ __forceinline__ uint32_t visible32(unsigned long long seen, int d0) {
     if (d0 <= -32) return ~0u;
     return ((1u << -d0) - 1) | (uint32_t)(seen << -d0);
 }
-// Largest byte of a warp's words.
-__device__ __forceinline__ uint32_t byte_max(uint32_t v) {
-    return __reduce_max_sync(0xffffffffu, max(max(v & 255, (v >> 8) & 255), max((v >> 16) & 255, v >> 24)));
-}
-// 2^e as two fp16 (zero below what fp16 has).
-__device__ __forceinline__ __half2 half2_pow2(int e) {
-    const uint32_t h = e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
-    const uint32_t w = h | (h << 16);
-    return *reinterpret_cast<const __half2*>(&w);
-}
+// 2^e, for e kept in the range of a normal number.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
-
-template <bool X> struct Flag { static constexpr bool value = X; };
 
 }  // namespace tree
 }  // namespace ptb

@@ -496,3 +496,32 @@ def test_keep_reports_bad_pages_and_paths():
         with pytest.raises(IndexError):
             P.check_status(DEV)
         assert torch.equal(k, before)
+
+
+@pytest.mark.parametrize("kind", ["e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [(6, 1), (5, 4), (8, 4), (16, 4), (20, 4), (40, 8), (64, 8)])
+@pytest.mark.parametrize("cached", [False, True])
+def test_a_large_token_without_weight(kind, D, T, G, cached):
+    """A token 2^40 and more times as large as all others: a drafted one that nobody sees, or a cached one that half of the rows weigh with zero (and the other half with one).  What the
+    others come to does not depend on it.  A score's terms are up to 2^8 (|q| to 4.5, |k| to 5, 128 of them, by D^-0.5) where the token has no weight: fp32 sums as in `close`."""
+    Hk, len0 = 2, 477
+    H, at = Hk * G, (300 if cached else len0 + T // 2)
+    g = gen(T + D)
+    table, n_pages = table_for([len0 + T], 1)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    page, place = int(table[0, at // PAGE]), at % PAGE
+    if kind == "bf16":
+        k[page, :, place], v[page, :, place] = 2.0 ** 60, 2.0 ** 60
+    else:
+        for pool, exps in ((k, ke), (v, ve)):
+            pool[page, :, place] = torch.full((D,), 448.0, device=DEV).to(R.E4M3)
+            exps[page, :, place] = 191
+    q = torch.randn(1, T, H * D, device=DEV, generator=g).bfloat16()
+    full = torch.tensor([[sum(1 << j for j in range(T) if cached or len0 + j != at) - (1 << 64 if T == 64 else 0)] * T], dtype=torch.int64, device=DEV)
+    lens = torch.tensor([len0], dtype=torch.int32, device=DEV)
+    got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, mask=full, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, [len0], [T], full, table, k, v, ke, ve, D ** -0.5)
+    small = want.abs() < 2.0 ** 30
+    assert bool(small.any()) and bool((~small).any()) == cached
+    close(got, want, mag, kind)
