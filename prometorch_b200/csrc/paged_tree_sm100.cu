@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
         const int g = (warp - SOFTMAX_WARP) >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + TM_S + (uint32_t)(g * BLOCK), to = lanes + TM_O + (uint32_t)(g * D);
         int base = 0, s_turn = 0, o_turn = 0;
+        const float f = P.scale_log2, grow = 8.f / f;    // weights are powers of two of f times a score less the row's reference m, which lags behind the maximum by no more than `grow`
         // what a thread knows of its row in an item
         struct Row { Item it; bool live, on; unsigned long long seen; };
         auto enter = [&](int u, int item) {
@@ -224,7 +225,6 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                 if (live && ok) {
                     const int bad = bad_pages[n & 7];
                     const bool some = t0 + BLOCK > len || bad;               // not every row sees every token
-                    const float f = P.scale_log2;
                     uint32_t r[BLOCK];                                       // all scores of the block
 #pragma unroll
                     for (int c = 0; c < BLOCK / 32; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
@@ -242,23 +242,23 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int i = 0; i < BLOCK; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                     float alpha = 1.f;
-                    if (mx > m + 8.f) {
-                        alpha = exp2f(m - mx);
+                    if (mx > m + grow) {
+                        alpha = exp2f((m - mx) * f);
                         m = mx;
                         l *= alpha;
                     }
-                    const float mu = m == -INFINITY ? 0.f : m;
-                    const uint64_t f2 = both(f), mu2 = both(-mu);
+                    const uint64_t f2 = both(f), mu2 = both(m == -INFINITY ? 0.f : -m);
                     uint64_t l2[2] = {0, 0};
-                    // the packed weights take the place of the scores, in registers and in tensor memory
+                    // The packed weights take the place of the scores, in registers and in tensor memory.  The reference is taken off before the scale: as one fused product and sum, against a
+                    // rounded product, the largest of scores around 2^31 would lie above its own reference by more than fp32 holds
 #pragma unroll
                     for (int c = 0; c < BLOCK / 32; ++c) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float x, y;
-                            apart(fma2(pair(r[32 * c + 2 * i], r[32 * c + 2 * i + 1]), f2, mu2), x, y);
+                            apart(mul2(add2(pair(r[32 * c + 2 * i], r[32 * c + 2 * i + 1]), mu2), f2), x, y);
                             x = exp2f(x);
                             y = exp2f(y);
                             l2[i & 1] = add2(l2[i & 1], pair(__float_as_uint(x), __float_as_uint(y)));
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                     }
                 }
             }
-            const float2 mine = on && it.n > g ? make_float2(m == -INFINITY && l != 0.f ? 0.f : m, l) : make_float2(-INFINITY, 0.f);      // a sum without a maximum is of no numbers
+            const float2 mine = on && it.n > g ? make_float2(m == -INFINITY && l != 0.f ? 0.f : m * f, l) : make_float2(-INFINITY, 0.f);      // a sum without a maximum is of no numbers
             if (live) *ml = mine;
             if (shared) both_sync();
             if (whole && live && it.n > g) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
     } else {
         // ------------------------------------------------------------------------------------ tiles
         regs_dec<REGS_OTHER>();
-        const int tid = threadIdx.x - CONVERT_WARP * 32;
+        const int tid = (threadIdx.x - CONVERT_WARP * 32) & 127;
         int n = 0, item = 0;
         for (int u = u0; u < u1; ++item) {               // after a wait that ran out as well: the four warps meet at every item
             const Item it = item_at(P, starts, u, u1);
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
             for (int j = 0; j < it.n; ++j, ++n) {
                 const int t0 = (it.first + j) * BLOCK, sV = n % NV, t = t0 + tid;
                 ok = wait(&v_full[sV], n / NV);
-                if (ok && t >= len) {                    // a drafted token, or none
+                if (ok && t0 + BLOCK > len && t >= len) {                    // a drafted token, or none
                     uint8_t* v = sv + sV * S::TILE + (tid >> 6) * (D / 64) * 8192 + (tid & 63) * 128;
                     bool odd = false;
                     for (int i = 0; i < D / 8; ++i) {

@@ -498,7 +498,7 @@ def test_keep_reports_bad_pages_and_paths():
         assert torch.equal(k, before)
 
 
-@pytest.mark.parametrize("kind", ["e4m3"])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T,G", [(6, 1), (5, 4), (8, 4), (16, 4), (20, 4), (40, 8), (64, 8)])
 @pytest.mark.parametrize("cached", [False, True])
