@@ -194,21 +194,21 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                     const int p0 = 2 * (it.first + j);
                     if (ids_from < 0 || p0 - ids_from >= 32) {
                         ids_from = p0;
-                        ids = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : -2;        // -2: behind the last page
-                        if (ids != -2 && (ids < 0 || ids >= P.n_pages)) {
+                        ids = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : 0;
+                        if (ids < 0 || ids >= P.n_pages) {
                             ids = -1;
                             if (P.status && (p0 + lane) / 2 < it.first + it.n) atomicExch(P.status, PTB_ERR_BOUNDS);
                         }
                     }
                     const int page[2] = {__shfl_sync(0xffffffffu, ids, p0 - ids_from), __shfl_sync(0xffffffffu, ids, p0 + 1 - ids_from)};
                     if (lane == 0) {
-                        const int there = page[1] == -2 ? 1 : 2, sK = n % NK, sV = n % NV;
+                        const int there = p0 + 1 < pages ? 2 : 1, sK = n % NK, sV = n % NV;
                         if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
                         else if (n >= 2) ok = wait(&k_full[n - 2], 0);               // two blocks under way at a time: what others fetch does not wait behind a whole ring
                         if (ok) {
                             bad_pages[n & 7] = (page[0] < 0 ? 1 : 0) | (page[1] < 0 ? 2 : 0);
                             mbar_expect_tx(&k_full[sK], there * (S::TILE / 2 + (Q8 ? 2 * PAGE : 0)));
-                            auto page_to = [&](uint8_t* dst, const CUtensorMap* map, int x, uint64_t* bar) {         // a page that is none of the pool's: any other in its place, which no row sees
+                            auto page_to = [&](uint8_t* dst, const CUtensorMap* map, int x, uint64_t* bar) {         // a page that is none of the pool's: any other in its place, which no row sees and whose values are cleared
                                 const int row = (max(page[x], 0) * P.Hk + it.kvh) * PAGE;
                                 if constexpr (Q8) tma_load_2d(dst + x * (S::TILE / 2), map, 0, row, bar);
                                 else
@@ -650,12 +650,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
             for (int j = 0; j < it.n; ++j, ++n) {
                 const int t0 = (it.first + j) * BLOCK, sV = n % NV, t = t0 + tid;
                 ok = wait(&v_full[sV], n / NV);
-                if (ok && t >= len) {                    // a drafted token, or none
+                const bool none = t >= total || (ok && (bad_pages[n & 7] >> (tid >> 6)) & 1);
+                if (ok && (t >= len || none)) {          // a drafted token, or none
                     uint8_t* v = sv + sV * S::TILE + (tid >> 6) * (S::TILE / 2) + (tid & 63) * (Q8 ? D : 128);
                     bool odd = false;
                     for (int i = 0; i < S::KEY / 16; ++i) {                  // in any order
                         uint4* w = reinterpret_cast<uint4*>(v + (Q8 ? i * 16 : (i / 8) * 8192 + (i & 7) * 16));
-                        if (t >= total) { *w = make_uint4(0, 0, 0, 0); continue; }
+                        if (none) { *w = make_uint4(0, 0, 0, 0); continue; }
                         uint4 x = *w;
                         uint32_t* y = reinterpret_cast<uint32_t*>(&x);
                         uint32_t any = 0;

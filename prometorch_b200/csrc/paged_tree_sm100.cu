@@ -98,15 +98,15 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                     const int p0 = 2 * (it.first + j);
                     static_assert(PAGE * 2 == BLOCK, "two pages a block");
                     if (lane < 2) {
-                        id = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : -2;        // -2: behind the last page
-                        if (id != -2 && (id < 0 || id >= P.n_pages)) {
+                        id = p0 + lane < pages ? P.page_table[(size_t)it.b * P.pt_stride + p0 + lane] : 0;
+                        if (id < 0 || id >= P.n_pages) {
                             id = -1;
                             if (P.status) atomicExch(P.status, PTB_ERR_BOUNDS);
                         }
                     }
                     const int page[2] = {__shfl_sync(0xffffffffu, id, 0), __shfl_sync(0xffffffffu, id, 1)};
                     if (lane == 0) {
-                        const int there = page[1] == -2 ? 1 : 2;
+                        const int there = p0 + 1 < pages ? 2 : 1;          // a page that is none of the pool's: any other in its place, which no row sees and whose values are cleared
                         const int sK = n % NK, sV = n % NV;
                         if (n >= NK) ok = wait(&k_empty[sK], n / NK - 1);
                         if (ok) {
@@ -379,12 +379,13 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
             for (int j = 0; j < it.n; ++j, ++n) {
                 const int t0 = (it.first + j) * BLOCK, sV = n % NV, t = t0 + tid;
                 ok = wait(&v_full[sV], n / NV);
-                if (ok && t0 + BLOCK > len && t >= len) {                    // a drafted token, or none
+                const bool none = t >= total || (ok && (bad_pages[n & 7] >> (tid >> 6)) & 1);
+                if (ok && (t >= len || none)) {          // a drafted token, or none
                     uint8_t* v = sv + sV * S::TILE + (tid >> 6) * (D / 64) * 8192 + (tid & 63) * 128;
                     bool odd = false;
                     for (int i = 0; i < D / 8; ++i) {
                         uint4* w = reinterpret_cast<uint4*>(v + (i / 8) * 8192 + (i & 7) * 16);
-                        if (t >= total) { *w = make_uint4(0, 0, 0, 0); continue; }
+                        if (none) { *w = make_uint4(0, 0, 0, 0); continue; }
                         uint4 x = *w;
                         uint32_t* y = reinterpret_cast<uint32_t*>(&x);
                         uint32_t any = 0;

@@ -525,3 +525,37 @@ def test_a_large_token_without_weight(kind, D, T, G, cached):
     small = want.abs() < 2.0 ** 30
     assert bool(small.any()) and bool((~small).any()) == cached
     close(got, want, mag, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [(3, 1), (8, 4), (12, 4), (20, 4), (64, 4)])
+@pytest.mark.parametrize("which", [0, 1, 2, 5])
+@pytest.mark.parametrize("what", [-1, -2, None, -2 ** 31, 2 ** 31 - 1])
+def test_any_id_outside_the_pool(kind, D, T, G, which, what):
+    """First or second page of a block, the one of the drafted tokens: reported, and the rest is as if its tokens were not there, whatever the pool's first page holds."""
+    Hk, have = 2, 320
+    H = Hk * G
+    g = gen(T + which)
+    n_pages = 9
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    for pool in (k, v):
+        if kind == "bf16":
+            pool[0] = math.nan
+        else:
+            pool.view(torch.uint8)[0] = 0x7f
+    table = torch.tensor([[4, 2, 7, 1, 8, 3, 5]], dtype=torch.int32, device=DEV)
+    bad = table.clone()
+    bad[0, which] = n_pages if what is None else what
+    q = torch.randn(1, T, H * D, device=DEV, generator=g).bfloat16()
+    lens = torch.tensor([have], dtype=torch.int32, device=DEV)
+    got = R.paged_attention_tree(q, H, Hk, D, lens, bad, k, v, k_exp=ke, v_exp=ve)
+    with pytest.raises(IndexError):
+        P.check_status(DEV)
+    P.check_status(DEV)
+    if which == 5:
+        want, mag = oracle(q, H, Hk, D, [have], [T], torch.zeros(1, T, dtype=torch.int64), table, k, v, ke, ve, D ** -0.5)
+    else:
+        kept = [i for i in range(table.shape[1]) if i != which]
+        want, mag = oracle(q, H, Hk, D, [have - PAGE], [T], None, table[:, kept].contiguous(), k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
