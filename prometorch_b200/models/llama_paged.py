@@ -10,7 +10,7 @@ import torch
 import torch.nn.functional as F
 
 from ..ops import paged as P
-from ..ops.paged_tree import paged_attention_tree, paged_write
+from ..ops.paged_tree import MAX_REQUESTS, paged_attention_tree, paged_write
 from .paged import PagedModel, PromptBatch, register_model
 
 
@@ -203,7 +203,10 @@ class PagedLlama(PagedModel):
         for l, L in enumerate(w.layers):
             if kv.quantised:
                 q, _ = paged_write(self._linear(h, L["wqkv"]), H, Hk, Dh, pos, req, table, self.cos, self.sin, kv.k[l], kv.v[l], k_exp=kv.k_exp[l], v_exp=kv.v_exp[l])
-                a = paged_attention_tree(q.view(B, 1, H * Dh), H, Hk, Dh, before, table, kv.k[l], kv.v[l], k_exp=kv.k_exp[l], v_exp=kv.v_exp[l]).view(B, H * Dh)
+                # a launch plans up to MAX_REQUESTS rows; drafted ids that are rows of the batch are more
+                parts = [paged_attention_tree(q[i:i + MAX_REQUESTS].unsqueeze(1), H, Hk, Dh, before[i:i + MAX_REQUESTS], table[i:i + MAX_REQUESTS], kv.k[l], kv.v[l], k_exp=kv.k_exp[l],
+                                              v_exp=kv.v_exp[l]) for i in range(0, B, MAX_REQUESTS)]
+                a = (parts[0] if len(parts) == 1 else torch.cat(parts)).view(B, H * Dh)
             else:
                 q = P.qkv_rope_write(h, L["wqkv"], H, Hk, Dh, pos, req, table, self.cos, self.sin, kv.k[l], kv.v[l],
                                      fuse_sum=True)

@@ -114,3 +114,23 @@ def test_more_requests_than_the_attention_of_trees_takes(kw):
             eng.set_weights(LlamaWeights.random(tiny(), seed=1))
     else:
         eng.set_weights(LlamaWeights.random(tiny(), seed=1))
+
+
+def test_drafted_rows_beyond_one_launch():
+    """Quantised pages, drafted ids as rows of the batch: 210 requests with four each are 1050 rows."""
+    w = LlamaWeights.random(tiny(num_hidden_layers=1, hidden_size=32, num_attention_heads=2, num_key_value_heads=1), seed=6)
+    got = []
+    for spec in (0, 4):
+        eng = LLMEngine(device="cpu", max_pages=220, max_active=210, kv_dtype="e4m3", spec_tokens=spec)
+        eng.set_weights(w)
+        for i in range(210):
+            eng.submit_request(Request(i, [1 + i % 90, 5, 6, 7, 8, 9] * 2 + [1 + i % 90], GenerationConfig(max_new_tokens=8, **GREEDY)))
+        rows = []
+        forward = eng._forward_rows
+        eng._draft = lambda s, k: [5, 6, 7, 8][:k]       # a draft for everybody, whatever was said before
+        eng._forward_rows = lambda r, **kw: (rows.append(len(r)), forward(r, **kw))[1]
+        for _ in range(3):
+            eng.step()
+        got.append([s.output_ids[:3] for s in eng.active])
+        assert (max(rows) > 1024) == (spec > 0)
+    assert got[0] == got[1]

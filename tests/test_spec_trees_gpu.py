@@ -82,3 +82,29 @@ def test_head_sizes_without_kernels_are_refused():
     for kw in (dict(kv_dtype="e4m3"), dict(spec_tokens=3, spec_branches=1)):
         with pytest.raises(ValueError):
             LLMEngine(device="cuda", max_pages=4, max_active=1, **kw).set_weights(w)
+
+
+def test_drafted_rows_beyond_one_launch():
+    """Quantised pages, drafted ids as rows of the batch: 129 requests with seven each share a graph of 2048 rows.  Tokens as above, for some of the requests."""
+    from prometorch_b200.serve.llm import GenerationConfig, LLMEngine, Request
+    w, prompts = setup(64, "e4m3")
+    config = dict(max_new_tokens=10, temperature=0.0, repetition_penalty=1.0, top_k=1)
+    e = LLMEngine(device="cuda", max_pages=400, max_active=129, kv_dtype="e4m3", spec_tokens=7)
+    e.set_weights(w)
+    for i in range(129):
+        e.submit_request(Request(i, prompts[i % 3][i % 7:], GenerationConfig(**config)))
+    got = {}
+    while e.num_active():
+        e.step()
+        got.update({r.request_id: r.token_ids for r in e.poll_responses()})
+    assert all(len(got[i]) == 10 for i in range(129)) and e.spec_accepted > 0
+    plain = LLMEngine(device="cuda", max_pages=64, max_active=4, kv_dtype="e4m3")
+    plain.set_weights(w)
+    for i in (0, 63, 64, 127, 128):
+        s = plain.open_sequence()
+        p = prompts[i % 3][i % 7:]
+        row = plain.feed([(s, p, [len(p) - 1])])[0]
+        for t in got[i]:
+            assert float(row.max() - row[t]) <= 2 * 5 * 3e-2 * float(row.square().mean().sqrt()), (i, t)
+            row = plain.feed([(s, [t], [0])])[0]
+        plain.close_sequence(s)
