@@ -19,7 +19,7 @@ namespace ptb {
 namespace {
 
 constexpr int VF_THREADS = 256, VF_EACH = 32, VF_CHUNK = VF_THREADS * VF_EACH;
-constexpr int VF_NODES = 64;                 // nodes of a request
+constexpr int VF_NODES = 64, VF_ROWS = 65536;      // nodes of a request, and of all: what the attention of trees takes
 constexpr int VF_CLUSTER = 16, VF_TOGETHER = 4;
 constexpr int VF_WIDE = 128;                 // CTAs of clusters of eight that surely find SMs of their own
 constexpr int VF_SLICE = 27 * 1024;          // logits, and the draft's probabilities, that a CTA can hold
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(const __grid_c
     __shared__ int place;
     pdl_wait();
     pdl_launch_dependents();
-    const int row = blockIdx.y, b = row / P.T, i = row - b * P.T, chunk = blockIdx.x, tid = threadIdx.x;
+    const int row = blockIdx.x / P.chunks, b = row / P.T, i = row - b * P.T, chunk = blockIdx.x - row * P.chunks, tid = threadIdx.x;
     if (i >= nodes_of(P, b)) return;
     if (tid == 0) place = 0x7fffffff;
     const float t = temperature_of(P, b), scale = (t > 0.f ? __frcp_rn(t) : 1.f) * 1.4426950408889634f;
@@ -394,8 +394,8 @@ PTB_API long long ptb_verify_work_bytes(int B, int T, int V) { return (long long
 PTB_API int ptb_verify_drafts(const void* logits, int bf16, long long l_batch, long long l_row, const float* probs, long long p_batch, long long p_row, const int* tokens, const int* parents,
                               const int* nodes, const float* u, const float* temperature, void* work, int* path, int* count, int* out, int B, int T, int V, cudaStream_t st) {
     if (B <= 0) return 0;
-    if (T < 1 || T > VF_NODES || V < 1 || (long long)B * T > 65535 || V > VF_SLICE * VF_CLUSTER) {
-        ptb_set_error("verify_drafts: %d requests of %d nodes over %d tokens (1 to %d nodes, %d in all, up to %d tokens)", B, T, V, VF_NODES, 65535, VF_SLICE * VF_CLUSTER);
+    if (T < 1 || T > VF_NODES || V < 1 || (long long)B * T > VF_ROWS || B > 65535 || V > VF_SLICE * VF_CLUSTER) {
+        ptb_set_error("verify_drafts: %d requests of %d nodes over %d tokens (1 to %d nodes, %d in all, up to %d tokens)", B, T, V, VF_NODES, VF_ROWS, VF_SLICE * VF_CLUSTER);
         return -1;
     }
     if (probs && parents) { ptb_set_error("verify_drafts: draft probabilities go with chains"); return -1; }
@@ -411,7 +411,7 @@ PTB_API int ptb_verify_drafts(const void* logits, int bf16, long long l_batch, l
     const int unit = bf16 ? 8 : 4;
     const bool vec = !((uintptr_t)logits & 15) && l_batch % unit == 0 && l_row % unit == 0;
     void (*k)(VerifyParams) = bf16 ? (vec ? verify_stats_kernel<true, true> : verify_stats_kernel<true, false>) : (vec ? verify_stats_kernel<false, true> : verify_stats_kernel<false, false>);
-    PTB_CUDA_OK(ptb_launch(k, dim3(p.chunks, B * T), dim3(VF_THREADS), 0, st, ptb_pdl_enabled(), p));
+    PTB_CUDA_OK(ptb_launch(k, dim3(B * T * p.chunks), dim3(VF_THREADS), 0, st, ptb_pdl_enabled(), p));
     // threads of a CTA of the walk: 1024 where each finds an SM of its own, else two of 512 share one
     const bool wide = (long long)B * cluster <= VF_WIDE;
     if (bf16 ? (wide ? launch_walk<true, 1024>(p, cluster, st) : launch_walk<true, 512>(p, cluster, st)) : (wide ? launch_walk<false, 1024>(p, cluster, st) : launch_walk<false, 512>(p, cluster, st)))

@@ -17,6 +17,7 @@ from .. import _native as N
 from .paged_tree import _index, _launch
 
 MAX_NODES = 64
+MAX_ROWS, MAX_VOCAB = 65536, 442368          # on the GPU: nodes of a batch, tokens that a cluster's shared memory holds
 MAX_TEMPERATURE = 2.0 ** 126
 
 
@@ -50,6 +51,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, t
 
     Returns ``(path, count, out)``, int32: ``path [B, T]`` the accepted nodes, the first one among them, -1 behind; ``count [B]`` how many drafted tokens were accepted (-1 for a
     request without nodes); ``out [B, T]`` their tokens and then the one that the target adds, -1 behind.
+
+    On the GPU a batch has up to 65536 nodes and a row up to 442368 tokens.
 
     A logit of -inf (or NaN) is a token of probability zero; where nothing is left to draw from, the arg-max of the row is taken.  Siblings with one token count
     once.  A token outside the vocabulary is rejected, a node whose parent does not come before it is never reached."""

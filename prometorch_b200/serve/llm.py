@@ -31,6 +31,7 @@ from ..models.llama_paged import LlamaConfig, LlamaWeights  # noqa: F401
 from ..models.paged import PagedModel, PromptBatch, entry_of, read_config, resolve_architecture
 from ..ops import paged as P
 from ..ops.paged_tree import E4M3, MAX_NODES, MAX_REQUESTS
+from ..ops.verify import MAX_VOCAB
 
 PAGE = P.PAGE
 
@@ -226,6 +227,8 @@ class LLMEngine:
             raise ValueError(f"{model.architecture or model.__name__}: no quantised pages for this model on {self.device.type}")
         if self.spec_branches and not (model.trees and model.takes_trees(w.cfg, self.device, self.dtype)):
             raise ValueError(f"{model.architecture or model.__name__}: no trees of drafted ids for this model on {self.device.type}")
+        if self.spec_branches and self.device.type == "cuda" and w.cfg.vocab_size > MAX_VOCAB:
+            raise ValueError(f"{model.architecture or model.__name__}: trees of drafted ids are verified over up to {MAX_VOCAB} tokens, not {w.cfg.vocab_size}")
         if (self.kv_dtype == E4M3 or self.spec_branches) and self.max_active > MAX_REQUESTS:
             raise ValueError(f"max_active: up to {MAX_REQUESTS} requests with quantised pages or trees of drafted ids, not {self.max_active}")
         self.model = model(w, self.device, self.dtype)

@@ -134,3 +134,11 @@ def test_drafted_rows_beyond_one_launch():
         got.append([s.output_ids[:3] for s in eng.active])
         assert (max(rows) > 1024) == (spec > 0)
     assert got[0] == got[1]
+
+
+def test_a_vocabulary_that_is_not_verified_is_refused_at_load():
+    from prometorch_b200.ops.verify import MAX_VOCAB
+    cfg = tiny(vocab_size=MAX_VOCAB + 1, hidden_size=128, num_attention_heads=2)
+    eng = LLMEngine(device="cuda", max_pages=4, max_active=1, dtype=torch.bfloat16, spec_tokens=2, spec_branches=1)
+    with pytest.raises(ValueError, match="verified"):
+        eng.set_weights(type("W", (), {"cfg": cfg})())

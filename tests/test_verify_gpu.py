@@ -170,3 +170,21 @@ def test_temperatures_of_any_size(dtype, t):
         u[:, 1:] *= (1.0, 1.0, 1e-4)[seed]                # small numbers accept tokens of a uniform row
         check(logits, tokens, u, torch.full((B,), t), parents=parents)
         check(logits, tokens, u, torch.full((B,), t))
+
+
+@pytest.mark.parametrize("B,T", [(1024, 64), (65535, 1), (8192, 8)])
+def test_as_many_nodes_as_the_attention_takes(B, T):
+    g = torch.Generator().manual_seed(T)
+    V = 5
+    logits = torch.randn(B, T, V, generator=g)
+    parents = (torch.arange(T).repeat(B, 1) - torch.randint(1, 4, (B, T), generator=g)).clamp_min(-1).int()
+    tokens, u = torch.randint(0, V, (B, T), generator=g).int(), torch.rand(B, T, generator=g)
+    args = [t.to(DEV) for t in (logits, tokens, u, torch.ones(B))]
+    got = verify_drafts(*args, parents=parents.to(DEV))
+    assert int(got[1].min()) >= 0 and bool((got[2] < V).all())
+    some = torch.cat([torch.arange(40), torch.arange(B - 200, B)])
+    want = verify_drafts_reference(logits[some], tokens[some], u[some], torch.ones(240), parents=parents[some])
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu()[some], b)
+    with pytest.raises(RuntimeError, match="in all"):
+        verify_drafts(torch.zeros(B + 1, T, V, device=DEV), torch.zeros(B + 1, T, dtype=torch.int32, device=DEV), torch.zeros(B + 1, T, device=DEV), torch.zeros(B + 1, device=DEV))
