@@ -20,7 +20,7 @@ struct WriteParams {
     const __nv_bfloat16* qkv;      // [n, ld]: q heads, then k heads, then v heads
     long long ld;
     const int* pos;                // [n] position (angle)
-    const int* slot;               // [n] place in the sequence's pages; null: the position.  Negative: nothing is stored
+    const int* slot;               // [n] place in the sequence's pages; null: the position.  Negative: nothing is stored, and a position outside the tables is no error
     const int* req;                // [n] row of the page table
     const int* page_table;
     int pt_stride, pt_rows, n_pages;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(PW_THREADS) paged_write_kernel(const __grid_co
     int page = -1;
     if (slot >= 0 && slot / PW_PAGE < P.pt_stride && req >= 0 && req < P.pt_rows) page = P.page_table[(size_t)req * P.pt_stride + slot / PW_PAGE];
     const bool stored = page >= 0 && page < P.n_pages && angle;
-    if (threadIdx.x == 0 && P.status && (!angle || (slot >= 0 && !stored))) atomicExch(P.status, PTB_ERR_BOUNDS);
+    if (threadIdx.x == 0 && P.status && slot >= 0 && !stored) atomicExch(P.status, PTB_ERR_BOUNDS);
     float c[8], s[8];
     if (angle) {
         const float4 *cs = reinterpret_cast<const float4*>(P.cos + (size_t)pos * HALF) + 2 * j, *sn = reinterpret_cast<const float4*>(P.sin + (size_t)pos * HALF) + 2 * j;
@@ -242,7 +242,7 @@ using namespace ptb;
 
 // Rotate q and k of `n` tokens (pairs (j, j + D/2)); q goes to q_out [n, H D], k and v to the page slots of (req, slot), slot null: the position, negative: not
 // stored.  qkv: [n, ld] bf16; cos / sin: [max_pos, D/2] fp32; k_out optional [n, Hk, D]: the rotated keys.  k_exp and v_exp null: bf16 pages
-// [n_pages, Hk, 64, D]; else e4m3 pages with one biased exponent byte for a token's keys (values) of a head.  D is 64 or 128.  Slots are distinct.
+// [n_pages, Hk, 64, D]; else e4m3 pages with one biased exponent byte for a token's keys (values) of a head.  D is 64 or 128.  Tokens of one slot are equal.
 PTB_API int ptb_paged_write(const void* qkv, long long ld, int n, int H, int Hk, int D, const int* pos, const int* slot, const int* req, const int* page_table, int pt_stride,
                             int pt_rows, int n_pages, const float* cos, const float* sin, int max_pos, void* q_out, void* k_out, void* k_pages, void* v_pages, void* k_exp,
                             void* v_exp, int* status, cudaStream_t st) {

@@ -311,7 +311,7 @@ int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_row, void*
 // ---------------------------------------------------------------------------- paged_write.cu
 // Rotate q and k of `n` tokens (pairs (j, j + D/2)); q goes to q_out [n, H D], k and v to the page slots of (req, slot), slot null: the position, negative: not
 // stored.  qkv: [n, ld] bf16; cos / sin: [max_pos, D/2] fp32; k_out optional [n, Hk, D]: the rotated keys.  k_exp and v_exp null: bf16 pages
-// [n_pages, Hk, 64, D]; else e4m3 pages with one biased exponent byte for a token's keys (values) of a head.  D is 64 or 128.  Slots are distinct.
+// [n_pages, Hk, 64, D]; else e4m3 pages with one biased exponent byte for a token's keys (values) of a head.  D is 64 or 128.  Tokens of one slot are equal.
 int ptb_paged_write(const void* qkv, long long ld, int n, int H, int Hk, int D, const int* pos, const int* slot, const int* req, const int* page_table, int pt_stride, int pt_rows, int n_pages, const float* cos, const float* sin, int max_pos, void* q_out, void* k_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, int* status, cudaStream_t st);
 
 // The cache entries of each request's accepted drafted tokens, moved from slot lens[b] + path[b][j] to lens[b] + j for j in 1 .. count[b], in every

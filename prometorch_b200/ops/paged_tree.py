@@ -127,8 +127,9 @@ def paged_write(qkv: torch.Tensor, H: int, Hk: int, D: int, pos: torch.Tensor, r
                 k_pages: torch.Tensor, v_pages: torch.Tensor, slot: Optional[torch.Tensor] = None, k_exp: Optional[torch.Tensor] = None,
                 v_exp: Optional[torch.Tensor] = None, want_k: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Rotates q and k of the ``n`` tokens of ``qkv [n, >= (H + 2 Hk) D]`` (pairs (j, j + D/2)) to the positions ``pos`` and stores k and v at
-    ``page_table[req[i], slot[i] // 64]``, place ``slot[i] % 64``.  ``slot`` None: the position; a negative one is not stored (padding).  No two tokens have one slot.  e4m3 pages
-    come with ``k_exp`` and ``v_exp``.  Returns the rotated ``q [n, H D]`` and, if asked for, the rotated keys ``[n, Hk, D]`` as they were before quantising."""
+    ``page_table[req[i], slot[i] // 64]``, place ``slot[i] % 64``.  ``slot`` None: the position.  A negative one is not stored (padding), and its q and k are turned only if its
+    position is one of the tables'.  Tokens of one slot are equal (rows that fill a batch up, with one id at one position).  e4m3 pages come with
+    ``k_exp`` and ``v_exp``.  Returns the rotated ``q [n, H D]`` and, if asked for, the rotated keys ``[n, Hk, D]`` as they were before quantising."""
     width, dev, home = (H + 2 * Hk) * D, qkv.device, qkv.get_device()
     if qkv.dim() != 2 or qkv.shape[1] < width or H < 0 or Hk <= 0 or D <= 0 or D % 2:
         raise ValueError(f"paged_write: rows of {width} values for {H} + 2 x {Hk} heads of {D} are needed, not {list(qkv.shape)}")
@@ -159,11 +160,13 @@ def paged_write(qkv: torch.Tensor, H: int, Hk: int, D: int, pos: torch.Tensor, r
             N.check(rc, "paged_write")
         return q, k
     x = qkv[:, :(H + 2 * Hk) * D].reshape(n, H + 2 * Hk, D).float()
-    c, s = cos[pos.long()][:, None], sin[pos.long()][:, None]
+    at = (pos if slot is None else slot).long()
+    keep, turns = at >= 0, (pos >= 0) & (pos < cos.shape[0])
+    if bool((keep & ~turns).any()):
+        raise IndexError(f"paged KV: a position outside the tables of {cos.shape[0]}")
+    c, s = (torch.where(turns[:, None], t[torch.where(turns, pos, 0).long()], torch.full((), none))[:, None] for t, none in ((cos, 1.0), (sin, 0.0)))
     a, b = x[:, :H + Hk, :D // 2], x[:, :H + Hk, D // 2:]
     turned = torch.cat([a * c - b * s, b * c + a * s], -1)
-    at = (pos if slot is None else slot).long()
-    keep = at >= 0
     page, at = _pages_of(page_table[req.long()[keep], at[keep] // PAGE], k_pages.shape[0]), at[keep] % PAGE
     for pages, exps, new in ((k_pages, k_exp, turned[keep][:, H:]), (v_pages, v_exp, x[keep][:, H + Hk:])):
         if quant:

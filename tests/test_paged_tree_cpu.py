@@ -209,3 +209,20 @@ def test_native_entries_refuse():
     assert "exponents" in (refused(L.ptb_paged_keep(ptrs, 1, 1, 4, 2, 128, 8, BASE, BASE, BASE, BASE, 4, BASE, None)) or "")
     assert "bytes" in (refused(L.ptb_paged_keep(ptrs, 1, 1, 4, 2, 100, 8, BASE, BASE, BASE, BASE, 4, BASE, None)) or "")
     assert L.ptb_paged_write(BASE, 1024, 0, 4, 2, 128, BASE, None, BASE, BASE, 2, 1, 8, BASE, BASE, 9, BASE, None, BASE, BASE, None, None, BASE, None) == 0
+
+
+def test_padding_may_have_any_position():
+    """Rows that are not stored: q and k are turned where the tables reach, else left as they are; a stored row outside the tables raises."""
+    D, H, Hk = 64, 2, 1
+    k, v, _, _ = pools(2, Hk, D, False)
+    before = k.clone()
+    qkv = torch.randn(4, (H + 2 * Hk) * D, generator=torch.Generator().manual_seed(1))
+    ang = torch.rand(5, D // 2) * 3
+    call = lambda pos, slot: R.paged_write(qkv, H, Hk, D, pos, i32(0, 0, 0, 0), i32(0, 1)[None], ang.cos(), ang.sin(), k, v, slot=slot, want_k=True)  # noqa: E731
+    q, kk = call(i32(-1, -7, -1, -2), None)
+    assert torch.equal(q, qkv[:, :H * D]) and torch.equal(kk[:, 0], qkv[:, H * D:(H + 1) * D]) and torch.equal(k, before)
+    q, _ = call(i32(3, 5, -1, 99), i32(-1, -1, -1, -1))
+    assert torch.equal(q[1:], qkv[1:, :H * D]) and not torch.equal(q[0], qkv[0, :H * D]) and torch.equal(k, before)
+    for pos in (i32(0, 5, 1, 2), i32(0, -1, 1, 2)):
+        with pytest.raises(IndexError):
+            call(pos, i32(0, 1, 2, 3))

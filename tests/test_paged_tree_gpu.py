@@ -559,3 +559,29 @@ def test_any_id_outside_the_pool(kind, D, T, G, which, what):
         kept = [i for i in range(table.shape[1]) if i != which]
         want, mag = oracle(q, H, Hk, D, [have - PAGE], [T], None, table[:, kept].contiguous(), k, v, ke, ve, D ** -0.5)
     close(got, want, mag, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_padding_may_have_any_position(kind):
+    """Rows that are not stored report nothing, and q and k are what the form for the CPU gives; a stored one outside the tables is reported."""
+    D, H, Hk, n = 128, 3, 2, 9
+    k, v, ke, ve = pools(gen(1), 2, Hk, D, kind)
+    before = R._as_bytes(k).clone()
+    qkv = torch.randn(n, (H + 2 * Hk) * D, device=DEV, generator=gen(2)).bfloat16()
+    ang = torch.rand(5, D // 2, generator=torch.Generator().manual_seed(1)) * 3
+    cos, sin = ang.cos(), ang.sin()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    on = lambda t: t.to(DEV) if t is not None else None  # noqa: E731
+    for pos, slot in ((i32(*[-1] * n), None), (i32(-5, 3, 5, 99, 4, -1, 0, 2 ** 31 - 1, -2 ** 31), i32(*[-1] * n)), (i32(-1, 2, 5, 99, 4, -1, 0, 1, -2), i32(-1, 70, -1, -1, 3, -9, 9, 127, -1))):
+        args = [torch.zeros(n, dtype=torch.int32), i32(0, 1)[None], cos, sin]
+        q, kk = R.paged_write(qkv, H, Hk, D, on(pos), *map(on, args), k, v, slot=on(slot), k_exp=ke, v_exp=ve, want_k=True)
+        P.check_status(DEV)
+        host = [t.cpu() if t is not None else None for t in (k, v, ke, ve)]
+        qc, kc = R.paged_write(qkv.cpu(), H, Hk, D, pos, *args, host[0], host[1], slot=slot, k_exp=host[2], v_exp=host[3], want_k=True)
+        assert torch.equal(q.cpu(), qc) and torch.equal(kk.cpu(), kc)
+        assert torch.equal(R._as_bytes(k).cpu(), R._as_bytes(host[0]))
+        if slot is None or int(slot.max()) < 0:
+            assert torch.equal(R._as_bytes(k), before)
+    R.paged_write(qkv, H, Hk, D, on(i32(*[-1] * n)), *map(on, args), k, v, slot=on(torch.arange(n, dtype=torch.int32)), k_exp=ke, v_exp=ve)
+    with pytest.raises(IndexError):
+        P.check_status(DEV)
