@@ -543,10 +543,10 @@ class LLMEngine:
         return logits, (ids, parents, table, lens, nodes)
 
     def _forward_trees(self, packed: torch.Tensor, mask: torch.Tensor) -> tuple:
-        """On a GPU a CUDA graph for each batch bucket; padding requests have no nodes."""
+        """On a GPU a CUDA graph for each batch bucket and number of nodes; padding requests have no nodes."""
         if self.device.type != "cuda" or not self.use_graphs:
             return self._tree_layers(packed.to(self.device), mask.to(self.device))
-        key = ("tree", packed.shape[0])
+        key = ("tree", *mask.shape)
         if key not in self._graphs:
             held = [t.clone().pin_memory() for t in (packed, mask)]
             on = [t.to(self.device) for t in held]

@@ -108,3 +108,13 @@ def test_drafted_rows_beyond_one_launch():
             assert float(row.max() - row[t]) <= 2 * 5 * 3e-2 * float(row.square().mean().sqrt()), (i, t)
             row = plain.feed([(s, [t], [0])])[0]
         plain.close_sequence(s)
+
+
+def test_the_number_of_drafted_ids_may_change():
+    from prometorch_b200.serve.llm import GenerationConfig, LLMEngine
+    w, prompts = setup(64, None)
+    e = LLMEngine(device="cuda", max_pages=64, max_active=4, spec_tokens=6, spec_branches=2)
+    e.set_weights(w)
+    for n in (6, 3, 6, 9):
+        e.spec_tokens = n
+        assert e.generate(prompts[0], GenerationConfig(max_new_tokens=12, temperature=0.0, repetition_penalty=1.0, top_k=1)).tokens_generated == 12
