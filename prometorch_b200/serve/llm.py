@@ -502,11 +502,11 @@ class LLMEngine:
             branched |= up != list(range(len(up)))
         self.launch_log.append(B)
         packed = torch.cat([ids, pos, slot, parents, rows[:, None], lens[:, None], nodes[:, None]], 1)
-        logits, (ids_d, parents_d, table, lens_d, nodes_d) = self._forward_trees(packed, tree_mask(parents))
+        chance = torch.cat([torch.rand(Bb, T, generator=self._gen), temperature[:, None]], 1)
+        logits, (ids_d, parents_d, table, lens_d, nodes_d, u, heat) = self._forward_trees(packed, tree_mask(parents), chance)
         heads = logits[:B, 0].clone() if not all(walked) else None          # before any is cut down
         logits = self._truncate(logits, running, walked)
-        u = torch.rand(Bb, T, generator=self._gen).to(dev)
-        path, count, out = verify_drafts(logits, ids_d, u, temperature.to(dev), parents=parents_d, nodes=nodes_d)
+        path, count, out = verify_drafts(logits, ids_d, u, heat, parents=parents_d, nodes=nodes_d)
         if branched:
             paged_keep(self.kv.layers(), lens_d, path, count, table)
         said = torch.cat([count[:, None], out], 1).tolist()                 # the pass's one synchronisation
@@ -533,22 +533,22 @@ class LLMEngine:
             logits[b] = torch.full_like(logits[b], -float("inf")).scatter_(1, at, vals)
         return logits
 
-    def _tree_layers(self, packed: torch.Tensor, mask: torch.Tensor) -> tuple:
+    def _tree_layers(self, packed: torch.Tensor, mask: torch.Tensor, chance: torch.Tensor) -> tuple:
         """The device work of a pass over trees: logits ``[B, T, V]`` and what the verification reads."""
         T = mask.shape[1]
         ids, pos, slot, parents = (packed[:, i * T:(i + 1) * T].contiguous() for i in range(4))
         rows, lens, nodes = (packed[:, 4 * T + i].contiguous() for i in range(3))
         table = self.page_table[rows.long()]
         logits = self.model.tree_pass(self.kv, table, ids, pos, slot, lens, nodes, mask)
-        return logits, (ids, parents, table, lens, nodes)
+        return logits, (ids, parents, table, lens, nodes, chance[:, :T].contiguous(), chance[:, T].contiguous())
 
-    def _forward_trees(self, packed: torch.Tensor, mask: torch.Tensor) -> tuple:
+    def _forward_trees(self, packed: torch.Tensor, mask: torch.Tensor, chance: torch.Tensor) -> tuple:
         """On a GPU a CUDA graph for each batch bucket and number of nodes; padding requests have no nodes."""
         if self.device.type != "cuda" or not self.use_graphs:
-            return self._tree_layers(packed.to(self.device), mask.to(self.device))
+            return self._tree_layers(*(t.to(self.device) for t in (packed, mask, chance)))
         key = ("tree", *mask.shape)
         if key not in self._graphs:
-            held = [t.clone().pin_memory() for t in (packed, mask)]
+            held = [t.clone().pin_memory() for t in (packed, mask, chance)]
             on = [t.to(self.device) for t in held]
             idle = on[0].clone()
             idle[:, -1] = 0                                                 # warm-up without nodes: it writes nothing
@@ -556,7 +556,7 @@ class LLMEngine:
             side = torch.cuda.Stream(device=self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(side):
-                self._tree_layers(idle, on[1])
+                self._tree_layers(idle, *on[1:])
             torch.cuda.current_stream(self.device).wait_stream(side)
             torch.cuda.synchronize(self.device)
             graph = torch.cuda.CUDAGraph()
@@ -564,7 +564,7 @@ class LLMEngine:
                 out = self._tree_layers(*on)
             self._graphs[key] = (graph, on, held, out)
         graph, on, held, out = self._graphs[key]
-        for h, d, t in zip(held, on, (packed, mask)):
+        for h, d, t in zip(held, on, (packed, mask, chance)):               # all that the pass and the verification read: nothing is copied behind the pass, which would wait for it
             h.copy_(t)
             d.copy_(h, non_blocking=True)
         graph.replay()

@@ -118,3 +118,27 @@ def test_the_number_of_drafted_ids_may_change():
     for n in (6, 3, 6, 9):
         e.spec_tokens = n
         assert e.generate(prompts[0], GenerationConfig(max_new_tokens=12, temperature=0.0, repetition_penalty=1.0, top_k=1)).tokens_generated == 12
+
+
+def test_a_pass_over_trees_synchronises_once():
+    """Nothing is copied to the GPU behind the pass: the host launches the verification while the layers run."""
+    import warnings
+    from prometorch_b200.serve.llm import GenerationConfig, LLMEngine, Request
+    w, prompts = setup(64, None)
+    e = LLMEngine(device="cuda", max_pages=64, max_active=4, spec_tokens=6, spec_branches=2)
+    e.set_weights(w)
+    for i, p in enumerate(prompts):
+        e.submit_request(Request(i, p, GenerationConfig(max_new_tokens=60, temperature=0.5 * i, repetition_penalty=1.0, top_k=20)))
+    for _ in range(3):
+        e.step()
+    waits = []
+    for _ in range(6):                       # one in which no request starts a page
+        with warnings.catch_warnings(record=True) as said:
+            warnings.simplefilter("always")
+            torch.cuda.set_sync_debug_mode("warn")
+            try:
+                e.step()
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+        waits.append(sum("synchroniz" in str(x.message) for x in said))
+    assert min(waits) == 1, waits
