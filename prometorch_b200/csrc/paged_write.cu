@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(PW_THREADS) paged_write_kernel(const __grid_co
     }
 }
 
-constexpr int KEEP_LAYERS = 36, KEEP_THREADS = 256, KEEP_AT_ONCE = 4;
+constexpr int KEEP_THREADS = 256, KEEP_AT_ONCE = 4;
+constexpr int KEEP_LAYERS = (4096 - 128) / (4 * (int)sizeof(void*));     // as many as the parameters of a launch hold, 4 KB
 static_assert(KEEP_THREADS == 64 * KEEP_AT_ONCE, "a thread for each layer and token");
 
 struct KeepParams {
@@ -180,6 +181,7 @@ struct KeepParams {
     int pt_stride, n_pages, Hk, row, T, layers;        // row: bytes of a token's keys of a head
     int* status;
 };
+static_assert(sizeof(KeepParams) <= 4096, "parameters of a launch");
 
 // A block moves the keys (or the values) of one head in up to four layers: threads are (token of the path, 16-byte piece), as many tokens at a time as fit.  A path ascends, so a token never
 // moves behind its own place and no later one reads a slot that an earlier one filled; within a group all are read before the first is written.  Latency

@@ -585,3 +585,21 @@ def test_padding_may_have_any_position(kind):
     R.paged_write(qkv, H, Hk, D, on(i32(*[-1] * n)), *map(on, args), k, v, slot=on(torch.arange(n, dtype=torch.int32)), k_exp=ke, v_exp=ve)
     with pytest.raises(IndexError):
         P.check_status(DEV)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("layers", [123, 124, 125, 250])
+def test_keep_of_many_layers(kind, layers):
+    """Up to as many as one launch takes, and more."""
+    T, Hk, D = 5, 1, 64
+    stacks = [pools(gen(l), 3, Hk, D, kind) for l in range(layers)]
+    lens, path, count, table = (torch.tensor(x, dtype=torch.int32) for x in ([62], [[0, 2, 4, -1, -1]], [2], [[2, 0]]))
+    host = [[t.cpu() if t is not None else None for t in s] for s in stacks]
+    give = (lambda s: s) if kind == "e4m3" else (lambda s: s[:2])
+    R.paged_keep([give(s) for s in stacks], *(t.to(DEV) for t in (lens, path, count, table)))
+    R.paged_keep([give(s) for s in host], lens, path, count, table)
+    P.check_status(DEV)
+    for s, t in zip(stacks, host):
+        for a, b in zip(s, t):
+            if a is not None:
+                assert torch.equal(R._as_bytes(a).cpu(), R._as_bytes(b))
