@@ -492,17 +492,20 @@ int sm_count() {
     }
     return n;
 }
-// Which kernel, by the rows of a (request, kv head), the type of the pages and what the page table has room for: its tile of rows, the tokens of a unit and the partial
-// results that a CTA leaves of an item.
+// Which kernel, by the rows of a (request, kv head), the type of the pages and how many of those there are: its tile of rows, the tokens of a unit and the partial
+// results that a CTA leaves of an item.  Nothing goes by the page table's width, which says how long a request may get and not how long it is.
 //   up to 16 rows, bf16: mma.sync.  16 requests of 8192 tokens, 8 rows of 128: 78.6 us, tokens along the lanes of tensor memory 81; one of 540 tokens, 4 rows: 12.2 and 17.7.
-//   up to 32 rows, bf16, and two pages a CTA at most: mma.sync, in one or two tiles.  One request of 540 tokens, 20 rows of 128: 14.9 us, tokens along the lanes 20.
-//   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 87 and 90 us, in tiles of 128 rows 104 and 108; e4m3, 64 rows over 4100
-//   tokens: 73 and 117.  e4m3, 4 rows over 8192 tokens, 32 requests: 85, where mma.sync, for which every warp converts what it reads, took 148.
+//   up to 32 rows, bf16, and requests times kv heads (two tiles each) for half of the SMs at most: mma.sync, in two tiles.  It starts, changes an item and ends in less time, and cuts a long item into
+//   smaller pieces; with many items the products in two tiles cost more.  One request of 8 kv heads, 20 rows of 128 over 540, 2000 and 8000 tokens: 12.5, 13.9 and 21.7 us, tokens along
+//   the lanes 15.6, 22.5 and 31.0; one of 2 kv heads, 32 rows over 8000: 19.6 and 49.8; four of 8 kv heads, 32 rows over 540 and 8000: 17.5 and 16.9, 46 and 42; eight: 19.5 and
+//   19.7, at 4000 45.5 and 40.1; 32: 52 and 45.
+//   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 87 and 90 us, in tiles of 128 rows 104 and 108; e4m3, 4 rows over 8192 tokens,
+//   32 requests: 85, where mma.sync, for which every warp converts what it reads, took 148.
 //   more, bf16: tiles of 128 rows.
 //   more, e4m3: tokens along the lanes, in tiles of 64 rows (see paged_tree_sm100.cu).
 struct Choice { int tile_rows, unit, parts; };
-Choice choose(int rows, bool q8, long long pages) {
-    if (!q8 && (rows <= ROWS || (rows <= 2 * ROWS && pages * ((rows + ROWS - 1) / ROWS) <= 2 * sm_count()))) return {ROWS, PAGE, 1};
+Choice choose(int rows, bool q8, long long heads) {
+    if (!q8 && (rows <= ROWS || (rows <= 2 * ROWS && heads <= sm_count() / 2 / 2))) return {ROWS, PAGE, 1};
     if (rows > 64) return q8 ? Choice{64, 128, 1} : Choice{128, 128, 2};
     if (rows <= 16) return {16, 128, 2};
     return {rows <= 32 ? 32 : 64, 128, rows <= 32 ? 2 : 1};
@@ -526,12 +529,11 @@ using namespace ptb;
 PTB_API long long ptb_paged_tree_work_floats(int B, int T, int H, int Hk, int D) {
     if (Hk <= 0 || T <= 0) return 0;
     long long most = 0;
-    for (const bool q8 : {false, true})                  // page tables with little room take the smallest tiles
-        for (const long long pages : {0ll, 1ll << 40}) {
-            const tree::Choice c = tree::choose(T * (H / Hk), q8, pages);
-            const long long n = (long long)tree::sm_count() * 2 * c.parts * (long long)tree::partial_floats(c.tile_rows, D);
-            most = n > most ? n : most;
-        }
+    for (const bool q8 : {false, true}) {
+        const tree::Choice c = tree::choose(T * (H / Hk), q8, (long long)B * Hk);
+        const long long n = (long long)tree::sm_count() * 2 * c.parts * (long long)tree::partial_floats(c.tile_rows, D);
+        most = n > most ? n : most;
+    }
     return most + B + 1;
 }
 
@@ -559,7 +561,7 @@ PTB_API int ptb_paged_attn_tree(const void* q, long long q_batch, long long q_ro
     p.q = (const __nv_bfloat16*)q; p.q_batch = q_batch; p.q_row = q_row; p.out = (__nv_bfloat16*)out; p.lens = lens; p.nodes = nodes; p.mask = (const unsigned long long*)mask;
     p.page_table = page_table; p.pt_stride = pt_stride; p.n_pages = n_pages; p.k_exp = (const uint8_t*)k_exp; p.v_exp = (const uint8_t*)v_exp; p.v_raw = (const uint8_t*)v_pages; p.work = work;
     p.B = B; p.T = T; p.H = H; p.Hk = Hk; p.G = H / Hk;
-    const tree::Choice c = tree::choose(T * p.G, k_exp != nullptr, (long long)B * Hk * pt_stride);
+    const tree::Choice c = tree::choose(T * p.G, k_exp != nullptr, (long long)B * Hk);
     p.tile_rows = c.tile_rows;
     p.unit = c.unit;
     p.parts = c.parts;

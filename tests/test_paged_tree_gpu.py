@@ -603,3 +603,55 @@ def test_keep_of_many_layers(kind, layers):
         for a, b in zip(s, t):
             if a is not None:
                 assert torch.equal(R._as_bytes(a).cpu(), R._as_bytes(b))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [(5, 4), (8, 4), (17, 1), (32, 1), (10, 4), (40, 3)])
+@pytest.mark.parametrize("B", [18, 19, 60])
+def test_strange_requests_beside_others(kind, D, T, G, B):
+    """In one batch, on both sides of the number of requests that another kernel takes 17 to 32 rows from: a masked token that is no number, a masked large one, a page that is none of the pool's,
+    a query that is no number, requests without nodes and without cached tokens, a page table with far more room than the requests need."""
+    Hk = 2
+    H = Hk * G
+    g = gen(T + B)
+    have = [(53 * b) % 700 for b in range(B)]
+    have[5] = 200
+    nodes = [T if b % 4 else max(1, T - b % 3) for b in range(B)]
+    nodes[7], have[8] = 0, 0
+    table, n_pages = table_for([n + T for n in have], 3)
+    table = torch.cat([table, torch.zeros(B, 500, dtype=torch.int32, device=DEV)], 1).contiguous()
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    behind = [n + t for n, t in zip(have, nodes)]
+    spoil(k, ke, table, behind, math.nan)
+    spoil(v, ve, table, behind, math.inf)
+    mask = random_masks(B, B, T)
+    q = torch.randn(B, T, H * D, device=DEV, generator=g).bfloat16()
+    clean = [t.clone() if t is not None else None for t in (k, v, ke, ve)]
+    for b, number in ((3, False), (4, True)):
+        mask[b] &= ~(1 << 2)
+        at = have[b] + 2
+        page = int(table[b, at // PAGE])
+        for pool, exps in ((k, ke), (v, ve)):
+            if kind == "bf16":
+                pool[page, :, at % PAGE] = 2.0 ** 60 if number else math.nan
+            else:
+                pool.view(torch.uint8)[page, :, at % PAGE] = 0x7e if number else 0x7f
+                exps[page, :, at % PAGE] = 191
+    lens, nd = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (have, nodes))
+    given, seen, seen_have = table.clone(), table.clone(), list(have)
+    given[5, 1] = -2
+    seen[5] = torch.cat([table[5, :1], table[5, 2:], table[5, :1]])
+    seen_have[5] -= PAGE
+    want, mag = oracle(q, H, Hk, D, seen_have, nodes, mask, seen, *clean, D ** -0.5)
+    strange = q.clone()
+    strange[6, 1, D + 3] = math.nan
+    got = R.paged_attention_tree(strange, H, Hk, D, lens, given, k, v, mask=mask.to(DEV), nodes=nd, k_exp=ke, v_exp=ve)
+    with pytest.raises(IndexError):
+        P.check_status(DEV)
+    if int(nodes[6]) > 1 and have[6]:
+        assert bool(got[6, 1, D:2 * D].isnan().all())
+    got[6, 1, D:2 * D] = want[6, 1, D:2 * D].bfloat16()
+    close(got, want, mag, kind)
+    for b, n in enumerate(nodes):
+        assert not got[b, n:].any()
