@@ -9,7 +9,7 @@
 // be any head element, so lane r holds one 16-byte piece of a value row for all tiles.  Which of eight tokens lane r takes (`token_of`) is chosen so
 // that the eight lanes of a quarter warp fall on the eight 16-byte columns of the swizzled rows, for keys and for values.
 //
-// P is rounded to bf16 (by at most 2^-9 of a weight's power of two, without a bias); scores, maxima, sums and accumulators are fp32.
+// A weight is two bf16, itself rounded and what that leaves (2^-18 of it is lost), each a product of its own; scores, maxima, sums and accumulators are fp32.
 #include "paged_tree.cuh"
 
 namespace ptb {
@@ -276,10 +276,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
                 }
                 const uint32_t pa[4] = {pack2<false>(sc[0][0], sc[0][1]), pack2<false>(sc[0][2], sc[0][3]), pack2<false>(sc[1][0], sc[1][1]), pack2<false>(sc[1][2], sc[1][3])};
                 if (!tail || !__any_sync(0xffffffffu, odd)) {
+                    uint32_t rest[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) rest[i] = pack2_rest(sc[i >> 1][2 * (i & 1)], sc[i >> 1][2 * (i & 1) + 1], pa[i]);
 #pragma unroll
                     for (int i = 0; i < VW; ++i) {
-                        mma(acc[2 * i], pa, __byte_perm(vw[0][i], vw[1][i], 0x5410), __byte_perm(vw[2][i], vw[3][i], 0x5410));
-                        mma(acc[2 * i + 1], pa, __byte_perm(vw[0][i], vw[1][i], 0x7632), __byte_perm(vw[2][i], vw[3][i], 0x7632));
+                        const uint32_t b[4] = {__byte_perm(vw[0][i], vw[1][i], 0x5410), __byte_perm(vw[2][i], vw[3][i], 0x5410), __byte_perm(vw[0][i], vw[1][i], 0x7632),
+                                               __byte_perm(vw[2][i], vw[3][i], 0x7632)};
+                        mma(acc[2 * i], pa, b[0], b[1]);
+                        mma(acc[2 * i + 1], pa, b[2], b[3]);
+                        mma(acc[2 * i], rest, b[0], b[1]);
+                        mma(acc[2 * i + 1], rest, b[2], b[3]);
                     }
                 } else {                                 // token by token, each for the rows that see it
 #pragma unroll

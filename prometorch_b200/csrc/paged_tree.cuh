@@ -149,6 +149,11 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return r;
 }
 
+// What two packed bf16 leave of two fp32, in bf16: sixteen bits of each between them.
+__device__ __forceinline__ uint32_t pack2_rest(float x, float y, uint32_t packed) {
+    return pack2<false>(x - __uint_as_float(packed << 16), y - __uint_as_float(packed & 0xffff0000u));
+}
+
 template <int D> int launch_tiles(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);               // paged_tree_sm100.cu: bf16
 template <int D, bool Q8> int launch_few(const Params& p, const void* k_pages, const void* v_pages, cudaStream_t st);        // paged_tree_few_sm100.cu
 

@@ -35,13 +35,13 @@ constexpr int THREADS = 512, REGS_SOFTMAX = 184, REGS_OTHER = 72;        // 256 
 template <int D, bool Q8, int N>
 struct Few {
     static constexpr int KEY = Q8 ? D : 2 * D;                         // bytes of a key, or a value
-    static constexpr int Q_PARTS = Q8 ? 2 : 1, P_PARTS = Q8 ? 3 : 1;
+    static constexpr int Q_PARTS = Q8 ? 2 : 1, P_PARTS = Q8 ? 3 : 2;
     static constexpr int Q_BYTES = N * D * 2, TILE = BLOCK * KEY;
     static constexpr int S_COLS = Q_PARTS * N;                         // columns of scores
-    static constexpr int O_COLS = Q8 ? P_PARTS * N : 64;               // of an accumulator, and of the weights' tile.  bf16: a whole line of 128 bytes for each token, whatever the number of rows
-    static constexpr int P_TILE = BLOCK * (Q8 && N == 64 ? 256 : 128); // lines of 128 bytes
+    static constexpr int O_COLS = P_PARTS * N;                         // of an accumulator, and of the weights' tile
+    static constexpr int P_TILE = BLOCK * (N == 64 ? 256 : 128);       // lines of 128 bytes
     static constexpr int TMEM = Q8 ? 512 : 256, TM_O = 2 * (Q8 ? 128 : 64);
-    static constexpr int NK = KEY == 256 ? 2 : Q8 && D == 128 && N == 64 ? 4 : 5, NV = KEY == 256 ? 3 : NK;
+    static constexpr int NK = KEY == 256 ? 2 : KEY == 128 && N == 64 ? 4 : 5, NV = KEY == 256 ? (N == 64 ? 2 : 3) : NK;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + NK * TILE, OFF_P = OFF_V + NV * TILE, OFF_E = OFF_P + 2 * P_TILE;
     static constexpr int OFF_M = OFF_E + (Q8 ? 8 * 2 * BLOCK : 0);     // exponents of eight blocks, then what the softmax groups share
     static constexpr int OFF_BAR = OFF_M + 5120 + 1024, OFF_PLAN = OFF_BAR + 512, TOTAL = OFF_PLAN + 1024;         // and the plan
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                 constexpr int LINE = Q8 ? 16 : 8;        // rows of a 16-byte piece
 #pragma unroll
                 for (int c = 0; c < R / LINE; ++c) {
-                    uint32_t w[LINE / 2];
+                    uint32_t w[LINE / 2], rest[LINE / 2];
 #pragma unroll
                     for (int k = 0; k < LINE / 2; ++k) {
                         const int i = LINE * c + 2 * k;
@@ -456,6 +456,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                         if constexpr (Q8) l2[i / 2] = fma2(xy, un2, l2[i / 2]);
                         else l2[i / 2] = add2(l2[i / 2], xy);
                         w[k] = pack2<Q8>(x, y);
+                        if constexpr (!Q8) rest[k] = pack2_rest(x, y, w[k]);
                     }
                     if constexpr (Q8) {
 #pragma unroll
@@ -471,7 +472,9 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                                 for (int k = 0; k < 8; ++k) w[k] = less_top_bytes(w[k], t[k]);
                         }
                     } else {
-                        *reinterpret_cast<uint4*>(pt + (((c + r0 / 8) ^ (tid & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        const int at = c + r0 / 8;               // what is left lies N rows on: in the other half of the line, or in the next line
+                        *reinterpret_cast<uint4*>(pt + ((at ^ (tid & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(pt + (N == 64 ? BLOCK * 128 : 0) + (((N == 64 ? at : at + N / 8) ^ (tid & 7)) * 16)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
                     }
                 }
                 fence_proxy_async();
