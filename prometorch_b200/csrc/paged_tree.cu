@@ -1,8 +1,8 @@
-// Up to sixteen rows of drafted tokens against a bf16 cache on mma.sync, and the merge of items that were cut; see paged_tree.cuh.
+// Sixteen rows of drafted tokens at a time against a bf16 cache on mma.sync (up to 32 rows in all), the merge of items that were cut, and which kernel takes what; see paged_tree.cuh.
 //
 // One CTA of eight warps per SM.  A warp takes every eighth piece of sixteen tokens of the CTA's run, keeps an online softmax of its own over them, and joins the others when
 // an item ends.  It brings its pieces itself: keys and values of a piece are one TMA box each of 128-byte rows with the 128-byte swizzle, into a ring that only this warp
-// reads, so that a stage is free again at a __syncwarp; the rings of an SM hold 64 to 128 KB, several times what the memory's latency needs.
+// reads, so that a stage is free again at a __syncwarp; the rings of an SM hold 128 KB, several times what the memory's latency needs.
 //
 // S = Q K^T and O = P V are m16n8k16 products whose operands come from shared memory 16 bytes a lane, without a transposing load.  The order of the contraction is
 // free as long as both operands keep it, so lane c of a row's four holds whole 16-byte pieces of a key; and output column n of tile t may
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
 
 // The partial results of items that were cut: one block per sixteen rows of an item, a thread (row, eight columns, every SLICES-th result); and the rows that no unit belongs
 // to, which are zeros.  With few blocks a chain of loads is what it costs, and four shorter ones cost less (a chain of 5 behind 540 tokens, both kernels: 14.9 us with one,
-// 12.3 with four); with more blocks than the SMs hold, more threads only wait (64 nodes, 8 requests: 9 and 18 us).
+// 12.4 with four); with more blocks than the SMs hold, more threads only wait (64 nodes, 8 requests: 9 and 18 us).
 // How the accumulators of a partial result lie: TILES [D / 8][rows][8], place i of a row column i % 8 of product tile i / 8;
 // EIGHTS the same in the order of the head; ROWWISE [rows][D].
 enum Layout { TILES, EIGHTS, ROWWISE };
@@ -501,18 +501,18 @@ int sm_count() {
 }
 // Which kernel, by the rows of a (request, kv head), the type of the pages and how many of those there are: its tile of rows, the tokens of a unit and the partial
 // results that a CTA leaves of an item.  Nothing goes by the page table's width, which says how long a request may get and not how long it is.
-//   up to 16 rows, bf16: mma.sync.  16 requests of 8192 tokens, 8 rows of 128: 78.6 us, tokens along the lanes of tensor memory 81; one of 540 tokens, 4 rows: 12.2 and 17.7.
-//   up to 32 rows, bf16, and requests times kv heads (two tiles each) for half of the SMs at most: mma.sync, in two tiles.  It starts, changes an item and ends in less time, and cuts a long item into
-//   smaller pieces; with many items the products in two tiles cost more.  One request of 8 kv heads, 20 rows of 128 over 540, 2000 and 8000 tokens: 12.5, 13.9 and 21.7 us, tokens along
-//   the lanes 15.6, 22.5 and 31.0; one of 2 kv heads, 32 rows over 8000: 19.6 and 49.8; four of 8 kv heads, 32 rows over 540 and 8000: 17.5 and 16.9, 46 and 42; eight: 19.5 and
-//   19.7, at 4000 45.5 and 40.1; 32: 52 and 45.
-//   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 87 and 90 us, in tiles of 128 rows 104 and 108; e4m3, 4 rows over 8192 tokens,
-//   32 requests: 85, where mma.sync, for which every warp converts what it reads, took 148.
+//   up to 16 rows, bf16: mma.sync.  16 requests of 8192 tokens, 16 rows of 128: 80 us, tokens along the lanes of tensor memory 93; one of 540 tokens, 4 rows: 11.0 and 15.8.
+//   up to 32 rows, bf16, and no more items of two tiles each than SMs: mma.sync.  It starts, changes an item and ends in less time, and cuts a long item into smaller pieces; with many
+//   items the products in two tiles cost more.  Requests of 60 to 8000 tokens, heads of 64 and 128, 20 or 32 rows: up to 16 items of a kv head it takes 0.72 to 0.87 of the time with the
+//   tokens along the lanes on average (one request, 8 kv heads, 20 rows over 540 tokens 12.7 and 16.2 us, over 8000 22 and 32; 2 kv heads, 32 rows over 8000 20 and 50), from 33 to 64 0.91
+//   (20 rows) and 0.98 (32; eight requests over 540 tokens 20.0 and 20.9, over 4000 47 and 43), with 256 0.92 and 1.08 (32 requests over 540 tokens, 32 rows: 54 and 49).
+//   up to 64 rows: tokens along the lanes.  16 requests of 8192 tokens, bf16, 40 or 64 rows of 128: 92 and 94 us, in tiles of 128 rows 106 and 110; e4m3, 4 rows over 8192 tokens,
+//   32 requests: 84, where mma.sync, for which every warp converted what it read, took 148.
 //   more, bf16: tiles of 128 rows.
 //   more, e4m3: tokens along the lanes, in tiles of 64 rows (see paged_tree_sm100.cu).
 struct Choice { int tile_rows, unit, parts; };
 Choice choose(int rows, bool q8, long long heads) {
-    if (!q8 && (rows <= ROWS || (rows <= 2 * ROWS && heads <= sm_count() / 2 / 2))) return {ROWS, PAGE, 1};
+    if (!q8 && (rows <= ROWS || (rows <= 2 * ROWS && 2 * heads <= sm_count()))) return {ROWS, PAGE, 1};
     if (rows > 64) return q8 ? Choice{64, 128, 1} : Choice{128, 128, 2};
     if (rows <= 16) return {16, 128, 2};
     return {rows <= 32 ? 32 : 64, 128, rows <= 32 ? 2 : 1};

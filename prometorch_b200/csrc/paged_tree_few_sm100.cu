@@ -19,10 +19,12 @@
 // parts' smallest step is 2^-16: at most 2^-17, 2^-28 of an item's largest weights, is lost of a small one.  Parts are columns of their own, of scores
 // and of accumulators, so that a page is read once.
 //
+// bf16: weights become two bf16 parts, themselves rounded and what that leaves, columns of their own as well; 2^-18 of a weight is lost.
+//
 // What bounds it.  Shared memory takes 128 bytes a cycle, and a product of few columns costs what its 4 KB of keys or values take (measured 42 cycles alone).  bf16: pages 64 KB written and
-// 64 KB read, weights and queries 24 KB: 1250 cycles a block of 128 elements, of the 2100 that the SM's share of the memory takes.  e4m3: 32 + 32 KB, and 32 KB for the parts,
-// 750 cycles of 1050.  Measured are 1300 with 16 rows (the chain of waits of the warp that issues the products), 1500 with 32 and 2400 with 64 (the softmax's): 32 requests of 8192 tokens,
-// 4 rows, 85 us, 74 % of the copy rate.  Values converted to fp16, the fp16 product and the two parts of queries one after the other took 148.
+// 64 KB read, weights (two parts) and queries 40 KB (64 rows: 80): 1340 (1660) cycles a block of 128 elements, of the 2100
+// that the SM's share of the memory takes.  e4m3: 32 + 32 KB, and 32 KB for the parts, 750 cycles of 1050.  Measured are 1300 with 16 rows (the chain of waits of the warp that issues the products), 1500 with 32 and 2400 with 64 (the softmax's): e4m3, 32 requests of 8192 tokens,
+// 4 rows, 84 us, 74 % of the copy rate.  Values converted to fp16, the fp16 product and the two parts of queries one after the other took 148.
 #include "paged_tree_sm100.cuh"
 
 int ptb_make_tmap_64b(CUtensorMap* map, const void* base, long long rows, int box_rows);

@@ -608,7 +608,7 @@ def test_keep_of_many_layers(kind, layers):
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T,G", [(5, 4), (8, 4), (17, 1), (32, 1), (10, 4), (40, 3)])
-@pytest.mark.parametrize("B", [18, 19, 60])
+@pytest.mark.parametrize("B", [37, 38, 60])
 def test_strange_requests_beside_others(kind, D, T, G, B):
     """In one batch, on both sides of the number of requests that another kernel takes 17 to 32 rows from: a masked token that is no number, a masked large one, a page that is none of the pool's,
     a query that is no number, requests without nodes and without cached tokens, a page table with far more room than the requests need."""
