@@ -405,6 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                         float down = 0.f, a = 1.f;
                         if (mx > (known ? GROW + UP : -INFINITY)) {
                             down = UP - mx;
+                            if (mx + down > UP) down = -mx;          // from 2^27 on UP may be rounded up, at an ulp of 16 beyond what fp16 holds
                             a = known ? exp2f(down) : 0.f;
                             nr[tid] += down;
                             known = true;

@@ -655,3 +655,30 @@ def test_strange_requests_beside_others(kind, D, T, G, B):
     close(got, want, mag, kind)
     for b, n in enumerate(nodes):
         assert not got[b, n:].any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [(1, 4), (8, 4), (16, 4), (40, 4)])
+@pytest.mark.parametrize("size", [-40, 20, 34, 36, 37, 38, 39, 40, 41, 42, 44, 60, 100, 118])
+def test_queries_of_any_size(kind, D, T, G, size):
+    """Up to 2^118 times the ordinary: the token with the largest score has all the weight.  No two tokens' scores are within fp32's reach of one another (a column of keys that grows by a quarter from
+    token to token, in any order, decides, against others of at most 2^-10 of it)."""
+    Hk, have = 2, 30
+    H = Hk * G
+    g = gen(T + D)
+    table, n_pages = table_for([have + T], 2)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    at = torch.arange(have + T, device=DEV)
+    x = torch.randn(have + T, Hk, D, device=DEV, generator=g) * 2.0 ** -10
+    x[:, :, 3] = 1.25 ** at[torch.randperm(have + T, device=DEV, generator=g)].float()[:, None] * 2.0 ** -20
+    R.paged_write(torch.cat([x.flatten(1), torch.randn(have + T, Hk * D, device=DEV, generator=g)], 1).bfloat16(), 0, Hk, D, at.int(), torch.zeros_like(at).int(), table, torch.ones(have + T, D // 2, device=DEV),
+                  torch.zeros(have + T, D // 2, device=DEV), k, v, k_exp=ke, v_exp=ve)
+    q = torch.randn(1, T, H * D, device=DEV, generator=g) * 2.0 ** -12
+    q[..., 3::D] = 1.0
+    q = (q * 2.0 ** size).bfloat16()
+    assert torch.isfinite(q).all()
+    lens = torch.tensor([have], dtype=torch.int32, device=DEV)
+    got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, [have], [T], None, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
