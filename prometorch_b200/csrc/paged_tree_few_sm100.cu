@@ -374,15 +374,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                         const float4 m = *reinterpret_cast<const float4*>(nr + i);
                         uint64_t a = pair(__float_as_uint(m.x), __float_as_uint(m.y)), b = pair(__float_as_uint(m.z), __float_as_uint(m.w));
                         if constexpr (Q8) { a = add2(a, e2); b = add2(b, e2); }
-                        uint64_t s0 = pair(r[i], r[i + 1]), s1 = pair(r[i + 2], r[i + 3]);
+                        uint64_t s0 = pair(r[i], r[i + 1]), s1 = pair(r[i + 2], r[i + 3]), f0 = g2, f1 = g2;
                         if constexpr (Q8) {
                             const float4 f = *reinterpret_cast<const float4*>(fac + i);
-                            s0 = mul2(s0, pair(__float_as_uint(f.x), __float_as_uint(f.y)));
-                            s1 = mul2(s1, pair(__float_as_uint(f.z), __float_as_uint(f.w)));
+                            s0 = mul2(s0, g2);           // the token's scale first: a row's may be as large as bf16 goes, and only with it is the product the score's size
+                            s1 = mul2(s1, g2);
+                            f0 = pair(__float_as_uint(f.x), __float_as_uint(f.y));
+                            f1 = pair(__float_as_uint(f.z), __float_as_uint(f.w));
                         }
                         float x[4];
-                        apart(fma2(s0, g2, a), x[0], x[1]);
-                        apart(fma2(s1, g2, b), x[2], x[3]);
+                        apart(fma2(s0, f0, a), x[0], x[1]);
+                        apart(fma2(s1, f1, b), x[2], x[3]);
                         m2[0] = max3(m2[0], x[0], x[1]);
                         m2[1] = max3(m2[1], x[2], x[3]);
 #pragma unroll

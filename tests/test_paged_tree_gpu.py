@@ -682,3 +682,25 @@ def test_queries_of_any_size(kind, D, T, G, size):
     got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, k_exp=ke, v_exp=ve)
     want, mag = oracle(q, H, Hk, D, [have], [T], None, table, k, v, ke, ve, D ** -0.5)
     close(got, want, mag, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [(1, 4), (8, 4), (16, 4), (40, 4)])
+@pytest.mark.parametrize("size,keys", [(40, 0), (112, 0), (118, 0), (100, -30), (118, -30), (60, 50)])
+def test_queries_large_in_every_column(kind, D, T, G, size, keys):
+    """As above with all columns alike: a score is the sum of all, D times one of them, and below 2^127."""
+    Hk, have = 2, 30
+    H = Hk * G
+    g = gen(T + D)
+    table, n_pages = table_for([have + T], 2)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    at = torch.arange(have + T, device=DEV)
+    x = torch.ones(have + T, Hk, D, device=DEV) * 1.25 ** -at[torch.randperm(have + T, device=DEV, generator=g)].float()[:, None, None] * 2.0 ** keys
+    R.paged_write(torch.cat([x.flatten(1), torch.randn(have + T, Hk * D, device=DEV, generator=g)], 1).bfloat16(), 0, Hk, D, at.int(), torch.zeros_like(at).int(), table, torch.ones(have + T, D // 2, device=DEV),
+                  torch.zeros(have + T, D // 2, device=DEV), k, v, k_exp=ke, v_exp=ve)
+    q = torch.full((1, T, H * D), 2.0 ** size, device=DEV).bfloat16()
+    lens = torch.tensor([have], dtype=torch.int32, device=DEV)
+    got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, [have], [T], None, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
