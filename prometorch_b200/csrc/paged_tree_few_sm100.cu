@@ -14,10 +14,10 @@
 //
 // e4m3: both products have 8-bit operands, and nothing is converted but what the kernel makes itself.  Queries become two e4m3 parts, q = q1 + q2: four bits and the next four
 // are what bf16 has; a row is scaled by a power of two, so that its largest element lies in [2^7, 2^8), the smallest step of a part is 2^-9, 2^-17 of that.  A token's
-// exponents scale its scores, and its weights: p' = 2^(s + e_v), of which the sum takes 2^-e_v.  Weights are rounded to fp16, and become
-// three e5m2 parts, which are top bytes of fp16: a part to nearest leaves at most an eighth of its power of two, with a sign, so that p = p1 + p2 + p3 has all eleven bits.  The
-// parts' smallest step is 2^-16: at most 2^-17, 2^-28 of an item's largest weights, is lost of a small one.  Parts are columns of their own, of scores
-// and of accumulators, so that a page is read once.
+// exponents scale its scores, and its weights: p' = 2^(s + e_v), of which the sum takes 2^-e_v (exponents of a row's values may be 100 apart: the sum of those with the least then still
+// has its place below one with the largest; zeros have the least there is, -64).  Weights are rounded to fp16, and become three e5m2 parts, which are top bytes of fp16: a part to nearest
+// leaves at most an eighth of its power of two, with a sign, so that p = p1 + p2 + p3 has all eleven bits.  The parts' smallest step is 2^-16: at most 2^-17, 2^-28 of an item's largest
+// weights, is lost of a small one.  Parts are columns of their own, of scores and of accumulators, so that a page is read once.
 //
 // bf16: weights become two bf16 parts, themselves rounded and what that leaves, columns of their own as well; 2^-18 of a weight is lost.
 //

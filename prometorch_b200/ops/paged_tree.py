@@ -6,7 +6,7 @@
 
 Quantised pages are :data:`E4M3` tensors ``[page, kv_head, 64, D]`` with one byte ``[page, kv_head, 64]`` for a token's keys (and one for its values) of a head: the
 values stand for ``value * 2^(byte - 127)``.  The exponent is the least with ``max |x| <= 448 * 2^e``, between -64 and 64; larger magnitudes are stored as the largest,
-infinities and NaN as NaN.
+infinities and NaN as NaN.  Attention holds for values whose exponents lie up to 100 apart (those of zeros are -64: for values up to 2^44 beside zeros).
 
 CUDA tensors go through csrc/paged_write.cu and csrc/paged_tree.cu; CPU tensors take the plain torch form below.  A kernel that meets a page id or a
 slot outside its extent skips the access and reports it: ``ops.paged.check_status`` raises."""

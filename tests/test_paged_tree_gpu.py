@@ -704,3 +704,26 @@ def test_queries_large_in_every_column(kind, D, T, G, size, keys):
     got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, k_exp=ke, v_exp=ve)
     want, mag = oracle(q, H, Hk, D, [have], [T], None, table, k, v, ke, ve, D ** -0.5)
     close(got, want, mag, kind)
+
+
+@pytest.mark.parametrize("T", [1, 5, 12, 48])
+@pytest.mark.parametrize("n", [500, 5000])
+@pytest.mark.parametrize("where", [0, 250, -1])
+def test_exponents_of_values_a_hundred_apart(T, n, where):
+    """One token's values of 2^44, zeros (which have the least exponent) in whole pages and among others, values of ordinary size: the sums hold, within an item and where it is cut.  Scores of
+    twelve terms' size in fp32 as in `close`, three times as large: 2^-8 in place of 2^-11 covers it."""
+    D, H, Hk = 128, 4, 2
+    g = gen(T + n)
+    table, n_pages = table_for([n + T], 1)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, "e4m3")
+    zero = torch.rand(n_pages, Hk, PAGE, device=DEV, generator=g) < 0.3
+    zero[table[0, 3:6].long()] = True
+    v.view(torch.uint8)[zero], ve[zero] = 0, 63
+    at = where % n
+    page = int(table[0, at // PAGE])
+    v[page, :, at % PAGE] = torch.full((D,), 256.0, device=DEV).to(R.E4M3)
+    ve[page, :, at % PAGE] = 127 + 36
+    q = torch.randn(1, T, H * D, device=DEV, generator=g).bfloat16() * 3
+    got = R.paged_attention_tree(q, H, Hk, D, torch.tensor([n], dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, [n], [T], None, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, "bf16")
