@@ -64,6 +64,15 @@ __device__ __forceinline__ constexpr int v_elem(int t, int n) { return (t / 8) *
 // Pieces of an item's part that have tokens.
 __device__ __forceinline__ int pieces_of(const Item& it) { return min(it.n * PIECES, (it.r.len + it.r.nodes - it.first * PAGE + PIECE - 1) / PIECE); }
 
+// Piece `count` of a warp's ring.  Where the wait runs out, the pieces behind it that are on their way are waited for as well: nobody leaves while copies arrive in its shared memory.
+template <int STAGES>
+__device__ __noinline__ bool wait_or_drain(uint64_t* full, int count, int* status) {
+    bool ok = mbar_wait(&full[count % STAGES], (uint32_t)((count / STAGES) & 1), status);
+    if (!ok)
+        for (int k = count; k < count + STAGES; ++k) mbar_wait(&full[k % STAGES], (uint32_t)((k / STAGES) & 1), status);
+    return ok;
+}
+
 // What a warp still has to fetch: its pieces of the run, one after another, across items.
 struct Fetch {
     int u, piece, ids_from, kvh, n, pieces, row, ids;    // ids: this lane's page id, of the warp's pages from ids_from on; row: first entry of the item's pages in the table
@@ -181,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_kernel(const __grid_con
 #pragma unroll 1
         for (int piece = warp; piece < pieces; piece += WARPS, ++count) {
             const int s = count % Ge::STAGES, first = it.first * PAGE + piece * PIECE;       // first: the piece's first token
-            if (ok) ok = mbar_wait(&full[s], (uint32_t)((count / Ge::STAGES) & 1), P.status);
+            if (ok && !mbar_try_wait(&full[s], (uint32_t)((count / Ge::STAGES) & 1))) ok = wait_or_drain<Ge::STAGES>(full, count, P.status);
             if (ok && !((bad >> s) & 1)) {
                 const uint8_t *sk = ring + s * Ge::STAGE, *sv = sk + Ge::BYTES;
                 const bool tail = first + PIECE > len;   // some of its tokens are drafted, or lie behind the last

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
         regs_dec<REGS_OTHER>();                          // one instruction for the warp group
         if (warp == 0) {
             // -------------------------------------------------------------------------------- pages
-            int n = 0;                                   // block of the run
+            int n = 0, sent_v = 0;                       // block of the run; blocks whose values are on their way or there
             if (u0 < u1) asm volatile("bar.sync 5, 160;" ::: "memory");          // the first queries go before the first pages, behind which they would wait
             for (int u = u0; u < u1 && ok;) {
                 const Item it = item_at(P, starts, u, u1);
@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                             if (ok) {
                                 mbar_expect_tx(&v_full[sV], there * (S::TILE / 2));
                                 for (int x = 0; x < there; ++x) page_to(sv + sV * S::TILE, &tmV, x, &v_full[sV]);
+                                sent_v = n + 1;
                             }
                         }
                     }
@@ -235,7 +236,10 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_few_kernel(const __grid
                 }
                 u += it.n;
             }
-            if (!ok) *abort_flag = 1;
+            if (!ok) {
+                *abort_flag = 1;
+                if (lane == 0) drain<NK, NV>(k_full, v_full, n, sent_v, P.status);
+            }
         } else if (warp == 1) {
             // -------------------------------------------------------------------------------- products
             constexpr uint32_t id_s = idesc<Q8>(S::S_COLS, 0, 0);                            // e4m3 has the number that fp16 has

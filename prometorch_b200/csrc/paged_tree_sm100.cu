@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
         regs_dec<REGS_OTHER>();                          // one instruction for the warp group
         if (warp == 0) {
             // ------------------------------------------------------------------------------------ pages
-            int n = 0;                                       // block of the run
+            int n = 0, sent_v = 0;                           // block of the run; blocks whose values are on their way or there
             for (int u = u0; u < u1 && ok;) {
                 const Item it = item_at(P, starts, u, u1);
                 const int pages = (it.r.len + it.r.nodes + PAGE - 1) / PAGE;
@@ -126,13 +126,17 @@ __global__ void __launch_bounds__(THREADS, 1) paged_tree_tiles_kernel(const __gr
                             for (int x = 0; x < there; ++x)
                                 for (int c = 0; c < D / 64; ++c)
                                     tma_load_2d(sv + sV * S::TILE + (x * (D / 64) + c) * 8192, &tmV, c * 64, (max(page[x], 0) * P.Hk + it.kvh) * PAGE, &v_full[sV]);
+                            sent_v = n + 1;
                         }
                     }
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0);
                 }
                 u += it.n;
             }
-            if (!ok) *abort_flag = 1;
+            if (!ok) {
+                *abort_flag = 1;
+                if (lane == 0) drain<NK, NV>(k_full, v_full, n, sent_v, P.status);
+            }
         } else if (warp == 1) {
             // ------------------------------------------------------------------------------------ products
             if (lane == 0) {

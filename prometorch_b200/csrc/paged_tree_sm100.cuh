@@ -57,6 +57,14 @@ __device__ __forceinline__ uint32_t visible32(unsigned long long seen, int d0) {
     if (d0 <= -32) return ~0u;
     return ((1u << -d0) - 1) | (uint32_t)(seen << -d0);
 }
+// A wait ran out, in the block before `blocks`, the loader's last: nobody leaves while copies are on their way into its shared memory.  That block's values were perhaps not sent for (its
+// keys neither: their wait is over at once, or runs out as well).
+template <int NK, int NV>
+__device__ __noinline__ void drain(uint64_t* k_full, uint64_t* v_full, int blocks, int sent_v, int* status) {
+    for (int n = max(0, blocks - NK); n < blocks; ++n) mbar_wait(&k_full[n % NK], (uint32_t)((n / NK) & 1), status);
+    for (int n = max(0, sent_v - NV); n < sent_v; ++n) mbar_wait(&v_full[n % NV], (uint32_t)((n / NV) & 1), status);
+}
+
 // 2^e, for e kept in the range of a normal number.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
 
