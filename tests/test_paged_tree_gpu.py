@@ -727,3 +727,25 @@ def test_exponents_of_values_a_hundred_apart(T, n, where):
     got = R.paged_attention_tree(q, H, Hk, D, torch.tensor([n], dtype=torch.int32, device=DEV), table, k, v, k_exp=ke, v_exp=ve)
     want, mag = oracle(q, H, Hk, D, [n], [T], None, table, k, v, ke, ve, D ** -0.5)
     close(got, want, mag, "bf16")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hk,T", [(64, 1, 3), (71, 1, 5), (130, 1, 2), (192, 2, 64), (63, 1, 7), (65, 1, 1), (33, 1, 2)])
+def test_large_groups(kind, D, H, Hk, T):
+    """Up to hundreds of heads of a kv head: a node's heads over several tiles, tiles that begin inside a node."""
+    g = gen(H + T)
+    have, nodes = [0, 77, 300], [T, max(1, T - 1), T]
+    table, n_pages = table_for([n + T for n in have], 3)
+    k, v, ke, ve = pools(g, n_pages, Hk, D, kind)
+    behind = [n + t for n, t in zip(have, nodes)]
+    spoil(k, ke, table, behind, math.nan)
+    spoil(v, ve, table, behind, math.inf)
+    mask = random_masks(T, 3, T)
+    q = torch.randn(3, T, H * D, device=DEV, generator=g).bfloat16()
+    lens, nd = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (have, nodes))
+    got = R.paged_attention_tree(q, H, Hk, D, lens, table, k, v, mask=mask.to(DEV), nodes=nd, k_exp=ke, v_exp=ve)
+    want, mag = oracle(q, H, Hk, D, have, nodes, mask, table, k, v, ke, ve, D ** -0.5)
+    close(got, want, mag, kind)
+    for b, n in enumerate(nodes):
+        assert not got[b, n:].any()
