@@ -9,7 +9,7 @@
 // be any head element, so lane r holds one 16-byte piece of a value row for all tiles.  Which of eight tokens lane r takes (`token_of`) is chosen so
 // that the eight lanes of a quarter warp fall on the eight 16-byte columns of the swizzled rows, for keys and for values.
 //
-// A weight is two bf16, itself rounded and what that leaves (2^-18 of it is lost), each a product of its own; scores, maxima, sums and accumulators are fp32.
+// A weight is two bf16, itself rounded and what that leaves (at most 2^-16 of it is lost), each a product of its own; scores, maxima, sums and accumulators are fp32.
 #include "paged_tree.cuh"
 
 namespace ptb {

@@ -19,7 +19,7 @@
 // leaves at most an eighth of its power of two, with a sign, so that p = p1 + p2 + p3 has all eleven bits.  The parts' smallest step is 2^-16: at most 2^-17, 2^-28 of an item's largest
 // weights, is lost of a small one.  Parts are columns of their own, of scores and of accumulators, so that a page is read once.
 //
-// bf16: weights become two bf16 parts, themselves rounded and what that leaves, columns of their own as well; 2^-18 of a weight is lost.
+// bf16: weights become two bf16 parts, themselves rounded and what that leaves, columns of their own as well; at most 2^-16 of a weight is lost.
 //
 // What bounds it.  Shared memory takes 128 bytes a cycle, and a product of few columns costs what its 4 KB of keys or values take (measured 42 cycles alone).  bf16: pages 64 KB written and
 // 64 KB read, weights (two parts) and queries 40 KB (64 rows: 80): 1340 (1660) cycles a block of 128 elements, of the 2100

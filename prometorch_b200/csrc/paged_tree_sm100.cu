@@ -7,12 +7,12 @@
 //               own: while one group works on its scores the tensor cores work for the other.  A thread owns a row, so nothing is exchanged.  Weights go back to
 //               tensor memory, over the scores they came from, as the first operand of the second product.  The accumulator is scaled, by its own threads, only
 //               when a row's maximum has grown by 2^8;
-//   warps 12-15 of a block with drafted tokens they clear the values that must not meet a weight.
+//   warps 12-15 clear the values that must not meet a weight: of drafted tokens, behind the last token, and of pages that are none of the pool's.
 //
 // What bounds it: the cache's bytes up to 128 rows (a block of 128 keys of 128 elements is 64 KB and takes an SM's share of the memory 1.5 us; exponentials, products and
 // softmax instructions take about 0.6 us each, side by side); with more tiles of rows, which fetch the pages again, the products and exponentials.
 //
-// Weights are rounded to bf16 (by up to 2^-9, without a bias; their sums are of the unrounded ones): the result is off by 2.3e-3 of its norm where rounding the output alone leaves 1.65e-3.
+// Weights are rounded to bf16 (by up to 2^-8, without a bias; their sums are of the unrounded ones): the result is off by 2.3e-3 of its norm where rounding the output alone leaves 1.65e-3.
 // With what the rounding leaves as a second operand, as the kernels for fewer rows have it, it is 1.65e-3, and 8 trees of 64 over 8191 tokens, 512 rows of 64, take 96 us in place of 66
 // (256 rows of 128: 82 and 68), for the softmax's instructions and for the products alike.
 //

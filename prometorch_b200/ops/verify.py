@@ -17,7 +17,7 @@ from .. import _native as N
 from .paged_tree import _index, _launch
 
 MAX_NODES = 64
-MAX_ROWS, MAX_VOCAB = 65536, 442368          # on the GPU: nodes of a batch, tokens that a cluster's shared memory holds
+MAX_VOCAB = 442368          # on the GPU: what a cluster's shared memory holds
 MAX_TEMPERATURE = 2.0 ** 126
 
 
